@@ -330,12 +330,16 @@ def _plain_rows(s):
 
 # ---- one pass through the framework -----------------------------------------------------------
 
+_binding = None
+
+
 def _capi():
-    root = str(Path(__file__).resolve().parent.parent / "hypermoe-engine_amd")
-    if root not in sys.path:
-        sys.path.insert(0, root)
-    from hmoe import capi
-    return capi
+    global _binding
+    if _binding is None:
+        sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "hypermoe-engine_amd"))
+        from hmoe import capi
+        _binding = capi
+    return _binding
 
 
 def _own_quantize(s, capi, stream):
