@@ -1,0 +1,223 @@
+// hm_fp8_quantize.hip -- rows and weight blocks to block-scaled e4m3 (hm_fp8.h).
+//
+// Memory bound: every value is read once and stays in registers between its block's maximum and its
+// conversion.
+//   rows, contiguous columns   16 lanes hold one block, 8 values each; the maximum goes over the lanes
+//                              by DPP, the 8 bytes of a lane are one store
+//   blocks of 128 rows         one workgroup a block, 4 rows x 8 columns a lane
+//   contiguous rows            (a transposed operand: column k of the output row r at x[k ld + r]) a
+//                              lane walks one row's k, so that a wave's loads are contiguous in r and
+//                              nothing is transposed through the LDS; four waves share a block's k
+#include "hm_fp8.h"
+
+#include <limits.h>
+
+namespace {
+
+constexpr int kQThreads = 256;
+
+// 8 consecutive values from p (VEC: 16-byte loads), zeros from column `left` on.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* __restrict__ p, int64_t left, float (&v)[8]) {
+    if (VEC && left >= 8) {
+        constexpr int N = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 8 / N; ++i) {
+            const hm_pack<T, N> w = reinterpret_cast<const hm_pack<T, N>*>(p)[i];
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[i * N + j] = (float)w.v[j];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? (float)p[i] : 0.0f;
+    }
+}
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(kQThreads) void f8_quantize_rows_kernel(
+    const T* __restrict__ x, int64_t rows, int64_t width, int64_t stride, uint8_t* __restrict__ q,
+    float* __restrict__ scale) {
+    const int64_t nb = hm_f8_blocks(width);
+    const int64_t g = (int64_t)blockIdx.x * (kQThreads / 16) + (threadIdx.x >> 4);
+    const bool live = g < rows * nb;
+    const int64_t gg = live ? g : 0;
+    const int64_t r = gg / nb, kb = gg - r * nb;
+    const int c = 8 * (threadIdx.x & 15);
+    const int64_t k = kb * kF8Block + c;
+    float v[8];
+    load8<T, VEC>(x + r * stride + k, width - k, v);
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = hm_f8_amax(amax, v[i]);
+    amax = hm_row16_max(amax);
+    const hm_f8_scaler s = hm_f8_scaler_of(amax);
+    if (!live) return;
+    uint2 w;
+    w.x = hm_f8_pack4(s, v[0], v[1], v[2], v[3]);
+    w.y = hm_f8_pack4(s, v[4], v[5], v[6], v[7]);
+    *reinterpret_cast<uint2*>(q + (r * nb + kb) * kF8Block + c) = w;
+    if ((threadIdx.x & 15) == 0) scale[r * nb + kb] = s.scale;
+}
+
+// The maximum over a workgroup of `waves` waves; every thread gets it.
+__device__ __forceinline__ float block_max(float v, float* s_max, int waves) {
+    v = hm_wave_max_dpp(v);
+    if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float m = s_max[0];
+    for (int i = 1; i < waves; ++i) m = fmaxf(m, s_max[i]);
+    return m;
+}
+
+// Block (blockIdx.y, blockIdx.x) of 128 rows x 128 columns, columns contiguous.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(512) void f8_quantize_blocks_kernel(
+    const T* __restrict__ x, int64_t rows, int64_t width, int64_t stride, uint8_t* __restrict__ q,
+    float* __restrict__ scale) {
+    __shared__ float s_max[8];
+    const int64_t nb = hm_f8_blocks(width);
+    const int64_t kb = blockIdx.x, rb = blockIdx.y;
+    const int c = 8 * (threadIdx.x & 15);
+    const int64_t k = kb * kF8Block + c;
+    const int64_t r0 = rb * kF8Block + (threadIdx.x >> 4);
+    float v[4][8];
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = r0 + 32 * i;
+        if (r < rows) {
+            load8<T, VEC>(x + r * stride + k, width - k, v[i]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = hm_f8_amax(amax, v[i][j]);
+    }
+    const hm_f8_scaler s = hm_f8_scaler_of(block_max(amax, s_max, 8));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = r0 + 32 * i;
+        if (r >= rows) break;
+        uint2 w;
+        w.x = hm_f8_pack4(s, v[i][0], v[i][1], v[i][2], v[i][3]);
+        w.y = hm_f8_pack4(s, v[i][4], v[i][5], v[i][6], v[i][7]);
+        *reinterpret_cast<uint2*>(q + (r * nb + kb) * kF8Block + c) = w;
+    }
+    if (threadIdx.x == 0) scale[rb * nb + kb] = s.scale;
+}
+
+// Contiguous rows: x[k ld + r].  A workgroup takes 64 RH rows (RH = 1: a scale for each row, 2: one
+// for the 128 x 128 block) x 128 columns, wave w the rows 64 (w / 4) .. and the columns 32 (w % 4) ...
+template <typename T, int RH>
+__global__ __launch_bounds__(256 * RH) void f8_quantize_transposed_kernel(
+    const T* __restrict__ x, int64_t rows, int64_t width, int64_t ld, uint8_t* __restrict__ q,
+    float* __restrict__ scale) {
+    __shared__ float s_max[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave & 3;
+    const int64_t nb = hm_f8_blocks(width);
+    const int64_t kb = blockIdx.x;
+    const int64_t r = (int64_t)blockIdx.y * (64 * RH) + 64 * (wave >> 2) + lane;
+    const int64_t k0 = kb * kF8Block + 32 * part;
+    const T* p = x + k0 * ld + r;
+    float v[32];
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = r < rows && k0 + i < width ? (float)p[(int64_t)i * ld] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) amax = hm_f8_amax(amax, v[i]);
+    if constexpr (RH == 1) {
+        s_max[part][lane] = amax;
+        __syncthreads();
+        amax = fmaxf(fmaxf(s_max[0][lane], s_max[1][lane]), fmaxf(s_max[2][lane], s_max[3][lane]));
+    } else {
+        amax = block_max(amax, s_max[0], 4 * RH);
+    }
+    const hm_f8_scaler s = hm_f8_scaler_of(amax);
+    if (r < rows) {
+        uint4* to = reinterpret_cast<uint4*>(q + (r * nb + kb) * kF8Block + 32 * part);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint4 w;
+            w.x = hm_f8_pack4(s, v[16 * h], v[16 * h + 1], v[16 * h + 2], v[16 * h + 3]);
+            w.y = hm_f8_pack4(s, v[16 * h + 4], v[16 * h + 5], v[16 * h + 6], v[16 * h + 7]);
+            w.z = hm_f8_pack4(s, v[16 * h + 8], v[16 * h + 9], v[16 * h + 10], v[16 * h + 11]);
+            w.w = hm_f8_pack4(s, v[16 * h + 12], v[16 * h + 13], v[16 * h + 14], v[16 * h + 15]);
+            to[h] = w;
+        }
+        if constexpr (RH == 1) {
+            if (part == 0) scale[r * nb + kb] = s.scale;
+        }
+    }
+    if constexpr (RH == 2) {
+        if (threadIdx.x == 0) scale[blockIdx.y * nb + kb] = s.scale;
+    }
+}
+
+template <typename T>
+int launch_quantize(const T* x, int64_t rows, int64_t width, int64_t row_stride, int64_t col_stride,
+                    int32_t block_rows, uint8_t* q, float* scale, hipStream_t s) {
+    const int64_t nb = hm_f8_blocks(width);
+    if (col_stride == 1) {
+        const bool vec = (uintptr_t)x % 16 == 0 && row_stride % (16 / (int64_t)sizeof(T)) == 0;
+        if (block_rows == 1) {
+            const int64_t grid = (rows * nb + kQThreads / 16 - 1) / (kQThreads / 16);
+            if (grid > INT_MAX / kQThreads) return HM_ERR_OVERFLOW;
+            hipLaunchKernelGGL((vec ? f8_quantize_rows_kernel<T, true> : f8_quantize_rows_kernel<T, false>),
+                               dim3((unsigned)grid), dim3(kQThreads), 0, s, x, rows, width, row_stride,
+                               q, scale);
+        } else {
+            const int64_t rb = hm_f8_blocks(rows);
+            if (rb > 65535 || nb > INT_MAX / 512) return HM_ERR_OVERFLOW;
+            hipLaunchKernelGGL((vec ? f8_quantize_blocks_kernel<T, true> : f8_quantize_blocks_kernel<T, false>),
+                               dim3((unsigned)nb, (unsigned)rb), dim3(512), 0, s, x, rows, width,
+                               row_stride, q, scale);
+        }
+    } else {
+        const int per = block_rows == 1 ? 64 : 128;
+        const int64_t rb = (rows + per - 1) / per;
+        if (rb > 65535 || nb > INT_MAX / 512) return HM_ERR_OVERFLOW;
+        const dim3 grid((unsigned)nb, (unsigned)rb);
+        if (block_rows == 1)
+            hipLaunchKernelGGL((f8_quantize_transposed_kernel<T, 1>), grid, dim3(256), 0, s, x, rows,
+                               width, col_stride, q, scale);
+        else
+            hipLaunchKernelGGL((f8_quantize_transposed_kernel<T, 2>), grid, dim3(512), 0, s, x, rows,
+                               width, col_stride, q, scale);
+    }
+    HM_LAUNCHED();
+    return HM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t hm_fp8_pitch(int64_t width) { return width > 0 ? hm_f8_pitch(width) : 0; }
+
+int hm_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t width, int64_t row_stride,
+                    int64_t col_stride, int32_t block_rows, uint8_t* q, float* scale, void* stream) {
+    HM_REQUIRE(x && q && scale && rows >= 0 && width > 0);
+    HM_REQUIRE(hm_row_dtype(dtype) && (block_rows == 1 || block_rows == kF8Block));
+    HM_REQUIRE((uintptr_t)x % hm_row_dtype_size(dtype) == 0 && (uintptr_t)q % 16 == 0 &&
+               (uintptr_t)scale % 4 == 0);
+    HM_REQUIRE(row_stride > 0 && col_stride > 0 && (row_stride == 1 || col_stride == 1));
+    if (rows == 0) return HM_OK;
+    if (rows > (int64_t)1 << 40 || width > (int64_t)1 << 31 ||
+        rows > INT64_MAX / 8 / row_stride || width > INT64_MAX / 8 / col_stride)
+        return HM_ERR_OVERFLOW;
+    hipStream_t s = hm_stream(stream);
+    switch (dtype) {
+    case HM_DTYPE_FP32:
+        return launch_quantize(static_cast<const float*>(x), rows, width, row_stride, col_stride,
+                               block_rows, q, scale, s);
+    case HM_DTYPE_FP16:
+        return launch_quantize(static_cast<const hm_f16*>(x), rows, width, row_stride, col_stride,
+                               block_rows, q, scale, s);
+    default:
+        return launch_quantize(static_cast<const hm_bf16*>(x), rows, width, row_stride, col_stride,
+                               block_rows, q, scale, s);
+    }
+}
+
+}  // extern "C"

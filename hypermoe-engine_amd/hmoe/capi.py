@@ -20,7 +20,8 @@ HM_EXEC_SPLIT_K = 0x800
 HM_GEMV_MAX_TOKENS = 16
 HM_GEMV_MAX_PAIRS = 64
 HM_EXEC_ROUTE_SEQUENTIAL = 0x400
-HM_DTYPE_FP32, HM_DTYPE_INT8 = 0, 3
+HM_DTYPE_FP32, HM_DTYPE_FP16, HM_DTYPE_BF16, HM_DTYPE_INT8, HM_DTYPE_FP8 = 0, 1, 2, 3, 4
+HM_FP8_BLOCK = 128
 
 
 class HmLayer(C.Structure):
@@ -93,6 +94,16 @@ SIGNATURES = {
                                      c_u32, c_i32, c_i32, C.POINTER(HmBlockIO), vp, c_sz, vp]),
     "hm_limb_quantize_rows": (c_i32, [vp, c_i64, c_i64, c_i32, vp, vp, vp]),
     "hm_limb_partials": (c_i32, [vp, c_i64, c_i64, c_i32, vp, c_i32, c_i64, vp, vp]),
+    "hm_fp8_pitch": (c_i64, [c_i64]),
+    "hm_fp8_quantize": (c_i32, [vp, c_i32, c_i64, c_i64, c_i64, c_i64, c_i32, vp, vp, vp]),
+    "hm_fp8_matmul": (c_i32, [vp, vp, vp, vp, c_i32, c_i64, c_i64, c_i64, vp, c_i32, vp]),
+    "hm_fp8_experts_workspace_bytes": (c_sz, [C.POINTER(HmLayer), c_i64, c_i64]),
+    "hm_fp8_experts": (c_i32, [C.POINTER(HmLayer), vp, c_i32, c_i64, vp, vp, c_i64, vp, c_i32, vp,
+                               c_sz, vp]),
+    "hm_dispatch_rows": (c_i32, [vp, vp, vp, c_i64, c_i32, c_i64, c_i64, c_i32, vp, vp]),
+    "hm_dispatch_rows_grad": (c_i32, [vp, vp, vp, vp, c_i64, c_i32, c_i64, c_i64, c_i32, vp, vp, vp]),
+    "hm_combine_rows": (c_i32, [vp, vp, vp, vp, c_i64, c_i32, c_i64, c_i64, c_i32, vp, vp]),
+    "hm_combine_rows_grad": (c_i32, [vp, vp, vp, vp, c_i64, c_i32, c_i64, c_i64, c_i32, vp, vp, vp]),
     "hm_debug_expf": (c_i32, [vp, vp, c_i64, vp]),
 }
 

@@ -86,9 +86,13 @@ typedef enum hm_status {
  * at every batch size measured (the tiles stream the same weights faster). */
 #define HM_EXEC_SPLIT_K 0x800u
 
-/* Expert weight dtypes (src/tensor/DType.hpp:9-14 numbering). */
+/* Element types (src/tensor/DType.hpp:9-14 numbering; FP8 has no counterpart
+ * there).  Expert weights are FP32, INT8 or FP8. */
 #define HM_DTYPE_FP32 0
+#define HM_DTYPE_FP16 1
+#define HM_DTYPE_BF16 2
 #define HM_DTYPE_INT8 3
+#define HM_DTYPE_FP8 4 /* e4m3 bytes with a float scale per block (F1) */
 
 int hm_abi_version(void);
 const char* hm_status_string(int status);
@@ -342,6 +346,100 @@ int hm_limb_quantize_rows(const float* x, int64_t rows, int64_t inner,
 int hm_limb_partials(const int8_t* digits, int64_t rows, int64_t inner,
                      int32_t limbs, const int8_t* q_packed, int32_t zp,
                      int64_t cols, int32_t* partials, void* stream);
+
+/* ---- F1  Block-scaled FP8 (no counterpart in the reference) -------------
+ * A matrix [rows x width] in FP8 is rows of hm_fp8_pitch(width) bytes (width
+ * rounded up to 128): e4m3 (OCP, largest 448), zeros past the width, 16-byte
+ * aligned.  Each block of block_rows rows (1: activations, 128: weights) x
+ * 128 columns has a float scale, scale[ceil(rows / block_rows) x
+ * ceil(width / 128)]; a byte stands for its e4m3 value times that scale.
+ * Checkpoints in this format whose inner dimension is a multiple of 128 are
+ * read as they are.
+ *
+ * hm_fp8_quantize: x (FP32, FP16 or BF16; element (r, k) at x[r row_stride +
+ * k col_stride], one of the strides 1) to that form.  With amax = max(|x|,
+ * 2^-100) over a block, scale = amax / 448 and each byte is the e4m3 value
+ * nearest to 448 x / amax, ties to even (decided exactly for 16-bit x).  A
+ * block that holds an infinity or a NaN becomes NaN throughout.  The blocks
+ * of a transposed matrix are the transposed blocks, so quantising the
+ * transposed view of a weight gives the operand of its input's gradient.
+ *
+ * hm_fp8_matmul: y[m, n] = sum_b xs[m, b] ws[n / w_block_rows, b]
+ * sum_{k in block b} x[m, k] w[n, k], x [rows x inner] with a scale per row
+ * and block, w [cols x inner] with w_block_rows 128 or 1, y [rows x cols] in
+ * y_dtype (FP32, FP16, BF16).  Sums and scale products are FP32, in an order
+ * that the sizes fix.  A layer's product: x W^T.  Its input's gradient: dY
+ * times the quantised transposed view of W.  Its weight's gradient: the
+ * transposed views of dY and x, both with a scale per row (w_block_rows 1).
+ * y must not overlap the operands. */
+int64_t hm_fp8_pitch(int64_t width);
+int hm_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t width,
+                    int64_t row_stride, int64_t col_stride, int32_t block_rows,
+                    uint8_t* q, float* scale, void* stream);
+int hm_fp8_matmul(const uint8_t* xq, const float* xs, const uint8_t* wq,
+                  const float* ws, int32_t w_block_rows, int64_t rows,
+                  int64_t inner, int64_t cols, void* y, int32_t y_dtype,
+                  void* stream);
+
+/* ---- F2  FP8 experts ---------------------------------------------------
+ * The SwiGLU experts of a routed batch (ExpertExecutor.cpp:43-138 over the
+ * groups of MoERuntime.cpp:282-306) with the weights of an FP8 layer:
+ * grouped row g of expert e, offsets[e] <= g < offsets[e + 1], is
+ *   y[g] = z D_e^T,  z = silu(x[perm_tokens[g]] G_e^T) * (x[..] U_e^T),
+ * x and z each quantised as by hm_fp8_quantize(block_rows 1) before their
+ * product.  layer->packed holds, expert after expert, gate [I x pitch(H)],
+ * up [I x pitch(H)] and down [H x pitch(I)] bytes, layer->scale [E x 3 x
+ * ceil(H / 128) ceil(I / 128)] their block scales, each projection's in its
+ * own [ceil(N / 128) x ceil(K / 128)] order; zero_point is unused.  x
+ * [tokens x H], y [pairs x H]; offsets [E + 1] and perm_tokens [pairs] as
+ * hm_permute gives them (a token outside 0 .. tokens - 1 reads token 0).
+ * Rows of y from offsets[E] on are left as they were.  At most 1024 experts.
+ * The workspace holds hm_fp8_experts_workspace_bytes(...) bytes; calls that
+ * overlap in time need one each. */
+size_t hm_fp8_experts_workspace_bytes(const hm_layer* layer, int64_t tokens,
+                                      int64_t pairs);
+int hm_fp8_experts(const hm_layer* layer, const void* x, int32_t x_dtype,
+                   int64_t tokens, const int32_t* offsets,
+                   const int32_t* perm_tokens, int64_t pairs, void* y,
+                   int32_t y_dtype, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
+/* ---- F3  Token rows to the experts and back, and the gradients -----------
+ * hm_gather_rows and hm_combine for FP32, FP16 and BF16 rows (`dtype`), with
+ * weights either way, pairs that no expert took, and backward passes.
+ * slots [tokens x top_k] is hm_permute's: the grouped row of a token's r-th
+ * expert, below `rows`, each row named once.  A slot outside 0 .. rows - 1
+ * marks a pair that was dropped (a full expert, an expert on another GPU):
+ * it is written nowhere, adds nothing and its weight's gradient is 0.
+ * Grouped rows that no slot names are left as they were.  weights and their
+ * gradients are FP32 [tokens x top_k]; sums are FP32, ranks ascending, and
+ * rounded once.
+ *   hm_dispatch_rows       out[slots[t,r]] = w[t,r] x[t] (weights NULL: x[t])
+ *   hm_dispatch_rows_grad  dx[t] = sum_r w[t,r] dout[slots[t,r]],
+ *                          dweights[t,r] = <dout[slots[t,r]], x[t]>
+ *   hm_combine_rows        out[t] = sum_r w[t,r] y[slots[t,r]], plus
+ *                          residual[t] last (weights NULL: 1; residual NULL:
+ *                          none; out may be residual)
+ *   hm_combine_rows_grad   dy[slots[t,r]] = w[t,r] dout[t],
+ *                          dweights[t,r] = <dout[t], y[slots[t,r]]>
+ * (the residual's gradient is dout).  dweights may be NULL, then x and y may
+ * be too; asking for it needs the weights.  Outputs must not overlap inputs
+ * otherwise. */
+int hm_dispatch_rows(const void* x, const int32_t* slots, const float* weights,
+                     int64_t tokens, int32_t top_k, int64_t rows, int64_t width,
+                     int32_t dtype, void* out, void* stream);
+int hm_dispatch_rows_grad(const void* dout, const void* x, const int32_t* slots,
+                          const float* weights, int64_t tokens, int32_t top_k,
+                          int64_t rows, int64_t width, int32_t dtype, void* dx,
+                          float* dweights, void* stream);
+int hm_combine_rows(const void* y, const int32_t* slots, const float* weights,
+                    const void* residual, int64_t tokens, int32_t top_k,
+                    int64_t rows, int64_t width, int32_t dtype, void* out,
+                    void* stream);
+int hm_combine_rows_grad(const void* dout, const void* y, const int32_t* slots,
+                         const float* weights, int64_t tokens, int32_t top_k,
+                         int64_t rows, int64_t width, int32_t dtype, void* dy,
+                         float* dweights, void* stream);
 
 /* ---- Test hooks --------------------------------------------------------
  * The device restatement of glibc expf used by the router softmax and SiLU,
