@@ -1,146 +1,12 @@
-// hm_fp8_gemm.hip -- products of block-scaled e4m3 matrices (hm_fp8.h) and the FP8 experts.
-//
-//   y[m, n] = sum over blocks b of 128 of  xs[m, b] ws[n, b] P(m, n, b),
-//   P(m, n, b) = sum_{k in block b} x[m, k] w[n, k]
-// with x [M x K] scaled by rows and w [N x K] by 128 x 128 blocks or by rows.  One
-// v_mfma_f32_16x16x128_f8f6f4 is 16 x 16 of the P of one block; one fused multiply-add by the block's
-// scale joins it to the FP32 sum.
-//
-// Operand layout of the instruction: lane l supplies 32 bytes of row l % 16 of A and of column l % 16
-// of B, the same K positions of both, so which 32 of the 128 a lane group l / 16 holds is free as long
-// as both operands agree (16-byte pieces g and g + 4).  Its 4 results are column l % 16, rows
-// 4 (l / 16) + v.  The weights are A and the rows of x are B: a lane's results are then four
-// consecutive outputs of one row, under one scale of x.
-#include "hm_fp8.h"
+// hm_fp8_gemm.hip -- products of block-scaled e4m3 matrices and the FP8 experts: the entry points, and
+// the kernel for few rows, which streams the weights (hm_fp8_product.h, hm_fp8_tile.hip).
+#include "hm_fp8_product.h"
 
 #include <limits.h>
 
+#include <algorithm>
+
 namespace {
-
-typedef int v4i __attribute__((ext_vector_type(4)));
-typedef int v8i __attribute__((ext_vector_type(8)));
-typedef float v4f __attribute__((ext_vector_type(4)));
-
-typedef __bf16 v2b __attribute__((ext_vector_type(2)));
-typedef __bf16 v8b __attribute__((ext_vector_type(8)));
-
-__device__ __forceinline__ v4f mfma_f8(v8i a, v8i b, v4f c) {
-    // formats 0, 0: e4m3; no block exponents
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);
-}
-
-// The lane's 32 bytes of a 128-byte block of one row: pieces g and g + 4.
-__device__ __forceinline__ v8i join_frag(v4i lo, v4i hi) {
-    return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-}
-__device__ __forceinline__ v8i load_frag(const uint8_t* block, int g) {
-    return join_frag(*reinterpret_cast<const v4i*>(block + 16 * g),
-                     *reinterpret_cast<const v4i*>(block + 16 * (g + 4)));
-}
-
-// The FP8 instruction aligns each eight consecutive products to the largest of them and drops what
-// lies more than 13 bits below it (measured: 2^16 + 2^2 is 2^16 inside a group of eight and exact
-// across groups), 1.3e-5 to 2.4e-5 of a sum's norm: under a sixth of FP16's rounding step and a
-// hundredth of BF16's, but 300 times FP32's.  Where that shows, the operands are widened to bf16
-// (exact) for v_mfma_f32_16x16x32_bf16, whose sums are FP32 (1e-8), at half the rate: Frag<true>.
-template <bool PREC>
-struct Frag;
-template <>
-struct Frag<false> {
-    v8i v;
-    __device__ __forceinline__ void set(v8i f) { v = f; }
-};
-template <>
-struct Frag<true> {
-    v8b v[4];
-    __device__ __forceinline__ void set(v8i f) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v2b w[4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                w[2 * h] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)f[2 * i + h], 1.0f, false);
-                w[2 * h + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)f[2 * i + h], 1.0f, true);
-            }
-            v[i] = v8b{w[0][0], w[0][1], w[1][0], w[1][1], w[2][0], w[2][1], w[3][0], w[3][1]};
-        }
-    }
-};
-// P of one block.
-__device__ __forceinline__ v4f block_product(const Frag<false>& a, const Frag<false>& b) {
-    return mfma_f8(a.v, b.v, v4f{});
-}
-__device__ __forceinline__ v4f block_product(const Frag<true>& a, const Frag<true>& b) {
-    v4f c = {};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b.v[i], c, 0, 0, 0);
-    return c;
-}
-
-// Four consecutive outputs of a row, columns n .. n + 3 (those below cols).
-template <typename T>
-__device__ __forceinline__ void store4(T* y, int64_t n, int64_t cols, v4f v, bool wide) {
-    if (wide && n + 4 <= cols) {
-        hm_pack<T, 4> w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w.v[i] = (T)v[i];
-        *reinterpret_cast<hm_pack<T, 4>*>(y + n) = w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (n + i < cols) y[n + i] = (T)v[i];
-    }
-}
-
-// A product's operands.  Grouped: expert e's rows are offsets[e] .. offsets[e + 1], row g of a group
-// reads row perm[g] of x (or g itself), and its matrix starts at w + e w_expert.
-struct Product {
-    const uint8_t* x;
-    const float* xs;
-    const uint8_t* w;
-    const float* ws;
-    int64_t w_expert, ws_expert;  // bytes, scales from one expert's matrix to the next one's
-    const int32_t* perm;
-    const int32_t* offsets;
-    int64_t rows, x_rows;         // output rows, rows of x
-    int64_t K, N;
-    int experts;
-    bool wide;                    // y's rows take 4-element stores
-};
-
-// The m-tile `tile` of `bm` rows, experts in ascending order: its expert, first row and row count.
-struct Tile {
-    int e;
-    int64_t row0, nrows;
-};
-// Every lane of the wave must be active.  False past the last tile; rows stays inside [0, rows).
-__device__ __forceinline__ bool locate(const int32_t* __restrict__ offsets, int experts, int64_t rows,
-                                       int bm, int64_t tile, Tile* t) {
-    const int lane = threadIdx.x & 63;
-    int64_t base = 0;
-    for (int c0 = 0; c0 < experts; c0 += 64) {
-        const int e = c0 + lane;
-        const int n = e < experts ? offsets[e + 1] - offsets[e] : 0;
-        const int64_t tiles = (n + bm - 1) / bm;
-        int64_t incl = tiles;
-#pragma unroll
-        for (int sft = 1; sft < 64; sft <<= 1) {
-            const int64_t o = __shfl_up(incl, sft, 64);
-            if (lane >= sft) incl += o;
-        }
-        const int64_t total = __shfl(incl, 63, 64);
-        if (tile < base + total) {
-            const int first = __ffsll((long long)__ballot(base + incl > tile)) - 1;
-            const int64_t in = tile - base - __shfl(incl - tiles, first, 64);
-            t->e = c0 + first;
-            t->row0 = offsets[t->e] + in * bm;
-            t->nrows = min((int64_t)bm, min((int64_t)offsets[t->e + 1], rows) - t->row0);
-            return t->row0 >= 0 && t->nrows > 0;
-        }
-        base += total;
-    }
-    return false;
-}
 
 constexpr int kSWaves = 8;
 
@@ -245,8 +111,49 @@ int launch_stream(const Product& p, int64_t m_tiles16, T* y, hipStream_t s) {
     return HM_OK;
 }
 
+// Which kernel takes one matrix product: the one of least time, estimated as a start plus steps (blocks
+// of K) x rounds of workgroups x the measured time of a step, alone on its CU while the tiles do not
+// fill the chip and with all CUs busy beyond that (us).  Tiles of 64 x 128 and, for FP8 instructions,
+// 128 x 128 sit two to a CU.  2048 x 2048 x K: 64 x 128 tiles 54 us at K = 8192, 128 x 256 58, 256 x 256
+// 93; 4096 x 4096: 104, 72 and 63 at K = 4096.  The stream kernel has no ring to fill: 16 rows of
+// 2048 x 2048 7 us against 8 for the smallest tile, 333 x 1000 x 777 (FP32) 7.3 against 10.5.
+struct Form {
+    int bm, bn, per_cu;
+    double alone, shared;
+};
+constexpr Form kFast[] = {{256, 256, 1, 1.35, 1.71}, {128, 256, 1, 0.79, 0.99},
+                          {128, 128, 2, 0.58, 1.14}, {64, 128, 2, 0.41, 0.85}};
+constexpr Form kExact[] = {{128, 256, 1, 1.9, 2.1}, {128, 128, 1, 1.3, 1.4}, {64, 128, 2, 0.85, 1.24}};
+constexpr int kCus = 256;
+
+// nullptr: the stream kernel
+const Form* choose_form(const Product& p, bool exact) {
+    const double steps = (double)hm_f8_blocks(p.K);
+    const double groups = (double)((p.N + 15) / 16) * (double)((p.rows + 63) / 64);
+    double best = 4.7 + steps / 16 * (groups <= kCus ? 4.0 : groups / (2 * kCus) * 12.0);
+    const Form* form = nullptr;
+    if (!hm_f8_tile_ok(p, false)) return nullptr;
+    const Form* forms = exact ? kExact : kFast;
+    for (int i = 0; i < (exact ? 3 : 4); ++i) {
+        const Form& f = forms[i];
+        const int64_t tiles = ((p.rows + f.bm - 1) / f.bm) * ((p.N + f.bn - 1) / f.bn);
+        const int64_t rounds = (tiles + kCus * f.per_cu - 1) / (kCus * f.per_cu);
+        const double t = 4.0 + steps * (tiles <= kCus ? f.alone : rounds * f.shared);
+        if (t < best) {
+            best = t;
+            form = &f;
+        }
+    }
+    return form;
+}
+
 template <typename T>
-int matmul(Product& p, int32_t w_block_rows, void* y, hipStream_t s) {
+int matmul(Product& p, int32_t w_block_rows, void* y, int32_t dtype, hipStream_t s) {
+    if (const Form* f = choose_form(p, dtype == HM_DTYPE_FP32)) {
+        p.wide = p.N * sizeof(T) % 16 == 0 && (uintptr_t)y % 16 == 0;
+        return hm_f8_launch_tiles(f->bm, f->bn, w_block_rows == 1, p, nullptr,
+                                  (p.rows + f->bm - 1) / f->bm, y, dtype, s);
+    }
     p.wide = p.N % 4 == 0 && (uintptr_t)y % (4 * sizeof(T)) == 0;
     T* out = static_cast<T*>(y);
     return w_block_rows == 1 ? launch_stream<false, true>(p, 0, out, s)
@@ -256,14 +163,41 @@ int matmul(Product& p, int32_t w_block_rows, void* y, hipStream_t s) {
 constexpr size_t kAlign = 256;
 size_t align_up(size_t v) { return (v + kAlign - 1) & ~(kAlign - 1); }
 
-// The experts' workspace: the quantised rows of x, z in floats, and its bytes and scales.
+// The experts' workspace.  Tiles: the quantised rows of x, the bytes and scales of z, the m-tile table.
+// Streamed: z in floats besides.
 struct ExpertsPlan {
     uint8_t* xq;
     float* xs;
     float* z;
     uint8_t* zq;
     float* zs;
+    int4* table;
 };
+
+// Few rows stream (a token or two: 21 and 27 us against 24 and 26 for tiles); others take tiles of 64 rows, or
+// 128 where an expert has that many on average (128 experts top-8, 2048 tokens: 194 us against 211; 1024:
+// 168 against 160).
+constexpr int64_t kStreamPairs = 8;
+struct ExpertsForm {
+    bool tiles;
+    int bm;
+    int cap;      // upper bound of the m-tiles
+};
+Product gate_up(const hm_layer* L, int64_t tokens, int64_t pairs) {
+    return Product{nullptr, nullptr, nullptr, nullptr, 0, 0, reinterpret_cast<const int32_t*>(4), nullptr, pairs,
+                   tokens, L->hidden, L->intermediate, (int)L->experts, false};
+}
+ExpertsForm experts_form(const hm_layer* L, int64_t tokens, int64_t pairs) {
+    ExpertsForm f;
+    const Product gu = gate_up(L, tokens, pairs);
+    const Product dn = {nullptr, nullptr, nullptr, nullptr, 0, 0, nullptr, nullptr, pairs, pairs,
+                        L->intermediate, L->hidden, (int)L->experts, false};
+    f.tiles = pairs > kStreamPairs && hm_f8_tile_ok(gu, true) && hm_f8_tile_ok(dn, false);
+    f.bm = pairs >= 128 * L->experts ? 128 : 64;
+    f.cap = (int)(pairs / f.bm + std::min(L->experts, pairs));
+    return f;
+}
+
 size_t plan_experts(const hm_layer* L, int64_t tokens, int64_t pairs, char* base, ExpertsPlan* p) {
     size_t used = 0;
     auto take = [&](size_t bytes) {
@@ -271,13 +205,15 @@ size_t plan_experts(const hm_layer* L, int64_t tokens, int64_t pairs, char* base
         used += align_up(bytes);
         return at;
     };
+    const ExpertsForm f = experts_form(L, tokens, pairs);
     const int64_t H = L->hidden, I = L->intermediate;
     ExpertsPlan q;
     q.xq = reinterpret_cast<uint8_t*>(take((size_t)tokens * hm_f8_pitch(H)));
     q.xs = reinterpret_cast<float*>(take((size_t)tokens * hm_f8_blocks(H) * sizeof(float)));
-    q.z = reinterpret_cast<float*>(take((size_t)pairs * I * sizeof(float)));
+    q.z = f.tiles ? nullptr : reinterpret_cast<float*>(take((size_t)pairs * I * sizeof(float)));
     q.zq = reinterpret_cast<uint8_t*>(take((size_t)pairs * hm_f8_pitch(I)));
     q.zs = reinterpret_cast<float*>(take((size_t)pairs * hm_f8_blocks(I) * sizeof(float)));
+    q.table = f.tiles ? reinterpret_cast<int4*>(take(((size_t)f.cap + 1) * sizeof(int4))) : nullptr;
     if (p) *p = q;
     return used;
 }
@@ -305,9 +241,9 @@ int hm_fp8_matmul(const uint8_t* xq, const float* xs, const uint8_t* wq, const f
     Product p = {xq, xs, wq, ws, 0, 0, nullptr, nullptr, rows, rows, inner, cols, 1, false};
     hipStream_t s = hm_stream(stream);
     switch (y_dtype) {
-    case HM_DTYPE_FP32: return matmul<float>(p, w_block_rows, y, s);
-    case HM_DTYPE_FP16: return matmul<hm_f16>(p, w_block_rows, y, s);
-    default: return matmul<hm_bf16>(p, w_block_rows, y, s);
+    case HM_DTYPE_FP32: return matmul<float>(p, w_block_rows, y, y_dtype, s);
+    case HM_DTYPE_FP16: return matmul<hm_f16>(p, w_block_rows, y, y_dtype, s);
+    default: return matmul<hm_bf16>(p, w_block_rows, y, y_dtype, s);
     }
 }
 
@@ -342,16 +278,31 @@ int hm_fp8_experts(const hm_layer* layer, const void* x, int32_t x_dtype, int64_
     const int64_t per = 2 * I * ph + H * pi;
     const uint8_t* packed = static_cast<const uint8_t*>(layer->packed);
     hipStream_t s = hm_stream(stream);
-    int rc = hm_fp8_quantize(x, x_dtype, tokens, H, H, 1, 1, ws.xq, ws.xs, stream);
-    if (rc) return rc;
+    const ExpertsForm form = experts_form(layer, tokens, pairs);
+    int rc;
     Product gu = {ws.xq, ws.xs, packed, layer->scale, per, 3 * hb * ib, perm_tokens, offsets,
                   pairs, tokens, H, I, (int)E, I % 4 == 0};
+    Product dn = {ws.zq, ws.zs, packed + 2 * I * ph, layer->scale + 2 * hb * ib, per, 3 * hb * ib,
+                  nullptr, offsets, pairs, pairs, I, H, (int)E, false};
+    const size_t ysize = hm_row_dtype_size(y_dtype);
+    if (form.tiles) {
+        rc = hm_f8_launch_prepare(x, x_dtype, tokens, H, ws.xq, ws.xs, offsets, (int)E, (int)pairs,
+                                  form.bm, form.cap, ws.table, s);
+        if (rc) return rc;
+        // z goes to 8 bits, so what the FP8 instruction drops can move a byte of it by a step (1.4e-3 of
+        // a BF16 result, whose own rounding is 1.7e-3): only where its rate counts and y is BF16
+        const bool exact = y_dtype != HM_DTYPE_BF16 || pairs < 128 * E;
+        rc = hm_f8_launch_gateup_tiles(form.bm, exact, gu, ws.table, form.cap, ws.zq, ws.zs, s);
+        if (rc) return rc;
+        dn.wide = H * ysize % 16 == 0 && (uintptr_t)y % 16 == 0;
+        return hm_f8_launch_tiles(form.bm, 256, false, dn, ws.table, form.cap, y, y_dtype, s);
+    }
+    rc = hm_fp8_quantize(x, x_dtype, tokens, H, H, 1, 1, ws.xq, ws.xs, stream);
+    if (rc) return rc;
     if ((rc = launch_stream<true, false>(gu, pairs, ws.z, s))) return rc;
     rc = hm_fp8_quantize(ws.z, HM_DTYPE_FP32, pairs, I, I, 1, 1, ws.zq, ws.zs, stream);
     if (rc) return rc;
-    Product dn = {ws.zq, ws.zs, packed + 2 * I * ph, layer->scale + 2 * hb * ib, per, 3 * hb * ib,
-                  nullptr, offsets, pairs, pairs, I, H, (int)E, false};
-    dn.wide = H % 4 == 0 && (uintptr_t)y % (4 * hm_row_dtype_size(y_dtype)) == 0;
+    dn.wide = H % 4 == 0 && (uintptr_t)y % (4 * ysize) == 0;
     switch (y_dtype) {
     case HM_DTYPE_FP32: return launch_stream<false, false>(dn, pairs, static_cast<float*>(y), s);
     case HM_DTYPE_FP16: return launch_stream<false, false>(dn, pairs, static_cast<hm_f16*>(y), s);

@@ -34,11 +34,11 @@ __device__ __forceinline__ void load8(const T* __restrict__ p, int64_t left, flo
 }
 
 template <typename T, bool VEC>
-__global__ __launch_bounds__(kQThreads) void f8_quantize_rows_kernel(
-    const T* __restrict__ x, int64_t rows, int64_t width, int64_t stride, uint8_t* __restrict__ q,
-    float* __restrict__ scale) {
+__device__ __forceinline__ void quantize_rows(const T* __restrict__ x, int64_t rows, int64_t width,
+                                              int64_t stride, uint8_t* __restrict__ q,
+                                              float* __restrict__ scale, int64_t block) {
     const int64_t nb = hm_f8_blocks(width);
-    const int64_t g = (int64_t)blockIdx.x * (kQThreads / 16) + (threadIdx.x >> 4);
+    const int64_t g = block * (kQThreads / 16) + (threadIdx.x >> 4);
     const bool live = g < rows * nb;
     const int64_t gg = live ? g : 0;
     const int64_t r = gg / nb, kb = gg - r * nb;
@@ -57,6 +57,68 @@ __global__ __launch_bounds__(kQThreads) void f8_quantize_rows_kernel(
     w.y = hm_f8_pack4(s, v[4], v[5], v[6], v[7]);
     *reinterpret_cast<uint2*>(q + (r * nb + kb) * kF8Block + c) = w;
     if ((threadIdx.x & 15) == 0) scale[r * nb + kb] = s.scale;
+}
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(kQThreads) void f8_quantize_rows_kernel(
+    const T* __restrict__ x, int64_t rows, int64_t width, int64_t stride, uint8_t* __restrict__ q,
+    float* __restrict__ scale) {
+    quantize_rows<T, VEC>(x, rows, width, stride, q, scale, blockIdx.x);
+}
+
+// The rows of an expert batch, and (workgroup 0) the table of its m-tiles: entry 0 their number, then
+// {expert, first row, rows} of each, experts ascending.  A launch of its own would cost as much as the
+// quantisation.  Offsets outside [0, pairs] are cut to it, tiles past `cap` dropped.
+constexpr int kMaxTableExperts = 1024;
+
+template <typename T, bool VEC>
+__global__ __launch_bounds__(kQThreads) void f8_prepare_kernel(
+    const T* __restrict__ x, int64_t rows, int64_t width, uint8_t* __restrict__ q,
+    float* __restrict__ scale, const int32_t* __restrict__ offsets, int experts, int pairs, int bm,
+    int cap, int4* __restrict__ table) {
+    if (blockIdx.x > 0) {
+        quantize_rows<T, VEC>(x, rows, width, width, q, scale, (int64_t)blockIdx.x - 1);
+        return;
+    }
+    __shared__ int s_first[kMaxTableExperts + 1];   // an expert's first tile
+    const int tid = threadIdx.x, lane = tid & 63;
+    auto bounds = [&](int e, int* lo) __attribute__((always_inline)) {
+        *lo = max(0, min(offsets[e], pairs));
+        return max(0, min(offsets[e + 1], pairs) - *lo);
+    };
+    if (tid < 64) {
+        int base = 0;
+        for (int c0 = 0; c0 < experts; c0 += 64) {
+            const int e = c0 + lane;
+            int lo;
+            const int n = e < experts ? (bounds(e, &lo) + bm - 1) / bm : 0;
+            int incl = n;
+#pragma unroll
+            for (int s = 1; s < 64; s <<= 1) {
+                const int o = __shfl_up(incl, s, 64);
+                if (lane >= s) incl += o;
+            }
+            if (e < experts) s_first[e] = min(base + incl - n, cap);
+            base = min(base + __shfl(incl, 63, 64), cap);
+        }
+        if (lane == 0) {
+            s_first[experts] = base;
+            table[0] = make_int4(base, 0, 0, 0);
+        }
+    }
+    __syncthreads();
+    const int total = s_first[experts];
+    for (int t = tid; t < total; t += kQThreads) {
+        int a = 0, b = experts;                     // s_first[a] <= t < s_first[b]
+        while (b - a > 1) {
+            const int m = (a + b) / 2;
+            if (s_first[m] <= t) a = m;
+            else b = m;
+        }
+        int lo;
+        const int n = bounds(a, &lo), at = (t - s_first[a]) * bm;
+        table[1 + t] = make_int4(a, lo + at, min(bm, n - at), 0);
+    }
 }
 
 // The maximum over a workgroup of `waves` waves; every thread gets it.
@@ -189,7 +251,38 @@ int launch_quantize(const T* x, int64_t rows, int64_t width, int64_t row_stride,
     return HM_OK;
 }
 
+template <typename T>
+int launch_prepare(const T* x, int64_t rows, int64_t width, uint8_t* q, float* scale,
+                   const int32_t* offsets, int experts, int pairs, int bm, int cap, int4* table,
+                   hipStream_t s) {
+    const bool vec = (uintptr_t)x % 16 == 0 && width % (16 / (int64_t)sizeof(T)) == 0;
+    const int64_t grid = (rows * hm_f8_blocks(width) + kQThreads / 16 - 1) / (kQThreads / 16) + 1;
+    if (grid > INT_MAX / kQThreads) return HM_ERR_OVERFLOW;
+    hipLaunchKernelGGL((vec ? f8_prepare_kernel<T, true> : f8_prepare_kernel<T, false>),
+                       dim3((unsigned)grid), dim3(kQThreads), 0, s, x, rows, width, q, scale, offsets,
+                       experts, pairs, bm, cap, table);
+    HM_LAUNCHED();
+    return HM_OK;
+}
+
 }  // namespace
+
+// x [rows x width] to FP8, and the m-tile table of a batch of at most kMaxTableExperts experts.
+int hm_f8_launch_prepare(const void* x, int32_t dtype, int64_t rows, int64_t width, uint8_t* q,
+                         float* scale, const int32_t* offsets, int experts, int pairs, int bm, int cap,
+                         int4* table, hipStream_t s) {
+    switch (dtype) {
+    case HM_DTYPE_FP32:
+        return launch_prepare(static_cast<const float*>(x), rows, width, q, scale, offsets, experts,
+                              pairs, bm, cap, table, s);
+    case HM_DTYPE_FP16:
+        return launch_prepare(static_cast<const hm_f16*>(x), rows, width, q, scale, offsets, experts,
+                              pairs, bm, cap, table, s);
+    default:
+        return launch_prepare(static_cast<const hm_bf16*>(x), rows, width, q, scale, offsets, experts,
+                              pairs, bm, cap, table, s);
+    }
+}
 
 extern "C" {
 

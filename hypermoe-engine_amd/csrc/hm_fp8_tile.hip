@@ -1,0 +1,443 @@
+// hm_fp8_tile.hip -- tiles of the block-scaled FP8 product (hm_fp8_product.h) through an LDS ring: one
+// matrix, or the experts' groups; plain, or gate and up with SwiGLU and the quantisation of z.
+//
+// Persistent workgroups of 8 waves, 2 (rows of x) x 4 (rows of w); a wave owns 16 XF x 16 WF outputs
+// (tile BM = 32 XF rows of x, BN = 64 WF of w).  A stage is one block of 128 of K: (BM + BN) rows of 128
+// bytes, moved to the LDS by DMA, and the stage's scales (one float a row, whatever block it covers).
+// Stages of consecutive tiles form one stream, so a tile's first stages load while its predecessor ends.
+//   LDS   row r's 16-byte piece c sits at position c ^ s(r): a fragment read takes rows of one piece
+//         by 16 lanes, and s separates those 16 (eight values and the row's parity), for w with the
+//         row order below.  No bank conflicts.
+//   w     fragment j's row i is w row 4 SH (i / 4) + 4 j + i % 4 of the wave's, so that a lane ends
+//         with 4 SH consecutive outputs of one row (SH: fragments side by side).
+//   order tiles are cut into 8 contiguous ranges, one per XCD (workgroup i runs on XCD i % 8); n-tiles
+//         of an m-tile lie together, for one matrix in groups of 4 m-tiles, so what is read by
+//         several workgroups at once is in one L2.
+// Epilogue of gate/up (GU): z = silu(g) u for one block of 128 columns; its maximum over the block goes
+// over lanes, then through the LDS over the four waves of a row; the bytes and scale are stored.
+#include "hm_fp8_product.h"
+#include "hm_lds_dma.h"
+
+#include <limits.h>
+
+#include <algorithm>
+#include <type_traits>
+
+namespace {
+
+constexpr int kXcds = 8;
+constexpr int kTThreads = 512;
+constexpr int kSuper = 4;    // m-tiles walked together (one matrix)
+
+__device__ __forceinline__ float fast_silu(float g) {
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896f));
+}
+
+struct TileAt {
+    int e, row0, nrows, n0;
+};
+
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+template <typename P>
+__device__ __forceinline__ P* uni(P* p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<P*>(((uint64_t)(uint32_t)uni((int)(v >> 32)) << 32) | (uint32_t)uni((int)v));
+}
+
+// Tile j: n-tiles of an m-tile lie together, for one matrix in groups of kSuper m-tiles.
+template <int BM, int TN>
+__device__ __forceinline__ TileAt tile_at(const Product& p, const int4* __restrict__ table, int j, int mt,
+                                          int ntn) {
+    TileAt t;
+    if (table) {
+        const int m = j / ntn;
+        const int4 e = table[1 + m];
+        t.e = uni(e.x);
+        t.row0 = uni(e.y);
+        t.nrows = uni(e.z);
+        t.n0 = (j - m * ntn) * TN;
+    } else {
+        const int grp = j / (kSuper * ntn), first = grp * kSuper;
+        const int gm = min(mt - first, kSuper), r = j - first * ntn;
+        t.e = 0;
+        t.row0 = (first + r % gm) * BM;
+        t.nrows = min(BM, (int)p.rows - t.row0);
+        t.n0 = r / gm * TN;
+    }
+    return t;
+}
+
+// A tile's results.  The lane holds column run c0 .. c0 + 4 SH - 1 of the rows 16 i + i16 (from wm 16 XF).
+template <int XF, int WF, typename T>
+__device__ __forceinline__ void store_y(const Product& p, const TileAt& t, const v4f (&acc)[XF][WF], T* y,
+                                        int r0, int c0) {
+    constexpr int VN = 16 / sizeof(T);
+    const int N = (int)p.N;
+#pragma unroll
+    for (int i = 0; i < XF; ++i) {
+        const int r = r0 + 16 * i;
+        if (r >= t.nrows) continue;
+        T* to = y + (int64_t)(t.row0 + r) * N + c0;
+        if (p.wide && c0 + 4 * WF <= N) {
+#pragma unroll
+            for (int q = 0; q < 4 * WF; q += VN) {
+                hm_pack<T, VN> w;
+#pragma unroll
+                for (int v = 0; v < VN; ++v) w.v[v] = (T)acc[i][(q + v) / 4][(q + v) % 4];
+                *reinterpret_cast<hm_pack<T, VN>*>(to + q) = w;
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4 * WF; ++q)
+                if (c0 + q < N) to[q] = (T)acc[i][q / 4][q % 4];
+        }
+    }
+}
+// z = silu(gate) up and its quantisation (one block of 128 columns; s_amax: a maximum for each of the
+// four waves of a row).  Every wave of the workgroup calls it.
+template <int XF, int WF, int BM>
+__device__ __forceinline__ void store_z(const Product& p, const TileAt& t, v4f (&acc)[XF][WF],
+                                        float (&s_amax)[4][BM], uint8_t* zq, float* zs, int r0, int c0,
+                                        int wn, int g) {
+    constexpr int SH = WF / 2;
+    const int N = (int)p.N, nbn = (int)hm_f8_blocks(p.N);
+#pragma unroll
+    for (int i = 0; i < XF; ++i) {
+        float amax = 0.0f, bad = 0.0f;
+#pragma unroll
+        for (int q = 0; q < SH; ++q)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const float z = c0 + 4 * q + v < N ? fast_silu(acc[i][q][v]) * acc[i][SH + q][v] : 0.0f;
+                acc[i][q][v] = z;
+                amax = fmaxf(amax, fabsf(z));
+                bad = __builtin_fmaf(z, 0.0f, bad);  // NaN from an infinity or a NaN
+            }
+        amax = bad == 0.0f ? amax : __builtin_inff();
+        amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
+        amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+        if (g == 0) s_amax[wn][r0 + 16 * i] = amax;
+    }
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < XF; ++i) {
+        const int r = r0 + 16 * i;
+        const hm_f8_scaler s = hm_f8_scaler_of(
+            fmaxf(fmaxf(s_amax[0][r], s_amax[1][r]), fmaxf(s_amax[2][r], s_amax[3][r])));
+        if (r >= t.nrows) continue;
+        uint32_t w[SH];
+#pragma unroll
+        for (int q = 0; q < SH; ++q)
+            w[q] = hm_f8_pack4(s, acc[i][q][0], acc[i][q][1], acc[i][q][2], acc[i][q][3]);
+        const int64_t row = t.row0 + r;
+        uint32_t* to = reinterpret_cast<uint32_t*>(zq + row * (nbn * kF8Block) + c0);
+#pragma unroll
+        for (int q = 0; q < SH; ++q) to[q] = w[q];
+        if (wn == 0 && g == 0) zs[row * nbn + t.n0 / kF8Block] = s.scale;
+    }
+}
+
+template <int XF, int WF, int NS, bool GU, bool BROW, bool PREC, typename T>
+__global__ __launch_bounds__(kTThreads) void f8_tile_kernel(Product p, const int4* __restrict__ table,
+                                                            T* __restrict__ y, uint8_t* __restrict__ zq,
+                                                            float* __restrict__ zs) {
+    constexpr int BM = 32 * XF, BN = 64 * WF, ROWS = BM + BN;
+    constexpr int LPW = ROWS / 64;             // a wave's 1 KB (8-row) DMAs per stage
+    constexpr int XL = BM / 64;                // the first of them are rows of x
+    constexpr int SH = GU ? WF / 2 : WF;
+    constexpr int SB = 2 + (SH == 4 ? 2 : SH == 2 ? 1 : 0);  // where i / 4 sits in a w row
+    constexpr int TN = GU ? BN / 2 : BN;       // output columns per tile
+    constexpr int STAGE = ROWS * kF8Block;
+    constexpr int XA = XF >= 4 ? 2 : 1;        // fragments of x read ahead
+    constexpr bool GATHER = GU;                // rows of x by perm, else consecutive
+    static_assert(BM % 64 == 0 && (!GU || TN == kF8Block), "tile shape");
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * STAGE];
+    __shared__ __attribute__((aligned(16))) float s_sc[NS][ROWS];
+    __shared__ __attribute__((aligned(16))) int32_t s_rt[GATHER ? 2 : 1][GATHER ? BM : 64];  // x rows of a tile
+    __shared__ float s_amax[GU ? 4 : 1][GU ? BM : 1];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 2, wn = wave & 3;
+    const int i16 = lane & 15, g = lane >> 4;
+    const int nb = (int)hm_f8_blocks(p.K);
+    const uint32_t pitch = (uint32_t)nb * kF8Block;
+    const int N = (int)p.N, nbn = (int)hm_f8_blocks(p.N);
+    const int ntn = (N + TN - 1) / TN;
+    const int mt = table ? table[0].x : (int)((p.rows + BM - 1) / BM);
+    const int total = mt * ntn;
+    const int per = (total + kXcds - 1) / kXcds;
+    const int step = gridDim.x / kXcds;
+    const int jbeg = (blockIdx.x % kXcds) * per + blockIdx.x / kXcds;
+    const int jend = min((int)(blockIdx.x % kXcds + 1) * per, total);
+    if (jbeg >= jend) return;
+
+    auto info = [&](int j) __attribute__((always_inline)) { return tile_at<BM, TN>(p, table, j, mt, ntn); };
+
+    // ---- sources.  Lane l of DMA c of a wave: row 8 (wave + 8 c) + l / 8, position l % 8.
+    const int lr = lane >> 3, pos = lane & 7;
+    uint32_t voff[LPW];
+    uint32_t soff;
+    const uint8_t *xbase, *wbase;
+    const float* sbase;
+    const int sgrp = wave % LPW;               // this wave's 64 of the stage's ROWS scales
+    // the x row (of the product's x) of tile row r
+    auto make_src = [&](const TileAt& t, int m) __attribute__((always_inline)) {
+        xbase = p.x + (GATHER ? 0 : (int64_t)t.row0 * pitch);
+        wbase = p.w + (int64_t)t.e * p.w_expert;
+        auto x_row = [&](int r) __attribute__((always_inline)) {
+            if constexpr (!GATHER) return min(r, t.nrows - 1);
+            const int v = s_rt[m][r];
+            return v >= 0 && v < (int)p.x_rows ? v : 0;
+        };
+        // row r of the tile's w rows, of the expert's matrices (up follows gate)
+        auto w_row = [&](int r) __attribute__((always_inline)) {
+            if (GU && r >= TN) return N + min(t.n0 + r - TN, N - 1);
+            return min(t.n0 + r, N - 1);
+        };
+#pragma unroll
+        for (int c = 0; c < LPW; ++c) {
+            const int r = 8 * (wave + 8 * c) + lr;
+            if (c < XL) {
+                voff[c] = (uint32_t)x_row(r) * pitch + 16 * (pos ^ ((r >> 1) & 7));
+            } else {
+                const int wr = r - BM;
+                const int s = ((wr >> 1) & 1) | (((wr >> SB) & 3) << 1);
+                voff[c] = (uint32_t)w_row(wr) * pitch + 16 * (pos ^ s);
+            }
+        }
+        const int sr = 64 * sgrp + lane;
+        if (64 * sgrp < BM) {
+            sbase = p.xs + (GATHER ? 0 : (int64_t)t.row0 * nb);
+            soff = (uint32_t)x_row(sr) * nb * 4;
+        } else {
+            sbase = p.ws + (int64_t)t.e * p.ws_expert;
+            const int wr = w_row(sr - BM);
+            if (BROW) soff = (uint32_t)wr * nb * 4;
+            else if (GU && wr >= N) soff = (uint32_t)(nbn + (wr - N) / kF8Block) * nb * 4;
+            else soff = (uint32_t)(wr / kF8Block) * nb * 4;
+        }
+    };
+    // load c (0 .. LPW) of stage ks into a slot
+    auto issue = [&](int slot, int ks, int c) __attribute__((always_inline)) {
+        if (c < LPW)
+            dma16_off(uni((c < XL ? xbase : wbase) + ks * kF8Block), voff[c],
+                      ring + slot * STAGE + 1024 * wave + 8192 * c);
+        else
+            dma4_off(uni(sbase + ks), soff, &s_sc[slot][64 * sgrp]);
+    };
+    // the x rows of a gathered tile (rows past its last repeat that one)
+    auto fetch_rows = [&](const TileAt& t, int m) __attribute__((always_inline)) {
+        const int r = 64 * (wave % XL) + lane;
+        dma4_off(uni(p.perm + t.row0), 4u * (uint32_t)min(r, t.nrows - 1), &s_rt[m][64 * (wave % XL)]);
+    };
+
+    // ---- fragments
+    const int xrd = (wm * 16 * XF + i16) * kF8Block + 16 * (g ^ ((i16 >> 1) & 7));
+    const int wrd = (BM + wn * 16 * SH + 4 * SH * (i16 >> 2) + (i16 & 3)) * kF8Block +
+                    16 * (g ^ (((i16 >> 1) & 1) | ((i16 >> 2) << 1)));
+    auto read = [&](const uint8_t* at, int off) __attribute__((always_inline)) {
+        return join_frag(*reinterpret_cast<const v4i*>(at + off), *reinterpret_cast<const v4i*>(at + (off ^ 64)));
+    };
+    v4f acc[XF][WF];
+
+    // The stage in `slot`, and between its matrix instructions the loads of stage `ks` into `to`: issued
+    // at once they would hold the wave, since the vector memory unit takes one in 16 cycles.  A
+    // multiply-add takes the result of the matrix instruction before the last.
+    auto compute = [&](int slot, int to, int ks) __attribute__((always_inline)) {
+        const uint8_t* st = ring + slot * STAGE;
+        v8i raw[XA + 1];
+        float sx[XA + 1];
+        auto read_x = [&](int i) __attribute__((always_inline)) {
+            raw[i % (XA + 1)] = read(st + i * 16 * kF8Block, xrd);
+            sx[i % (XA + 1)] = s_sc[slot][wm * 16 * XF + 16 * i + i16];
+        };
+        // in the order of their use: the first instruction waits for four of the reads
+        read_x(0);
+        v8i wraw[WF];
+#pragma unroll
+        for (int j = 0; j < WF; ++j) {
+            wraw[j] = read(st + (j / SH) * TN * kF8Block + (j % SH) * 4 * kF8Block, wrd);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int i = 1; i < XA && i < XF; ++i) read_x(i);
+        Frag<PREC> fw[WF];
+        float sw1[2];
+        v4f swv[WF];
+        const float* sc = s_sc[slot] + BM + wn * 16 * SH;
+        if constexpr (BROW) {
+#pragma unroll
+            for (int j = 0; j < WF; ++j) swv[j] = *reinterpret_cast<const v4f*>(sc + 4 * SH * g + 4 * j);
+        } else {
+            sw1[0] = sc[0];
+            sw1[1] = GU ? sc[TN] : 0.0f;
+        }
+        constexpr int LAG = 2, NT = XF * WF, NI = LPW + 1;
+        constexpr int EVERY = NT / NI > 1 ? 2 : 1;
+        static_assert(NI * EVERY <= NT + EVERY - 1, "a slot for every load");
+        v4f part[LAG + 1];
+        float sxi[2];
+        Frag<PREC> fx;
+#pragma unroll
+        for (int t = 0; t < NT + LAG; ++t) {
+            if (t < NT) {
+                const int i = t / WF, j = t % WF;
+                if (j == 0) {
+                    fx.set(raw[i % (XA + 1)]);
+                    sxi[i & 1] = sx[i % (XA + 1)];
+                    if (i + XA < XF) read_x(i + XA);
+                }
+                if (i == 0) fw[j].set(wraw[j]);
+                part[t % (LAG + 1)] = block_product(fw[j], fx);
+                if (t % EVERY == 0 && t / EVERY < NI) issue(to, ks, t / EVERY);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (t >= LAG) {
+                const int u = t - LAG, i = u / WF, j = u % WF;
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+                    acc[i][j][v] = __builtin_fmaf(part[u % (LAG + 1)][v],
+                                                  sxi[i & 1] * (BROW ? swv[j][v] : sw1[GU ? j / SH : 0]),
+                                                  acc[i][j][v]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto issue_all = [&](int to, int ks) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c <= LPW; ++c) issue(to, ks, c);
+    };
+
+    // ---- the stream
+    TileAt cur = info(jbeg);
+    int m = 0;
+    if constexpr (GATHER) {
+        fetch_rows(cur, 0);
+        wait_vmcnt<0>();
+        lds_barrier();
+    }
+    make_src(cur, 0);
+#pragma unroll
+    for (int s = 0; s < NS - 1; ++s) issue_all(s, s);
+#pragma unroll
+    for (int i = 0; i < XF; ++i)
+#pragma unroll
+        for (int k = 0; k < WF; ++k) acc[i][k] = v4f{};
+    int j = jbeg, slot = 0, ks = 0;
+    bool has_next = j + step < jend;
+    TileAt nxt = cur;
+    if (has_next) nxt = info(j + step);
+    while (true) {
+        // this wave's loads of the stage have landed (at most the NS - 2 stages after it are in
+        // flight), then every wave's; and every wave has read the slot that is refilled below
+        wait_vmcnt<(NS - 2) * (LPW + 1)>();
+        lds_barrier();
+        int ahead = ks + NS - 1;
+        if constexpr (GATHER) {
+            if (ks == 0 && has_next) fetch_rows(nxt, m ^ 1);
+        }
+        if (ahead >= nb) {
+            if (ahead == nb && has_next) make_src(nxt, m ^ 1);
+            // (the stream's end loads stages once more that nothing reads, so that loads and waits have
+            // no conditions)
+            ahead -= nb;
+        }
+        const int to = slot == 0 ? NS - 1 : slot - 1;
+        // a wave whose rows all lie past the tile's last only loads
+        if (wm * 16 * XF < cur.nrows) compute(slot, to, ahead);
+        else issue_all(to, ahead);
+        slot = slot == NS - 1 ? 0 : slot + 1;
+        if (++ks < nb) continue;
+        const int r0 = wm * 16 * XF + i16, c0 = cur.n0 + wn * 16 * SH + 4 * SH * g;
+        if constexpr (GU) store_z<XF, WF, BM>(p, cur, acc, s_amax, zq, zs, r0, c0, wn, g);
+        else store_y<XF, WF, T>(p, cur, acc, y, r0, c0);
+        if (!has_next) break;
+#pragma unroll
+        for (int i = 0; i < XF; ++i)
+#pragma unroll
+            for (int k = 0; k < WF; ++k) acc[i][k] = v4f{};
+        ks = 0;
+        m ^= 1;
+        cur = nxt;
+        j += step;
+        has_next = j + step < jend;
+        if (has_next) nxt = info(j + step);
+    }
+    wait_vmcnt<0>();  // the LDS is not given back under a load
+}
+
+int cu_count() {
+    static int cached[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = 0;
+    if (cached[dev] == 0) {
+        int cus = 0;
+        if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < kXcds)
+            cus = 256;
+        cached[dev] = cus;
+    }
+    return cached[dev];
+}
+
+// per_cu workgroups share a CU (their LDS)
+template <int XF, int WF, int NS, bool GU, bool BROW, bool PREC, typename T>
+int launch(const Product& p, const int4* table, int64_t m_tiles, T* y, uint8_t* zq, float* zs,
+           hipStream_t s) {
+    constexpr int TN = GU ? 32 * WF : 64 * WF;
+    constexpr size_t lds = (size_t)NS * (32 * XF + 64 * WF) * (kF8Block + 4);
+    const int64_t tiles = m_tiles * ((p.N + TN - 1) / TN);
+    if (tiles > INT_MAX / 2) return HM_ERR_OVERFLOW;
+    const int64_t slots = (int64_t)cu_count() / kXcds * (lds > 76 * 1024 ? 1 : 2);
+    const int64_t grid = kXcds * std::min((tiles + kXcds - 1) / kXcds, slots);
+    hipLaunchKernelGGL((f8_tile_kernel<XF, WF, NS, GU, BROW, PREC, T>), dim3((unsigned)grid),
+                       dim3(kTThreads), 0, s, p, table, y, zq, zs);
+    HM_LAUNCHED();
+    return HM_OK;
+}
+
+template <bool BROW, bool PREC, typename T>
+int launch_plain(int bm, int bn, const Product& p, const int4* table, int64_t m_tiles, void* y,
+                 hipStream_t s) {
+    T* out = static_cast<T*>(y);
+    if constexpr (!PREC) {
+        if (bm == 256) return launch<8, 4, 2, false, BROW, PREC, T>(p, table, m_tiles, out, nullptr, nullptr, s);
+    }
+    if (bn == 256)
+        return bm == 128 ? launch<4, 4, 3, false, BROW, PREC, T>(p, table, m_tiles, out, nullptr, nullptr, s)
+                         : launch<2, 4, 3, false, BROW, PREC, T>(p, table, m_tiles, out, nullptr, nullptr, s);
+    return bm == 128 ? launch<4, 2, 2, false, BROW, PREC, T>(p, table, m_tiles, out, nullptr, nullptr, s)
+                     : launch<2, 2, 3, false, BROW, PREC, T>(p, table, m_tiles, out, nullptr, nullptr, s);
+}
+
+}  // namespace
+
+bool hm_f8_tile_ok(const Product& p, bool gu) {
+    const uint64_t pitch = (uint64_t)hm_f8_pitch(p.K), top = (uint64_t)1 << 32;
+    return p.K > 3 * kF8Block && p.rows < (int64_t)1 << 30 && p.N < (int64_t)1 << 28 &&
+           (uint64_t)(gu ? 2 * p.N : p.N) * pitch < top && (!p.perm || (uint64_t)p.x_rows * pitch < top) &&
+           256 * pitch < top;
+}
+
+int hm_f8_launch_tiles(int bm, int bn, bool brow, const Product& p, const int4* table, int64_t m_tiles,
+                       void* y, int32_t dtype, hipStream_t s) {
+    if (dtype == HM_DTYPE_FP32)
+        return brow ? launch_plain<true, true, float>(bm, bn, p, table, m_tiles, y, s)
+                    : launch_plain<false, true, float>(bm, bn, p, table, m_tiles, y, s);
+    if (dtype == HM_DTYPE_FP16)
+        return brow ? launch_plain<true, false, hm_f16>(bm, bn, p, table, m_tiles, y, s)
+                    : launch_plain<false, false, hm_f16>(bm, bn, p, table, m_tiles, y, s);
+    return brow ? launch_plain<true, false, hm_bf16>(bm, bn, p, table, m_tiles, y, s)
+                : launch_plain<false, false, hm_bf16>(bm, bn, p, table, m_tiles, y, s);
+}
+
+int hm_f8_launch_gateup_tiles(int bm, bool prec, const Product& p, const int4* table, int64_t m_tiles,
+                              uint8_t* zq, float* zs, hipStream_t s) {
+    float* none = nullptr;
+    if (prec)
+        return bm == 128 ? launch<4, 4, 3, true, false, true, float>(p, table, m_tiles, none, zq, zs, s)
+                         : launch<2, 4, 3, true, false, true, float>(p, table, m_tiles, none, zq, zs, s);
+    if (bm == 256) return launch<8, 4, 2, true, false, false, float>(p, table, m_tiles, none, zq, zs, s);
+    return bm == 128 ? launch<4, 4, 3, true, false, false, float>(p, table, m_tiles, none, zq, zs, s)
+                     : launch<2, 4, 3, true, false, false, float>(p, table, m_tiles, none, zq, zs, s);
+}

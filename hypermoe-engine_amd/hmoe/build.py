@@ -45,14 +45,15 @@ HIP_FLAGS = [
 ]
 KERNEL_SOURCES = ["hm_runtime.hip", "hm_router.hip", "hm_gemm.hip", "hm_gemm_mfma.hip",
                   "hm_gemm_f32_mfma.hip", "hm_op_gemm.hip", "hm_gemv.hip", "hm_block.hip", "hm_noalloc.hip",
-                  "hm_fp8_quantize.hip", "hm_fp8_gemm.hip", "hm_rows.hip"]
+                  "hm_fp8_quantize.hip", "hm_fp8_gemm.hip", "hm_fp8_tile.hip", "hm_rows.hip"]
 # Per-source flags.  The FP64 router MFMAs keep their accumulators in VGPRs
 # (otherwise the compiler copies them to AGPRs and back on every K chunk).
 SOURCE_FLAGS = {"hm_router.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
                 "hm_gemm_f32_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-                "hm_op_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+                "hm_op_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+                "hm_fp8_tile.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 # Sources with hand-written memory statements: LDS-DMA loads that set M0.
-CHECKED_SOURCES = {"hm_gemm_mfma.hip", "hm_router.hip", "hm_gemm_f32_mfma.hip"}
+CHECKED_SOURCES = {"hm_gemm_mfma.hip", "hm_router.hip", "hm_gemm_f32_mfma.hip", "hm_fp8_tile.hip"}
 HOST_SOURCES = ["hip_backend.cpp", "hip_tensor_backend.cpp", "moe_block.cpp", "artefact.cpp"]
 
 KERNELS_SO = LIB / "libhm_kernels.so"
