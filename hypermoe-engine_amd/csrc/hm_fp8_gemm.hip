@@ -111,6 +111,201 @@ int launch_stream(const Product& p, int64_t m_tiles16, T* y, hipStream_t s) {
     return HM_OK;
 }
 
+// ---- Experts of a few rows: two launches, each quantising what it multiplies.
+// A decode step reads every chosen expert's weights for a row or two; the rest is latency.  A workgroup
+// of 8 waves owns 8 / KP x 16 outputs (GU: gate and up) of up to 16 rows of one expert.  Its weights are
+// sent for first (KP waves split K, two blocks each in flight), then its rows are cut to 8 bits into the
+// LDS, 16 lanes a block, so that nothing is launched before or between the products; the waves' sums
+// meet in the LDS in wave order.
+struct Decode {
+    const void* x;
+    const uint8_t* w;
+    const float* ws;
+    const int32_t* perm;       // rows of x, nullptr: the grouped rows themselves
+    const int32_t* offsets;
+    void* y;
+    int64_t w_expert;
+    int ws_expert, experts, pairs, x_rows, K, N;
+    bool vec, wide;            // x takes 16-byte loads, y 4-element stores
+};
+
+// The 16-row tile `tile`, as locate() does; in a batch whose groups have at most 16 rows each it is the
+// tile-th expert with rows, found by ballots (128 experts a round, their offsets in one round trip).
+__device__ __forceinline__ bool locate16(const int32_t* __restrict__ offsets, int experts, int pairs,
+                                         int tile, Tile* t) {
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    for (int c0 = 0; c0 < experts; c0 += 128) {
+        int lo[2], hi[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int e = min(c0 + 64 * h + lane, experts - 1);
+            lo[h] = offsets[e];
+            hi[h] = offsets[e + 1];
+            if (c0 + 64 * h + lane >= experts) hi[h] = lo[h];
+        }
+        if (__ballot(hi[0] - lo[0] > 16 || hi[1] - lo[1] > 16))
+            return locate(offsets, experts, pairs, 16, tile, t);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            unsigned long long m = __ballot(hi[h] > lo[h]);
+            const int here = __popcll(m);
+            if (tile < base + here) {
+                for (int i = base; i < tile; ++i) m &= m - 1;
+                const int l = __builtin_amdgcn_readfirstlane(__ffsll((long long)m) - 1);
+                t->e = c0 + 64 * h + l;
+                t->row0 = __builtin_amdgcn_readlane(lo[h], l);
+                t->nrows = min(__builtin_amdgcn_readlane(hi[h], l), pairs) - t->row0;
+                return t->row0 >= 0 && t->nrows > 0;
+            }
+            base += here;
+        }
+    }
+    return false;
+}
+
+// Bytes of LDS of a decode workgroup for `rows` rows: each row's bytes (and 16, against bank conflicts),
+// then the scales.
+__host__ __device__ __forceinline__ int decode_stride(int K) { return (int)hm_f8_pitch(K) + 16; }
+__host__ __device__ __forceinline__ int decode_lds(int rows, int K) {
+    return rows * (decode_stride(K) + 4 * (int)hm_f8_blocks(K));
+}
+
+template <typename XT, bool GU, int KP, typename T>
+__global__ __launch_bounds__(64 * kSWaves, 4) void f8_decode_kernel(Decode p) {
+    constexpr int NP = GU ? 2 : 1, D = 2;   // D blocks in flight
+    extern __shared__ __attribute__((aligned(16))) uint8_t s_x[];
+    __shared__ __attribute__((aligned(16))) v4f s_part[kSWaves][NP][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int j = lane & 15, g = lane >> 4;
+    const int part = wave % KP;
+    const int n0 = 16 * ((int)blockIdx.x * (kSWaves / KP) + wave / KP);
+    // (the batch's rows of x, beside the offsets rather than after them)
+    const int rows_of = p.perm ? p.perm[min(lane, p.pairs - 1)] : 0;
+    Tile t;
+    if (!locate16(p.offsets, p.experts, p.pairs, blockIdx.y, &t)) return;
+    const int nb = (int)hm_f8_blocks(p.K), stride = decode_stride(p.K), nrows = (int)t.nrows;
+    const int64_t pitch = (int64_t)nb * kF8Block;
+    const uint8_t* w[NP];
+    const float* ws[NP];
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {  // columns past the last re-read it
+        w[q] = p.w + t.e * p.w_expert + ((int64_t)q * p.N + min(n0 + j, p.N - 1)) * pitch;
+        ws[q] = p.ws + (int64_t)t.e * p.ws_expert +
+                (q * (int)hm_f8_blocks(p.N) + min(n0, p.N - 1) / kF8Block) * nb;
+    }
+    v8i raw[D][NP];
+    float sw[D][NP];
+    auto load_w = [&](int b0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            const int b = min(b0 + d * KP, nb - 1);   // (past the last block: read again, not used)
+#pragma unroll
+            for (int q = 0; q < NP; ++q) {
+                raw[d][q] = load_frag(w[q] + b * kF8Block, g);
+                sw[d][q] = ws[q][b];
+            }
+        }
+    };
+    // unit u of the rows: block u % nb of row u / nb, 8 values a lane.  The first round's loads go out
+    // before the weights', which arrive later and in order.
+    const int units = nrows * nb;
+    float v[8];
+    auto load_unit = [&](int u) __attribute__((always_inline)) {
+        const int r = u / nb, k = (u - r * nb) * kF8Block + 8 * j;
+        int xr = p.perm ? __shfl(rows_of, (int)t.row0 + r, 64) : (int)t.row0 + r;
+        if (xr < 0 || xr >= p.x_rows) xr = 0;
+        const XT* x = static_cast<const XT*>(p.x) + (int64_t)xr * p.K + k;
+        if (p.vec && k + 8 <= p.K) {
+            constexpr int N = 16 / sizeof(XT);
+#pragma unroll
+            for (int i = 0; i < 8 / N; ++i) {
+                const hm_pack<XT, N> pk = reinterpret_cast<const hm_pack<XT, N>*>(x)[i];
+#pragma unroll
+                for (int q = 0; q < N; ++q) v[i * N + q] = (float)pk.v[q];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = k + i < p.K ? (float)x[i] : 0.0f;
+        }
+    };
+    float* s_scale = reinterpret_cast<float*>(s_x + nrows * stride);
+    auto store_unit = [&](int u) __attribute__((always_inline)) {
+        const int r = u / nb, k = (u - r * nb) * kF8Block + 8 * j;
+        float amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax = hm_f8_amax(amax, v[i]);
+        const hm_f8_scaler s = hm_f8_scaler_of(hm_row16_max(amax));
+        uint2 bytes;
+        bytes.x = hm_f8_pack4(s, v[0], v[1], v[2], v[3]);
+        bytes.y = hm_f8_pack4(s, v[4], v[5], v[6], v[7]);
+        *reinterpret_cast<uint2*>(s_x + r * stride + k) = bytes;
+        if (j == 0) s_scale[u] = s.scale;
+    };
+    // (past the last unit: that one again, the same bytes)
+    const int u0 = min((int)(threadIdx.x >> 4), units - 1);
+    load_unit(u0);
+    __builtin_amdgcn_sched_barrier(0);
+    load_w(part);
+    __builtin_amdgcn_sched_barrier(0);
+    store_unit(u0);
+    for (int u = 32 + (int)(threadIdx.x >> 4); u - (int)(threadIdx.x >> 4) < units; u += 32) {
+        load_unit(min(u, units - 1));
+        store_unit(min(u, units - 1));
+    }
+    __syncthreads();
+    const int row = min(j, nrows - 1);
+    const uint8_t* x = s_x + row * stride;
+    v4f acc[NP] = {};
+    for (int b0 = part; b0 < nb; b0 += D * KP) {
+        if (b0 != part) load_w(b0);
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            const int b = b0 + d * KP;
+            if (b >= nb) break;
+            Frag<true> fx, fw;
+            fx.set(load_frag(x + b * kF8Block, g));
+            const float sx = s_scale[row * nb + b];
+#pragma unroll
+            for (int q = 0; q < NP; ++q) {
+                fw.set(raw[d][q]);
+                const v4f r4 = block_product(fw, fx);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[q][i] = __builtin_fmaf(r4[i], sx * sw[d][q], acc[q][i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < NP; ++q) s_part[wave][q][lane] = acc[q];
+    __syncthreads();
+    if (part || n0 >= p.N || j >= nrows) return;
+#pragma unroll
+    for (int q = 0; q < NP; ++q)
+#pragma unroll
+        for (int i = 1; i < KP; ++i) acc[q] += s_part[wave + i][q][lane];
+    if constexpr (GU) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[0][i] = fast_silu(acc[0][i]) * acc[NP - 1][i];
+    }
+    store4(static_cast<T*>(p.y) + (t.row0 + j) * p.N, n0 + 4 * g, p.N, acc[0], p.wide);
+}
+
+template <typename XT, bool GU, typename T>
+int launch_decode(const Decode& p, hipStream_t s) {
+    // parts of two blocks each
+    const int64_t nb = hm_f8_blocks(p.K);
+    auto run = [&](auto kernel, int kp) {
+        const int cols = 16 * kSWaves / kp;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((p.N + cols - 1) / cols), (unsigned)p.pairs),
+                           dim3(64 * kSWaves), decode_lds(std::min(p.pairs, 16), p.K), s, p);
+    };
+    if (nb > 8) run(f8_decode_kernel<XT, GU, 8, T>, 8);
+    else if (nb > 4) run(f8_decode_kernel<XT, GU, 4, T>, 4);
+    else run(f8_decode_kernel<XT, GU, 2, T>, 2);
+    HM_LAUNCHED();
+    return HM_OK;
+}
+
 // Which kernel takes one matrix product: the one of least time, estimated as a start plus steps (blocks
 // of K) x rounds of workgroups x the measured time of a step, alone on its CU while the tiles do not
 // fill the chip and with all CUs busy beyond that (us).  Tiles of 64 x 128 and, for FP8 instructions,
@@ -164,7 +359,7 @@ constexpr size_t kAlign = 256;
 size_t align_up(size_t v) { return (v + kAlign - 1) & ~(kAlign - 1); }
 
 // The experts' workspace.  Tiles: the quantised rows of x, the bytes and scales of z, the m-tile table.
-// Streamed: z in floats besides.
+// Decode: z in floats.  Shapes without either (short or very large dimensions): all but the table.
 struct ExpertsPlan {
     uint8_t* xq;
     float* xs;
@@ -174,27 +369,32 @@ struct ExpertsPlan {
     int4* table;
 };
 
-// Few rows stream (a token or two: 21 and 27 us against 24 and 26 for tiles); others take tiles of 64 rows, or
-// 128 where an expert has that many on average (128 experts top-8, 2048 tokens: 194 us against 211; 1024:
-// 168 against 160).
-constexpr int64_t kStreamPairs = 8;
+// Up to kDecodePairs rows take the decode kernels; others tiles of 64 rows, or 128 where an expert has
+// that many on average (128 experts top-8, 2048 tokens: 194 us against 211; 1024: 168 against 160).
+constexpr int64_t kDecodePairs = 16;
+enum class Experts { kDecode, kTiles, kStream };
 struct ExpertsForm {
-    bool tiles;
+    Experts kind;
     int bm;
     int cap;      // upper bound of the m-tiles
 };
-Product gate_up(const hm_layer* L, int64_t tokens, int64_t pairs) {
-    return Product{nullptr, nullptr, nullptr, nullptr, 0, 0, reinterpret_cast<const int32_t*>(4), nullptr, pairs,
-                   tokens, L->hidden, L->intermediate, (int)L->experts, false};
-}
 ExpertsForm experts_form(const hm_layer* L, int64_t tokens, int64_t pairs) {
-    ExpertsForm f;
-    const Product gu = gate_up(L, tokens, pairs);
-    const Product dn = {nullptr, nullptr, nullptr, nullptr, 0, 0, nullptr, nullptr, pairs, pairs,
-                        L->intermediate, L->hidden, (int)L->experts, false};
-    f.tiles = pairs > kStreamPairs && hm_f8_tile_ok(gu, true) && hm_f8_tile_ok(dn, false);
-    f.bm = pairs >= 128 * L->experts ? 128 : 64;
-    f.cap = (int)(pairs / f.bm + std::min(L->experts, pairs));
+    ExpertsForm f = {Experts::kStream, 64, 0};
+    const int64_t H = L->hidden, I = L->intermediate;
+    static const int32_t gathered = 0;
+    Product gu = {}, dn = {};
+    gu.rows = dn.rows = dn.x_rows = pairs;
+    gu.x_rows = tokens;
+    gu.K = dn.N = H;
+    gu.N = dn.K = I;
+    gu.perm = &gathered;
+    if (pairs <= kDecodePairs && decode_lds(16, (int)std::max(H, I)) <= 65536) {
+        f.kind = Experts::kDecode;
+    } else if (hm_f8_tile_ok(gu, true) && hm_f8_tile_ok(dn, false)) {
+        f.kind = Experts::kTiles;
+        if (pairs >= 128 * L->experts) f.bm = 128;
+        f.cap = (int)(pairs / f.bm + std::min(L->experts, pairs));
+    }
     return f;
 }
 
@@ -208,12 +408,18 @@ size_t plan_experts(const hm_layer* L, int64_t tokens, int64_t pairs, char* base
     const ExpertsForm f = experts_form(L, tokens, pairs);
     const int64_t H = L->hidden, I = L->intermediate;
     ExpertsPlan q;
-    q.xq = reinterpret_cast<uint8_t*>(take((size_t)tokens * hm_f8_pitch(H)));
-    q.xs = reinterpret_cast<float*>(take((size_t)tokens * hm_f8_blocks(H) * sizeof(float)));
-    q.z = f.tiles ? nullptr : reinterpret_cast<float*>(take((size_t)pairs * I * sizeof(float)));
-    q.zq = reinterpret_cast<uint8_t*>(take((size_t)pairs * hm_f8_pitch(I)));
-    q.zs = reinterpret_cast<float*>(take((size_t)pairs * hm_f8_blocks(I) * sizeof(float)));
-    q.table = f.tiles ? reinterpret_cast<int4*>(take(((size_t)f.cap + 1) * sizeof(int4))) : nullptr;
+    q.table = nullptr;
+    q.z = nullptr;
+    q.xq = q.zq = nullptr;
+    q.xs = q.zs = nullptr;
+    if (f.kind != Experts::kTiles) q.z = reinterpret_cast<float*>(take((size_t)pairs * I * sizeof(float)));
+    if (f.kind != Experts::kDecode) {
+        q.xq = reinterpret_cast<uint8_t*>(take((size_t)tokens * hm_f8_pitch(H)));
+        q.xs = reinterpret_cast<float*>(take((size_t)tokens * hm_f8_blocks(H) * sizeof(float)));
+        q.zq = reinterpret_cast<uint8_t*>(take((size_t)pairs * hm_f8_pitch(I)));
+        q.zs = reinterpret_cast<float*>(take((size_t)pairs * hm_f8_blocks(I) * sizeof(float)));
+    }
+    if (f.kind == Experts::kTiles) q.table = reinterpret_cast<int4*>(take(((size_t)f.cap + 1) * sizeof(int4)));
     if (p) *p = q;
     return used;
 }
@@ -285,7 +491,23 @@ int hm_fp8_experts(const hm_layer* layer, const void* x, int32_t x_dtype, int64_
     Product dn = {ws.zq, ws.zs, packed + 2 * I * ph, layer->scale + 2 * hb * ib, per, 3 * hb * ib,
                   nullptr, offsets, pairs, pairs, I, H, (int)E, false};
     const size_t ysize = hm_row_dtype_size(y_dtype);
-    if (form.tiles) {
+    if (form.kind == Experts::kDecode) {
+        Decode d = {x, packed, layer->scale, perm_tokens, offsets, ws.z, per, (int)(3 * hb * ib), (int)E,
+                    (int)pairs, (int)tokens, (int)H, (int)I, false, I % 4 == 0};
+        const size_t xsize = hm_row_dtype_size(x_dtype);
+        d.vec = (uintptr_t)x % 16 == 0 && H * xsize % 16 == 0;
+        rc = x_dtype == HM_DTYPE_FP32   ? launch_decode<float, true, float>(d, s)
+             : x_dtype == HM_DTYPE_FP16 ? launch_decode<hm_f16, true, float>(d, s)
+                                        : launch_decode<hm_bf16, true, float>(d, s);
+        if (rc) return rc;
+        d = {ws.z, packed + 2 * I * ph, layer->scale + 2 * hb * ib, nullptr, offsets, y, per,
+             (int)(3 * hb * ib), (int)E, (int)pairs, (int)pairs, (int)I, (int)H, I % 4 == 0,
+             H % 4 == 0 && (uintptr_t)y % (4 * ysize) == 0};
+        return y_dtype == HM_DTYPE_FP32   ? launch_decode<float, false, float>(d, s)
+               : y_dtype == HM_DTYPE_FP16 ? launch_decode<float, false, hm_f16>(d, s)
+                                          : launch_decode<float, false, hm_bf16>(d, s);
+    }
+    if (form.kind == Experts::kTiles) {
         rc = hm_f8_launch_prepare(x, x_dtype, tokens, H, ws.xq, ws.xs, offsets, (int)E, (int)pairs,
                                   form.bm, form.cap, ws.table, s);
         if (rc) return rc;

@@ -75,6 +75,11 @@ __device__ __forceinline__ v4f block_product(const Frag<true>& a, const Frag<tru
     return c;
 }
 
+// g / (1 + e^-g) on the exponential and reciprocal units, a unit in the last place each.
+__device__ __forceinline__ float fast_silu(float g) {
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896f));
+}
+
 // Four consecutive outputs of a row, columns n .. n + 3 (those below cols).
 template <typename T>
 __device__ __forceinline__ void store4(T* y, int64_t n, int64_t cols, v4f v, bool wide) {

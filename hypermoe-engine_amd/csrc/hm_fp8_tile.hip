@@ -29,10 +29,6 @@ constexpr int kXcds = 8;
 constexpr int kTThreads = 512;
 constexpr int kSuper = 4;    // m-tiles walked together (one matrix)
 
-__device__ __forceinline__ float fast_silu(float g) {
-    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896f));
-}
-
 struct TileAt {
     int e, row0, nrows, n0;
 };
@@ -44,7 +40,7 @@ __device__ __forceinline__ P* uni(P* p) {
     return reinterpret_cast<P*>(((uint64_t)(uint32_t)uni((int)(v >> 32)) << 32) | (uint32_t)uni((int)v));
 }
 
-// Tile j: n-tiles of an m-tile lie together, for one matrix in groups of kSuper m-tiles.
+// Tile j: n-tiles of an m-tile lie together, for one matrix in groups of kSuper m-tiles.  (Per lane.)
 template <int BM, int TN>
 __device__ __forceinline__ TileAt tile_at(const Product& p, const int4* __restrict__ table, int j, int mt,
                                           int ntn) {
@@ -52,9 +48,9 @@ __device__ __forceinline__ TileAt tile_at(const Product& p, const int4* __restri
     if (table) {
         const int m = j / ntn;
         const int4 e = table[1 + m];
-        t.e = uni(e.x);
-        t.row0 = uni(e.y);
-        t.nrows = uni(e.z);
+        t.e = e.x;
+        t.row0 = e.y;
+        t.nrows = e.z;
         t.n0 = (j - m * ntn) * TN;
     } else {
         const int grp = j / (kSuper * ntn), first = grp * kSuper;
@@ -150,6 +146,9 @@ __global__ __launch_bounds__(kTThreads) void f8_tile_kernel(Product p, const int
     constexpr int STAGE = ROWS * kF8Block;
     constexpr int XA = XF >= 4 ? 2 : 1;        // fragments of x read ahead
     constexpr bool GATHER = GU;                // rows of x by perm, else consecutive
+    // store instructions that a wave issues at least for a whole tile
+    constexpr int STORES = GU ? XF : XF * 4 * WF * (int)sizeof(T) / 16;
+    static_assert((NS - 2) * (LPW + 1) + STORES < 64, "vmcnt range");
     static_assert(BM % 64 == 0 && (!GU || TN == kF8Block), "tile shape");
     __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * STAGE];
     __shared__ __attribute__((aligned(16))) float s_sc[NS][ROWS];
@@ -172,7 +171,19 @@ __global__ __launch_bounds__(kTThreads) void f8_tile_kernel(Product p, const int
     const int jend = min((int)(blockIdx.x % kXcds + 1) * per, total);
     if (jbeg >= jend) return;
 
-    auto info = [&](int j) __attribute__((always_inline)) { return tile_at<BM, TN>(p, table, j, mt, ntn); };
+    // The workgroup's tiles, one a lane, 64 at a time: a tile's place is a lane read, not a memory access
+    // and divisions at the head of every tile.
+    const int ntiles = (jend - jbeg + step - 1) / step;
+    TileAt mine;
+    auto list = [&](int first) __attribute__((always_inline)) {
+        mine = tile_at<BM, TN>(p, table, min(jbeg + (first + lane) * step, jend - 1), mt, ntn);
+    };
+    auto info = [&](int i) __attribute__((always_inline)) {
+        if ((i & 63) == 0) list(i);
+        const int l = i & 63;
+        return TileAt{__builtin_amdgcn_readlane(mine.e, l), __builtin_amdgcn_readlane(mine.row0, l),
+                      __builtin_amdgcn_readlane(mine.nrows, l), __builtin_amdgcn_readlane(mine.n0, l)};
+    };
 
     // ---- sources.  Lane l of DMA c of a wave: row 8 (wave + 8 c) + l / 8, position l % 8.
     const int lr = lane >> 3, pos = lane & 7;
@@ -310,7 +321,7 @@ __global__ __launch_bounds__(kTThreads) void f8_tile_kernel(Product p, const int
     };
 
     // ---- the stream
-    TileAt cur = info(jbeg);
+    TileAt cur = info(0);
     int m = 0;
     if constexpr (GATHER) {
         fetch_rows(cur, 0);
@@ -324,14 +335,17 @@ __global__ __launch_bounds__(kTThreads) void f8_tile_kernel(Product p, const int
     for (int i = 0; i < XF; ++i)
 #pragma unroll
         for (int k = 0; k < WF; ++k) acc[i][k] = v4f{};
-    int j = jbeg, slot = 0, ks = 0;
-    bool has_next = j + step < jend;
+    int tile = 0, slot = 0, ks = 0, stored = 0;
+    bool has_next = ntiles > 1;
     TileAt nxt = cur;
-    if (has_next) nxt = info(j + step);
+    if (has_next) nxt = info(1);
     while (true) {
         // this wave's loads of the stage have landed (at most the NS - 2 stages after it are in
         // flight), then every wave's; and every wave has read the slot that is refilled below
-        wait_vmcnt<(NS - 2) * (LPW + 1)>();
+        // (after a whole tile's stores, which are younger, they may be in flight too)
+        if (stored) wait_vmcnt<(NS - 2) * (LPW + 1) + STORES>();
+        else wait_vmcnt<(NS - 2) * (LPW + 1)>();
+        stored = 0;
         lds_barrier();
         int ahead = ks + NS - 1;
         if constexpr (GATHER) {
@@ -352,6 +366,7 @@ __global__ __launch_bounds__(kTThreads) void f8_tile_kernel(Product p, const int
         const int r0 = wm * 16 * XF + i16, c0 = cur.n0 + wn * 16 * SH + 4 * SH * g;
         if constexpr (GU) store_z<XF, WF, BM>(p, cur, acc, s_amax, zq, zs, r0, c0, wn, g);
         else store_y<XF, WF, T>(p, cur, acc, y, r0, c0);
+        stored = cur.nrows >= (wm + 1) * 16 * XF && (GU || (p.wide && cur.n0 + TN <= N));
         if (!has_next) break;
 #pragma unroll
         for (int i = 0; i < XF; ++i)
@@ -360,9 +375,8 @@ __global__ __launch_bounds__(kTThreads) void f8_tile_kernel(Product p, const int
         ks = 0;
         m ^= 1;
         cur = nxt;
-        j += step;
-        has_next = j + step < jend;
-        if (has_next) nxt = info(j + step);
+        has_next = ++tile + 1 < ntiles;
+        if (has_next) nxt = info(tile + 1);
     }
     wait_vmcnt<0>();  // the LDS is not given back under a load
 }
@@ -414,7 +428,7 @@ int launch_plain(int bm, int bn, const Product& p, const int4* table, int64_t m_
 
 bool hm_f8_tile_ok(const Product& p, bool gu) {
     const uint64_t pitch = (uint64_t)hm_f8_pitch(p.K), top = (uint64_t)1 << 32;
-    return p.K > 3 * kF8Block && p.rows < (int64_t)1 << 30 && p.N < (int64_t)1 << 28 &&
+    return p.K > 2 * kF8Block && p.rows < (int64_t)1 << 30 && p.N < (int64_t)1 << 28 &&
            (uint64_t)(gu ? 2 * p.N : p.N) * pitch < top && (!p.perm || (uint64_t)p.x_rows * pitch < top) &&
            256 * pitch < top;
 }

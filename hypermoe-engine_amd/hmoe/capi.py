@@ -108,6 +108,7 @@ SIGNATURES = {
 }
 
 _LIB: C.CDLL | None = None
+_FUNCTIONS: dict = {}  # name -> the library's function, bound once
 
 
 class HmError(RuntimeError):
@@ -135,16 +136,18 @@ def load() -> C.CDLL:
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args
+            _FUNCTIONS[name] = fn
         _LIB = lib
     return _LIB
 
 
 def call(name: str, *args) -> int:
     """Call a C-ABI function and raise HmError on a non-zero status."""
-    lib = load()
-    rc = getattr(lib, name)(*args)
-    if SIGNATURES[name][0] is c_i32 and name not in ("hm_abi_version", "hm_last_hip_error") and rc != 0:
-        raise HmError(name, rc, lib.hm_last_hip_error())
+    if _LIB is None:
+        load()
+    rc = _FUNCTIONS[name](*args)
+    if rc and SIGNATURES[name][0] is c_i32 and name not in ("hm_abi_version", "hm_last_hip_error"):
+        raise HmError(name, rc, _LIB.hm_last_hip_error())
     return rc
 
 
