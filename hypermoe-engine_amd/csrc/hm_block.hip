@@ -1,7 +1,7 @@
 // hm_block.hip -- the fused MoE block entry (MoERuntime::executeBatch,
 // src/core/runtime/MoERuntime.cpp:58-349, with every expert device
 // resident) and the host-side INT8 packer.
-#include "hm_device.h"
+#include "hm_fp8.h"
 
 #include <limits.h>
 #include <math.h>
@@ -116,6 +116,8 @@ struct BlockPlan {
     float* y;
     int32_t* status;
     int32_t* counters;  // decode: the fused select's completion counter
+    char* f8;           // FP8 layers: the experts' workspace
+    size_t f8_bytes;
 };
 
 // Decode-size INT8 blocks of at most HM_GEMV_MAX_PAIRS (token, expert) pairs
@@ -132,6 +134,9 @@ bool layer_valid(const hm_layer* L) {
     if (!L || !L->packed || L->experts <= 0 || L->hidden <= 0 || L->intermediate <= 0)
         return false;
     if (L->dtype == HM_DTYPE_INT8) return L->scale && L->zero_point;
+    if (L->dtype == HM_DTYPE_FP8)
+        return L->scale && (uintptr_t)L->packed % 16 == 0 && L->experts <= 1024 &&
+               L->hidden <= 1 << 24 && L->intermediate <= 1 << 24;
     return L->dtype == HM_DTYPE_FP32;
 }
 
@@ -152,7 +157,12 @@ size_t plan_block(const hm_layer* L, int64_t T, int32_t k, int32_t lx, int32_t l
     q.perm_weights = c.take<float>((size_t)P);
     q.slots = c.take<int32_t>((size_t)P);
     q.status = c.take<int32_t>(1);
-    if (use_gemv(L, T, k, flags)) {
+    if (L->dtype == HM_DTYPE_FP8) {
+        q.f8_bytes = hm_fp8_experts_workspace_bytes(L, T, P);
+        q.f8 = c.take<char>(q.f8_bytes);
+        // decode batches: the fused router's completion counter
+        if (T <= HM_GEMV_MAX_TOKENS) q.counters = c.take<int32_t>(1);
+    } else if (use_gemv(L, T, k, flags)) {
         q.zf = c.take<float>((size_t)P * I);
         q.counters = c.take<int32_t>(1);
     } else if (L->dtype == HM_DTYPE_INT8) {
@@ -282,7 +292,8 @@ int block_forward(const hm_layer* layer, const float* hidden, const float* route
     // activation digits
     const bool limb_decode = layer->dtype == HM_DTYPE_INT8 && !gemv &&
                              tokens <= HM_GEMV_MAX_TOKENS && p.counters && p.xdig;
-    const bool fuse = (gemv || gv32 || limb_decode) && H % 32 == 0 && E <= 1024 && top_k <= 64 &&
+    const bool f8_decode = layer->dtype == HM_DTYPE_FP8 && tokens <= HM_GEMV_MAX_TOKENS;
+    const bool fuse = (gemv || gv32 || limb_decode || f8_decode) && H % 32 == 0 && E <= 1024 && top_k <= 64 &&
                       P <= 1024;
     bool x_quantized = false;
     // one token on the GEMV path: the select runs inside the gate/up launch
@@ -341,7 +352,12 @@ int block_forward(const hm_layer* layer, const float* hidden, const float* route
         hm_timer() = {nullptr, nullptr};
         return r ? r : (kernel_timed ? HM_OK : mark(4));
     };
-    if (gemv) {
+    if (layer->dtype == HM_DTYPE_FP8) {
+        const hm_f8_experts_call call = {layer, hidden, HM_DTYPE_FP32, tokens, p.offsets, p.perm_tokens, P,
+                                         p.y, HM_DTYPE_FP32, p.f8, p.f8_bytes};
+        if ((rc = mark(3)) || (rc = hm_f8_experts_gate_up(call, s)) || (rc = mark(4))) return rc;
+        rc = hm_f8_experts_down(call, s);
+    } else if (gemv) {
         rc = gate_up([&] {
             return sel_gu ? hm_launch_select_gateup(hidden, router_w, top_k, route_bits, p.ids,
                                                     p.scores, status, p.route_ws, p.counts,

@@ -74,3 +74,20 @@ __device__ __forceinline__ float hm_f8_amax(float amax, float x) {
     const float m = fabsf(x);
     return m <= amax ? amax : (m == m ? m : __builtin_inff());
 }
+
+// One hm_fp8_experts call (hm_fp8_gemm.hip): its two stages, for the block to time them apart.
+struct hm_f8_experts_call {
+    const hm_layer* layer;
+    const void* x;
+    int32_t x_dtype;
+    int64_t tokens;
+    const int32_t* offsets;
+    const int32_t* perm_tokens;
+    int64_t pairs;
+    void* y;
+    int32_t y_dtype;
+    void* workspace;
+    size_t workspace_bytes;
+};
+int hm_f8_experts_gate_up(const hm_f8_experts_call& c, hipStream_t s);
+int hm_f8_experts_down(const hm_f8_experts_call& c, hipStream_t s);

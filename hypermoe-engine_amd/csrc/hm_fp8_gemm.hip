@@ -432,6 +432,107 @@ bool layer_ok(const hm_layer* L) {
 
 }  // namespace
 
+namespace {
+
+// The checks of an experts call, its form and its workspace.  *empty: nothing to do.
+int check_experts(const hm_f8_experts_call& c, ExpertsForm* form, ExpertsPlan* plan, bool* empty) {
+    const hm_layer* L = c.layer;
+    HM_REQUIRE(layer_ok(L) && c.x && c.offsets && c.perm_tokens && c.y && c.tokens >= 0 && c.pairs >= 0);
+    HM_REQUIRE(hm_row_dtype(c.x_dtype) && hm_row_dtype(c.y_dtype));
+    HM_REQUIRE((uintptr_t)c.x % hm_row_dtype_size(c.x_dtype) == 0 &&
+               (uintptr_t)c.y % hm_row_dtype_size(c.y_dtype) == 0 && (uintptr_t)c.offsets % 4 == 0 &&
+               (uintptr_t)c.perm_tokens % 4 == 0);
+    *empty = c.pairs == 0 || c.tokens == 0;
+    if (*empty) return HM_OK;
+    if (L->experts > 1024) return HM_ERR_UNSUPPORTED;
+    if (c.pairs > INT_MAX || c.tokens > INT_MAX || L->hidden > 1 << 24 || L->intermediate > 1 << 24)
+        return HM_ERR_OVERFLOW;
+    HM_REQUIRE(c.workspace);
+    char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(c.workspace) + kAlign - 1) &
+                                         ~(uintptr_t)(kAlign - 1));
+    const size_t need = plan_experts(L, c.tokens, c.pairs, base, plan);
+    HM_REQUIRE(c.workspace_bytes >= need + (size_t)(base - static_cast<char*>(c.workspace)));
+    *form = experts_form(L, c.tokens, c.pairs);
+    return HM_OK;
+}
+
+struct LayerDims {
+    int64_t H, I, E, ph, pi, hb, ib, per, scales;
+    explicit LayerDims(const hm_layer* L)
+        : H(L->hidden), I(L->intermediate), E(L->experts), ph(hm_f8_pitch(H)), pi(hm_f8_pitch(I)),
+          hb(hm_f8_blocks(H)), ib(hm_f8_blocks(I)), per(2 * I * ph + H * pi), scales(3 * hb * ib) {}
+};
+
+}  // namespace
+
+// z of every grouped row, in the form that the down projection reads.
+int hm_f8_experts_gate_up(const hm_f8_experts_call& c, hipStream_t s) {
+    ExpertsForm form;
+    ExpertsPlan ws;
+    bool empty;
+    int rc = check_experts(c, &form, &ws, &empty);
+    if (rc || empty) return rc;
+    const hm_layer* L = c.layer;
+    const LayerDims d(L);
+    const uint8_t* packed = static_cast<const uint8_t*>(L->packed);
+    if (form.kind == Experts::kDecode) {
+        const bool vec = (uintptr_t)c.x % 16 == 0 && d.H * hm_row_dtype_size(c.x_dtype) % 16 == 0;
+        const Decode p = {c.x, packed, L->scale, c.perm_tokens, c.offsets, ws.z, d.per, (int)d.scales,
+                          (int)d.E, (int)c.pairs, (int)c.tokens, (int)d.H, (int)d.I, vec, d.I % 4 == 0};
+        return c.x_dtype == HM_DTYPE_FP32   ? launch_decode<float, true, float>(p, s)
+               : c.x_dtype == HM_DTYPE_FP16 ? launch_decode<hm_f16, true, float>(p, s)
+                                            : launch_decode<hm_bf16, true, float>(p, s);
+    }
+    const Product gu = {ws.xq, ws.xs, packed, L->scale, d.per, d.scales, c.perm_tokens, c.offsets,
+                        c.pairs, c.tokens, d.H, d.I, (int)d.E, d.I % 4 == 0};
+    if (form.kind == Experts::kTiles) {
+        rc = hm_f8_launch_prepare(c.x, c.x_dtype, c.tokens, d.H, ws.xq, ws.xs, c.offsets, (int)d.E,
+                                  (int)c.pairs, form.bm, form.cap, ws.table, s);
+        if (rc) return rc;
+        // z goes to 8 bits, so what the FP8 instruction drops can move a byte of it by a step (1.4e-3 of
+        // a BF16 result, whose own rounding is 1.7e-3): only where its rate counts and y is BF16
+        const bool exact = c.y_dtype != HM_DTYPE_BF16 || c.pairs < 128 * d.E;
+        return hm_f8_launch_gateup_tiles(form.bm, exact, gu, ws.table, form.cap, ws.zq, ws.zs, s);
+    }
+    rc = hm_fp8_quantize(c.x, c.x_dtype, c.tokens, d.H, d.H, 1, 1, ws.xq, ws.xs, s);
+    if (rc) return rc;
+    if ((rc = launch_stream<true, false>(gu, c.pairs, ws.z, s))) return rc;
+    return hm_fp8_quantize(ws.z, HM_DTYPE_FP32, c.pairs, d.I, d.I, 1, 1, ws.zq, ws.zs, s);
+}
+
+int hm_f8_experts_down(const hm_f8_experts_call& c, hipStream_t s) {
+    ExpertsForm form;
+    ExpertsPlan ws;
+    bool empty;
+    const int rc = check_experts(c, &form, &ws, &empty);
+    if (rc || empty) return rc;
+    const hm_layer* L = c.layer;
+    const LayerDims d(L);
+    const uint8_t* packed = static_cast<const uint8_t*>(L->packed) + 2 * d.I * d.ph;
+    const float* scale = L->scale + 2 * d.hb * d.ib;
+    const size_t ysize = hm_row_dtype_size(c.y_dtype);
+    if (form.kind == Experts::kDecode) {
+        const Decode p = {ws.z, packed, scale, nullptr, c.offsets, c.y, d.per, (int)d.scales, (int)d.E,
+                          (int)c.pairs, (int)c.pairs, (int)d.I, (int)d.H, d.I % 4 == 0,
+                          d.H % 4 == 0 && (uintptr_t)c.y % (4 * ysize) == 0};
+        return c.y_dtype == HM_DTYPE_FP32   ? launch_decode<float, false, float>(p, s)
+               : c.y_dtype == HM_DTYPE_FP16 ? launch_decode<float, false, hm_f16>(p, s)
+                                            : launch_decode<float, false, hm_bf16>(p, s);
+    }
+    Product dn = {ws.zq, ws.zs, packed, scale, d.per, d.scales, nullptr, c.offsets, c.pairs, c.pairs,
+                  d.I, d.H, (int)d.E, false};
+    if (form.kind == Experts::kTiles) {
+        dn.wide = d.H * ysize % 16 == 0 && (uintptr_t)c.y % 16 == 0;
+        return hm_f8_launch_tiles(form.bm, 256, false, dn, ws.table, form.cap, c.y, c.y_dtype, s);
+    }
+    dn.wide = d.H % 4 == 0 && (uintptr_t)c.y % (4 * ysize) == 0;
+    switch (c.y_dtype) {
+    case HM_DTYPE_FP32: return launch_stream<false, false>(dn, c.pairs, static_cast<float*>(c.y), s);
+    case HM_DTYPE_FP16: return launch_stream<false, false>(dn, c.pairs, static_cast<hm_f16*>(c.y), s);
+    default: return launch_stream<false, false>(dn, c.pairs, static_cast<hm_bf16*>(c.y), s);
+    }
+}
+
 extern "C" {
 
 int hm_fp8_matmul(const uint8_t* xq, const float* xs, const uint8_t* wq, const float* ws,
@@ -454,8 +555,8 @@ int hm_fp8_matmul(const uint8_t* xq, const float* xs, const uint8_t* wq, const f
 }
 
 size_t hm_fp8_experts_workspace_bytes(const hm_layer* layer, int64_t tokens, int64_t pairs) {
-    if (!layer || layer->dtype != HM_DTYPE_FP8 || layer->hidden <= 0 || layer->intermediate <= 0 ||
-        tokens <= 0 || pairs <= 0)
+    if (!layer || layer->dtype != HM_DTYPE_FP8 || layer->experts <= 0 || layer->hidden <= 0 ||
+        layer->intermediate <= 0 || tokens <= 0 || pairs <= 0)
         return 0;
     return plan_experts(layer, tokens, pairs, nullptr, nullptr) + kAlign;
 }
@@ -463,73 +564,36 @@ size_t hm_fp8_experts_workspace_bytes(const hm_layer* layer, int64_t tokens, int
 int hm_fp8_experts(const hm_layer* layer, const void* x, int32_t x_dtype, int64_t tokens,
                    const int32_t* offsets, const int32_t* perm_tokens, int64_t pairs, void* y,
                    int32_t y_dtype, void* workspace, size_t workspace_bytes, void* stream) {
-    HM_REQUIRE(layer_ok(layer) && x && offsets && perm_tokens && y && tokens >= 0 && pairs >= 0);
-    HM_REQUIRE(hm_row_dtype(x_dtype) && hm_row_dtype(y_dtype));
-    HM_REQUIRE((uintptr_t)x % hm_row_dtype_size(x_dtype) == 0 &&
-               (uintptr_t)y % hm_row_dtype_size(y_dtype) == 0);
-    if (pairs == 0 || tokens == 0) return HM_OK;
-    if (layer->experts > 1024) return HM_ERR_UNSUPPORTED;
-    if (pairs > INT_MAX || tokens > INT_MAX || layer->hidden > 1 << 24 ||
-        layer->intermediate > 1 << 24)
-        return HM_ERR_OVERFLOW;
-    HM_REQUIRE(workspace);
-    char* base = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(workspace) + kAlign - 1) &
-                                         ~(uintptr_t)(kAlign - 1));
-    ExpertsPlan ws;
-    const size_t need = plan_experts(layer, tokens, pairs, base, &ws);
-    HM_REQUIRE(workspace_bytes >= need + (size_t)(base - static_cast<char*>(workspace)));
-    const int64_t H = layer->hidden, I = layer->intermediate, E = layer->experts;
-    const int64_t ph = hm_f8_pitch(H), pi = hm_f8_pitch(I);
-    const int64_t hb = hm_f8_blocks(H), ib = hm_f8_blocks(I);
-    const int64_t per = 2 * I * ph + H * pi;
-    const uint8_t* packed = static_cast<const uint8_t*>(layer->packed);
-    hipStream_t s = hm_stream(stream);
-    const ExpertsForm form = experts_form(layer, tokens, pairs);
-    int rc;
-    Product gu = {ws.xq, ws.xs, packed, layer->scale, per, 3 * hb * ib, perm_tokens, offsets,
-                  pairs, tokens, H, I, (int)E, I % 4 == 0};
-    Product dn = {ws.zq, ws.zs, packed + 2 * I * ph, layer->scale + 2 * hb * ib, per, 3 * hb * ib,
-                  nullptr, offsets, pairs, pairs, I, H, (int)E, false};
-    const size_t ysize = hm_row_dtype_size(y_dtype);
-    if (form.kind == Experts::kDecode) {
-        Decode d = {x, packed, layer->scale, perm_tokens, offsets, ws.z, per, (int)(3 * hb * ib), (int)E,
-                    (int)pairs, (int)tokens, (int)H, (int)I, false, I % 4 == 0};
-        const size_t xsize = hm_row_dtype_size(x_dtype);
-        d.vec = (uintptr_t)x % 16 == 0 && H * xsize % 16 == 0;
-        rc = x_dtype == HM_DTYPE_FP32   ? launch_decode<float, true, float>(d, s)
-             : x_dtype == HM_DTYPE_FP16 ? launch_decode<hm_f16, true, float>(d, s)
-                                        : launch_decode<hm_bf16, true, float>(d, s);
-        if (rc) return rc;
-        d = {ws.z, packed + 2 * I * ph, layer->scale + 2 * hb * ib, nullptr, offsets, y, per,
-             (int)(3 * hb * ib), (int)E, (int)pairs, (int)pairs, (int)I, (int)H, I % 4 == 0,
-             H % 4 == 0 && (uintptr_t)y % (4 * ysize) == 0};
-        return y_dtype == HM_DTYPE_FP32   ? launch_decode<float, false, float>(d, s)
-               : y_dtype == HM_DTYPE_FP16 ? launch_decode<float, false, hm_f16>(d, s)
-                                          : launch_decode<float, false, hm_bf16>(d, s);
+    const hm_f8_experts_call c = {layer, x, x_dtype, tokens, offsets, perm_tokens, pairs, y, y_dtype,
+                                  workspace, workspace_bytes};
+    const int rc = hm_f8_experts_gate_up(c, hm_stream(stream));
+    return rc ? rc : hm_f8_experts_down(c, hm_stream(stream));
+}
+
+int hm_fp8_pack_layer(const void* payload, int32_t dtype, int64_t experts, int64_t hidden,
+                      int64_t intermediate, void* packed, float* scale, void* stream) {
+    HM_REQUIRE(payload && packed && scale && payload != packed && experts > 0 && hidden > 0 &&
+               intermediate > 0 && hm_row_dtype(dtype));
+    HM_REQUIRE((uintptr_t)payload % hm_row_dtype_size(dtype) == 0 && (uintptr_t)packed % 16 == 0 &&
+               (uintptr_t)scale % 4 == 0);
+    if (hidden > 1 << 24 || intermediate > 1 << 24 || experts > 1 << 20) return HM_ERR_OVERFLOW;
+    const int64_t H = hidden, I = intermediate, blocks = hm_f8_blocks(H) * hm_f8_blocks(I);
+    uint8_t* q = static_cast<uint8_t*>(packed);
+    const char* src = static_cast<const char*>(payload);
+    const size_t matrix = (size_t)H * I * hm_row_dtype_size(dtype);
+    for (int64_t e = 0; e < experts; ++e) {
+        for (int p = 0; p < 3; ++p) {
+            // [K x N] row-major: output n's inner dimension runs at stride N
+            const int64_t K = p < 2 ? H : I, N = p < 2 ? I : H;
+            const int rc = hm_fp8_quantize(src, dtype, N, K, N == 1 ? K : 1, N == 1 ? 1 : N, kF8Block, q,
+                                           scale, stream);
+            if (rc) return rc;
+            src += matrix;
+            q += N * hm_f8_pitch(K);
+            scale += blocks;
+        }
     }
-    if (form.kind == Experts::kTiles) {
-        rc = hm_f8_launch_prepare(x, x_dtype, tokens, H, ws.xq, ws.xs, offsets, (int)E, (int)pairs,
-                                  form.bm, form.cap, ws.table, s);
-        if (rc) return rc;
-        // z goes to 8 bits, so what the FP8 instruction drops can move a byte of it by a step (1.4e-3 of
-        // a BF16 result, whose own rounding is 1.7e-3): only where its rate counts and y is BF16
-        const bool exact = y_dtype != HM_DTYPE_BF16 || pairs < 128 * E;
-        rc = hm_f8_launch_gateup_tiles(form.bm, exact, gu, ws.table, form.cap, ws.zq, ws.zs, s);
-        if (rc) return rc;
-        dn.wide = H * ysize % 16 == 0 && (uintptr_t)y % 16 == 0;
-        return hm_f8_launch_tiles(form.bm, 256, false, dn, ws.table, form.cap, y, y_dtype, s);
-    }
-    rc = hm_fp8_quantize(x, x_dtype, tokens, H, H, 1, 1, ws.xq, ws.xs, stream);
-    if (rc) return rc;
-    if ((rc = launch_stream<true, false>(gu, pairs, ws.z, s))) return rc;
-    rc = hm_fp8_quantize(ws.z, HM_DTYPE_FP32, pairs, I, I, 1, 1, ws.zq, ws.zs, stream);
-    if (rc) return rc;
-    dn.wide = H % 4 == 0 && (uintptr_t)y % (4 * ysize) == 0;
-    switch (y_dtype) {
-    case HM_DTYPE_FP32: return launch_stream<false, false>(dn, pairs, static_cast<float*>(y), s);
-    case HM_DTYPE_FP16: return launch_stream<false, false>(dn, pairs, static_cast<hm_f16*>(y), s);
-    default: return launch_stream<false, false>(dn, pairs, static_cast<hm_bf16*>(y), s);
-    }
+    return HM_OK;
 }
 
 }  // extern "C"

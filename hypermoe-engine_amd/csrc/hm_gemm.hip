@@ -819,6 +819,9 @@ size_t hm_packed_layer_bytes(int64_t experts, int64_t hidden, int64_t intermedia
     if (experts <= 0 || hidden <= 0 || intermediate <= 0) return 0;
     if (dtype == HM_DTYPE_INT8) return (size_t)experts * 3 * (size_t)hm_proj_bytes(hidden, intermediate);
     if (dtype == HM_DTYPE_FP32) return (size_t)experts * 3 * (size_t)hidden * (size_t)intermediate * 4;
+    if (dtype == HM_DTYPE_FP8)
+        return (size_t)experts * (2 * (size_t)intermediate * (size_t)hm_fp8_pitch(hidden) +
+                                  (size_t)hidden * (size_t)hm_fp8_pitch(intermediate));
     return 0;
 }
 

@@ -271,7 +271,7 @@ int hm_combine_rows_grad(const void* dout, const void* y, const int32_t* slots, 
                          void* dy, float* dweights, void* stream) {
     const int rc = check_rows(slots, weights, tokens, top_k, rows, width, dtype);
     if (rc) return rc;
-    HM_REQUIRE(dout && (dy || rows == 0) && dout != dy && y != dy);
+    HM_REQUIRE(dout && (dy || rows == 0) && dout != dy && (!y || y != dy));
     HM_REQUIRE(!dweights || ((y || rows == 0) && weights));
     const size_t size = hm_row_dtype_size(dtype);
     HM_REQUIRE(aligned(dout, size) && aligned(y, size) && aligned(dy, size) && aligned(dweights, 4));

@@ -63,6 +63,64 @@ class DeviceExpertLayer:
                                  self.zp.data_ptr() if self.int8 else None)
 
 
+    @classmethod
+    def _fp8(cls, packed, scale, experts: int, hidden: int, inter: int):
+        self = cls.__new__(cls)
+        self.experts, self.hidden, self.inter, self.int8 = experts, hidden, inter, False
+        self.dtype = capi.HM_DTYPE_FP8
+        self.packed, self.scale, self.zp = packed, scale, None
+        self.desc = capi.HmLayer(experts, hidden, inter, self.dtype, packed.data_ptr(),
+                                 scale.data_ptr(), None)
+        return self
+
+    @classmethod
+    def quantize_fp8(cls, payload, hidden: int, inter: int, stream=None):
+        """An FP8 layer (128 x 128 block scales) of a payload [E, 3, H*I] in
+        the reference layout: a float32 or float16 array, or a float32,
+        float16 or bfloat16 tensor on the device."""
+        torch = _torch()
+        if isinstance(payload, np.ndarray):
+            payload = torch.from_numpy(np.ascontiguousarray(payload)).to("cuda")
+        experts = payload.shape[0]
+        codes = {torch.float32: capi.HM_DTYPE_FP32, torch.float16: capi.HM_DTYPE_FP16,
+                 torch.bfloat16: capi.HM_DTYPE_BF16}
+        if payload.numel() != experts * 3 * hidden * inter or payload.dtype not in codes:
+            raise ValueError("payload does not match [E, 3, H*I] of float32, float16 or bfloat16")
+        payload = payload.contiguous()
+        with torch.cuda.device(payload.device):
+            nbytes = capi.load().hm_packed_layer_bytes(experts, hidden, inter, capi.HM_DTYPE_FP8)
+            packed = torch.empty(nbytes, dtype=torch.uint8, device=payload.device)
+            blocks = -(-hidden // capi.HM_FP8_BLOCK) * -(-inter // capi.HM_FP8_BLOCK)
+            scale = torch.empty((experts, 3, blocks), dtype=torch.float32, device=payload.device)
+            s = torch.cuda.current_stream().cuda_stream if stream is None else stream
+            capi.call("hm_fp8_pack_layer", payload.data_ptr(), codes[payload.dtype], experts, hidden,
+                      inter, packed.data_ptr(), scale.data_ptr(), s)
+            torch.cuda.synchronize()
+        return cls._fp8(packed, scale, experts, hidden, inter)
+
+    @classmethod
+    def from_fp8(cls, gate, up, down, gate_scale, up_scale, down_scale):
+        """An FP8 layer of a checkpoint's tensors: e4m3 (or uint8) weights
+        [E, out, in] on the device, gate and up [E, I, H], down [E, H, I], with
+        the float32 scale of each 128 x 128 block [E, ceil(out / 128),
+        ceil(in / 128)]."""
+        torch = _torch()
+        experts, inter, hidden = gate.shape
+        b = capi.HM_FP8_BLOCK
+        per, scales = [], []
+        for w, s, (n, k) in ((gate, gate_scale, (inter, hidden)), (up, up_scale, (inter, hidden)),
+                             (down, down_scale, (hidden, inter))):
+            if tuple(w.shape) != (experts, n, k) or w.element_size() != 1:
+                raise ValueError(f"FP8 weights must be [{experts}, {n}, {k}] bytes, got {tuple(w.shape)}")
+            if tuple(s.shape) != (experts, -(-n // b), -(-k // b)):
+                raise ValueError(f"block scales do not match [{experts}, {-(-n // b)}, {-(-k // b)}]")
+            w = torch.nn.functional.pad(w.view(torch.uint8), (0, -k % b))
+            per.append(w.reshape(experts, -1))
+            scales.append(s.to(torch.float32).reshape(experts, 1, -1))
+        return cls._fp8(torch.cat(per, dim=1), torch.cat(scales, dim=1).contiguous(), experts, hidden,
+                        inter)
+
+
 @dataclass
 class ExpertBatch:
     """ExpertBatch (src/experts/ExpertBatch.hpp:10-18)."""

@@ -100,6 +100,7 @@ SIGNATURES = {
     "hm_fp8_experts_workspace_bytes": (c_sz, [C.POINTER(HmLayer), c_i64, c_i64]),
     "hm_fp8_experts": (c_i32, [C.POINTER(HmLayer), vp, c_i32, c_i64, vp, vp, c_i64, vp, c_i32, vp,
                                c_sz, vp]),
+    "hm_fp8_pack_layer": (c_i32, [vp, c_i32, c_i64, c_i64, c_i64, vp, vp, vp]),
     "hm_dispatch_rows": (c_i32, [vp, vp, vp, c_i64, c_i32, c_i64, c_i64, c_i32, vp, vp]),
     "hm_dispatch_rows_grad": (c_i32, [vp, vp, vp, vp, c_i64, c_i32, c_i64, c_i64, c_i32, vp, vp, vp]),
     "hm_combine_rows": (c_i32, [vp, vp, vp, vp, c_i64, c_i32, c_i64, c_i64, c_i32, vp, vp]),

@@ -142,6 +142,42 @@ std::shared_ptr<DeviceExpertLayer> DeviceExpertLayer::fromPayload(
     return layer;
 }
 
+std::shared_ptr<DeviceExpertLayer> DeviceExpertLayer::quantizeFp8(
+    std::shared_ptr<backend::HipBackend> backend, std::span<const std::byte> payload,
+    std::size_t experts, std::size_t hidden, std::size_t intermediate) {
+    if (!backend) throw std::invalid_argument("expert layer requires a HIP backend");
+    if (experts == 0 || hidden == 0 || intermediate == 0) {
+        throw std::invalid_argument("expert layer dimensions must be nonzero");
+    }
+    const auto E = (int64_t)experts, H = (int64_t)hidden, I = (int64_t)intermediate;
+    const auto full = hm_packed_layer_bytes(E, H, I, HM_DTYPE_FP32);
+    const auto bytes = hm_packed_layer_bytes(E, H, I, HM_DTYPE_FP8);
+    if (full == 0 || bytes == 0) throw std::overflow_error("expert layer byte size overflow");
+    if (payload.size() != full) {
+        throw std::invalid_argument("expert payload size does not match [E x 3 x H x I] FP32");
+    }
+    const auto scales = 3 * experts * (std::size_t)(hm_fp8_pitch(H) / 128 * (hm_fp8_pitch(I) / 128));
+    auto layer = std::shared_ptr<DeviceExpertLayer>(new DeviceExpertLayer());
+    layer->backend_ = backend;
+    layer->experts_ = experts;
+    layer->hidden_ = hidden;
+    layer->intermediate_ = intermediate;
+    layer->dtype_ = DType::FP8;
+    layer->packed_ = std::make_unique<DeviceBuffer>(backend, bytes);
+    layer->scale_ = std::make_unique<DeviceBuffer>(backend, scales * sizeof(float));
+    auto stream = backend->computeStream();
+    DeviceBuffer staging(backend, full);
+    backend->copyToDevice(staging.data(), payload.data(), full, nullptr);
+    throwOnStatus(hm_fp8_pack_layer(staging.data(), HM_DTYPE_FP32, E, H, I, layer->packed_->data(),
+                                    static_cast<float*>(layer->scale_->data()), stream),
+                  "quantise expert layer");
+    backend->synchronize(stream);
+    layer->desc_ = std::make_unique<hm_layer>();
+    *layer->desc_ = hm_layer{E, H, I, HM_DTYPE_FP8, layer->packed_->data(),
+                             static_cast<const float*>(layer->scale_->data()), nullptr};
+    return layer;
+}
+
 // ---- HipMoEBlock -------------------------------------------------------------
 
 // Pinned host copies of the routing metadata and the device buffers they

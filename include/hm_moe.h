@@ -230,9 +230,9 @@ int hm_quantize_int8_host(const float* w /* host */, int64_t n,
  * 3*E*H*I elements of the same dtype. */
 typedef struct hm_layer {
     int64_t experts, hidden, intermediate;
-    int32_t dtype;              /* HM_DTYPE_INT8 or HM_DTYPE_FP32 */
-    const void* packed;         /* output of hm_pack_layer */
-    const float* scale;         /* [E x 3] {gate, up, down}, INT8 only */
+    int32_t dtype;              /* HM_DTYPE_INT8, HM_DTYPE_FP32 or HM_DTYPE_FP8 */
+    const void* packed;         /* output of hm_pack_layer; FP8: see F2 */
+    const float* scale;         /* INT8: [E x 3] {gate, up, down}; FP8: block scales (F2) */
     const int32_t* zero_point;  /* [E x 3], INT8 only */
 } hm_layer;
 size_t hm_packed_layer_bytes(int64_t experts, int64_t hidden,
@@ -252,6 +252,8 @@ int hm_pack_layer(const void* reference_payload, int64_t experts,
  * exact; the FP32 result is within 1e-4 of the reference W8A32 path for
  * limbs >= 2 and bit-exact against the build's CPU restatement.
  * FP32 experts use FP32 arithmetic (within 1e-3 of the reference).
+ * FP8 experts run as hm_fp8_experts does from FP32 rows to FP32 rows (F2);
+ * the limb arguments and the HM_EXEC_* bits of INT8 experts do not apply.
  *
  * Outputs (device, caller-owned; all but `out` may be NULL, in which case
  * the workspace copy is used):
@@ -398,6 +400,13 @@ int hm_fp8_matmul(const uint8_t* xq, const float* xs, const uint8_t* wq,
  * overlap in time need one each. */
 size_t hm_fp8_experts_workspace_bytes(const hm_layer* layer, int64_t tokens,
                                       int64_t pairs);
+/* An FP8 layer from a payload in the reference's layout (gate [H x I] | up
+ * [H x I] | down [I x H] per expert, as for hm_pack_layer; FP32, FP16 or
+ * BF16, on the device): `packed` (hm_packed_layer_bytes(..., HM_DTYPE_FP8)
+ * bytes, 16-byte aligned) and `scale` as above. */
+int hm_fp8_pack_layer(const void* payload, int32_t dtype, int64_t experts,
+                      int64_t hidden, int64_t intermediate, void* packed,
+                      float* scale, void* stream);
 int hm_fp8_experts(const hm_layer* layer, const void* x, int32_t x_dtype,
                    int64_t tokens, const int32_t* offsets,
                    const int32_t* perm_tokens, int64_t pairs, void* y,

@@ -138,6 +138,12 @@ public:
         std::shared_ptr<backend::HipBackend> backend, std::span<const std::byte> payload,
         std::size_t experts, std::size_t hidden, std::size_t intermediate, tensor::DType dtype,
         std::span<const ExpertQuantization> quantization = {});
+    // The same payload in FP32, quantised on the device to e4m3 with a scale
+    // for each 128 x 128 block (hm_fp8_pack_layer).  No counterpart in the
+    // reference.
+    static std::shared_ptr<DeviceExpertLayer> quantizeFp8(
+        std::shared_ptr<backend::HipBackend> backend, std::span<const std::byte> payload,
+        std::size_t experts, std::size_t hidden, std::size_t intermediate);
     ~DeviceExpertLayer();
 
     [[nodiscard]] std::size_t experts() const noexcept { return experts_; }

@@ -35,6 +35,7 @@ enum class DType : std::uint32_t {
     FP16 = 1,
     BF16 = 2,
     INT8 = 3,
+    FP8 = 4,  // e4m3 with block scales (hm_moe.h, F1); no counterpart in the reference
 };
 
 [[nodiscard]] constexpr std::size_t sizeOf(DType dtype) noexcept {
@@ -42,7 +43,8 @@ enum class DType : std::uint32_t {
     case DType::FP32: return 4;
     case DType::FP16:
     case DType::BF16: return 2;
-    case DType::INT8: return 1;
+    case DType::INT8:
+    case DType::FP8: return 1;
     }
     return 0;
 }

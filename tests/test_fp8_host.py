@@ -62,7 +62,7 @@ def test_experts_refusals():
     _refused("hm_fp8_experts", good, [
         (0, None, INVALID), (1, None, INVALID), (2, INT8, INVALID), (3, -1, INVALID), (4, None, INVALID),
         (5, None, INVALID), (6, -1, INVALID), (7, None, INVALID), (8, FP8, INVALID), (9, None, INVALID),
-        (10, need - 4096, INVALID), (1, D + 1, INVALID), (6, 1 << 40, OVERFLOW)])
+        (10, need - 257, INVALID), (1, D + 1, INVALID), (6, 1 << 40, OVERFLOW)])
     for field, value, status in (("dtype", INT8, INVALID), ("packed", None, INVALID),
                                  ("scale", None, INVALID), ("packed", A + 8, INVALID),
                                  ("hidden", 0, INVALID), ("experts", 2000, UNSUPPORTED)):
