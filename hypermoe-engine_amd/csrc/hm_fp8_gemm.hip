@@ -307,18 +307,20 @@ int launch_decode(const Decode& p, hipStream_t s) {
 }
 
 // Which kernel takes one matrix product: the one of least time, estimated as a start plus steps (blocks
-// of K) x rounds of workgroups x the measured time of a step, alone on its CU while the tiles do not
-// fill the chip and with all CUs busy beyond that (us).  Tiles of 64 x 128 and, for FP8 instructions,
-// 128 x 128 sit two to a CU.  2048 x 2048 x K: 64 x 128 tiles 54 us at K = 8192, 128 x 256 58, 256 x 256
-// 93; 4096 x 4096: 104, 72 and 63 at K = 4096.  The stream kernel has no ring to fill: 16 rows of
-// 2048 x 2048 7 us against 8 for the smallest tile, 333 x 1000 x 777 (FP32) 7.3 against 10.5.
+// of K) x rounds of workgroups x the measured time of a step (us): of a workgroup alone on the chip, of
+// one on every CU (between them by the share of CUs at work: clocks and L2 are shared), and of two on
+// every CU where the form's LDS lets them.  The constants fit 14 shapes of K = 1024 and 4096 within 20 %.
+// 2048 x 2048 x 4096: 64 x 128 tiles 29 us, 128 x 128 34, 128 x 256 34, 256 x 256 50; 4096 x 4096: 111, 88,
+// 76 and 66.  The stream kernel has no ring to fill: 16 rows of 2048 x 2048 7 us against 8 for the smallest
+// tile, 333 x 777 x 4096 (FP32) 21 against 28.
 struct Form {
     int bm, bn, per_cu;
-    double alone, shared;
+    double alone, every, shared;
 };
-constexpr Form kFast[] = {{256, 256, 1, 1.35, 1.71}, {128, 256, 1, 0.79, 0.99},
-                          {128, 128, 2, 0.58, 1.14}, {64, 128, 2, 0.41, 0.85}};
-constexpr Form kExact[] = {{128, 256, 1, 1.9, 2.1}, {128, 128, 1, 1.3, 1.4}, {64, 128, 2, 0.85, 1.24}};
+constexpr Form kFast[] = {{256, 256, 1, 1.43, 1.95, 1.95}, {128, 256, 1, 0.92, 1.1, 1.1},
+                          {128, 128, 2, 0.58, 0.95, 1.3}, {64, 128, 2, 0.44, 0.47, 0.82}};
+constexpr Form kExact[] = {{128, 256, 1, 1.9, 2.1, 2.1}, {128, 128, 1, 1.2, 1.2, 1.2},
+                           {64, 128, 2, 0.8, 0.84, 1.27}};
 constexpr int kCus = 256;
 
 // nullptr: the stream kernel
@@ -333,7 +335,8 @@ const Form* choose_form(const Product& p, bool exact) {
         const Form& f = forms[i];
         const int64_t tiles = ((p.rows + f.bm - 1) / f.bm) * ((p.N + f.bn - 1) / f.bn);
         const int64_t rounds = (tiles + kCus * f.per_cu - 1) / (kCus * f.per_cu);
-        const double t = 4.0 + steps * (tiles <= kCus ? f.alone : rounds * f.shared);
+        const double t = 4.0 + steps * (tiles <= kCus ? f.alone + (f.every - f.alone) * tiles / kCus
+                                                      : rounds * f.shared);
         if (t < best) {
             best = t;
             form = &f;
@@ -370,7 +373,9 @@ struct ExpertsPlan {
 };
 
 // Up to kDecodePairs rows take the decode kernels; others tiles of 64 rows, or 128 where an expert has
-// that many on average (128 experts top-8, 2048 tokens: 194 us against 211; 1024: 168 against 160).
+// that many on average (128 experts top-8, 2048 tokens: 194 us against 211; 1024: 168 against 160), or, with
+// the FP8 instruction, 256 from 384 rows an expert (6144 tokens: 367 us against 395; 4096: 315 against 293;
+// 8 experts top-2 of 4096 x 2048, 16384 tokens: 932 us, 1.77 PFLOP/s, against 1079).
 constexpr int64_t kDecodePairs = 16;
 enum class Experts { kDecode, kTiles, kStream };
 struct ExpertsForm {
@@ -378,7 +383,7 @@ struct ExpertsForm {
     int bm;
     int cap;      // upper bound of the m-tiles
 };
-ExpertsForm experts_form(const hm_layer* L, int64_t tokens, int64_t pairs) {
+ExpertsForm experts_form(const hm_layer* L, int64_t tokens, int64_t pairs, bool exact) {
     ExpertsForm f = {Experts::kStream, 64, 0};
     const int64_t H = L->hidden, I = L->intermediate;
     static const int32_t gathered = 0;
@@ -392,7 +397,7 @@ ExpertsForm experts_form(const hm_layer* L, int64_t tokens, int64_t pairs) {
         f.kind = Experts::kDecode;
     } else if (hm_f8_tile_ok(gu, true) && hm_f8_tile_ok(dn, false)) {
         f.kind = Experts::kTiles;
-        if (pairs >= 128 * L->experts) f.bm = 128;
+        if (pairs >= 128 * L->experts) f.bm = !exact && pairs >= 384 * L->experts ? 256 : 128;
         f.cap = (int)(pairs / f.bm + std::min(L->experts, pairs));
     }
     return f;
@@ -405,7 +410,7 @@ size_t plan_experts(const hm_layer* L, int64_t tokens, int64_t pairs, char* base
         used += align_up(bytes);
         return at;
     };
-    const ExpertsForm f = experts_form(L, tokens, pairs);
+    const ExpertsForm f = experts_form(L, tokens, pairs, true);  // of the two the one with more m-tiles
     const int64_t H = L->hidden, I = L->intermediate;
     ExpertsPlan q;
     q.table = nullptr;
@@ -434,6 +439,12 @@ bool layer_ok(const hm_layer* L) {
 
 namespace {
 
+// z goes to 8 bits, so what the FP8 instruction drops can move a byte of it by a step (1.4e-3 of a BF16
+// result, whose own rounding is 1.7e-3): taken only where its rate counts and y is BF16.
+bool exact_z(const hm_f8_experts_call& c) {
+    return c.y_dtype != HM_DTYPE_BF16 || c.pairs < 128 * c.layer->experts;
+}
+
 // The checks of an experts call, its form and its workspace.  *empty: nothing to do.
 int check_experts(const hm_f8_experts_call& c, ExpertsForm* form, ExpertsPlan* plan, bool* empty) {
     const hm_layer* L = c.layer;
@@ -452,7 +463,7 @@ int check_experts(const hm_f8_experts_call& c, ExpertsForm* form, ExpertsPlan* p
                                          ~(uintptr_t)(kAlign - 1));
     const size_t need = plan_experts(L, c.tokens, c.pairs, base, plan);
     HM_REQUIRE(c.workspace_bytes >= need + (size_t)(base - static_cast<char*>(c.workspace)));
-    *form = experts_form(L, c.tokens, c.pairs);
+    *form = experts_form(L, c.tokens, c.pairs, exact_z(c));
     return HM_OK;
 }
 
@@ -489,10 +500,7 @@ int hm_f8_experts_gate_up(const hm_f8_experts_call& c, hipStream_t s) {
         rc = hm_f8_launch_prepare(c.x, c.x_dtype, c.tokens, d.H, ws.xq, ws.xs, c.offsets, (int)d.E,
                                   (int)c.pairs, form.bm, form.cap, ws.table, s);
         if (rc) return rc;
-        // z goes to 8 bits, so what the FP8 instruction drops can move a byte of it by a step (1.4e-3 of
-        // a BF16 result, whose own rounding is 1.7e-3): only where its rate counts and y is BF16
-        const bool exact = c.y_dtype != HM_DTYPE_BF16 || c.pairs < 128 * d.E;
-        return hm_f8_launch_gateup_tiles(form.bm, exact, gu, ws.table, form.cap, ws.zq, ws.zs, s);
+        return hm_f8_launch_gateup_tiles(form.bm, exact_z(c), gu, ws.table, form.cap, ws.zq, ws.zs, s);
     }
     rc = hm_fp8_quantize(c.x, c.x_dtype, c.tokens, d.H, d.H, 1, 1, ws.xq, ws.xs, s);
     if (rc) return rc;

@@ -19,8 +19,8 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
-typedef __bf16 v2b __attribute__((ext_vector_type(2)));
-typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ v4f mfma_f8(v8i a, v8i b, v4f c) {
     // formats 0, 0: e4m3; no block exponents
@@ -39,8 +39,8 @@ __device__ __forceinline__ v8i load_frag(const uint8_t* block, int g) {
 // The FP8 instruction aligns each eight consecutive products to the largest of them and drops what
 // lies more than 13 bits below it (measured: 2^16 + 2^2 is 2^16 inside a group of eight and exact
 // across groups), 1.3e-5 to 2.4e-5 of a sum's norm: under a sixth of FP16's rounding step and a
-// hundredth of BF16's, but 300 times FP32's.  Where that shows, the operands are widened to bf16
-// (exact) for v_mfma_f32_16x16x32_bf16, whose sums are FP32 (1e-8), at half the rate: Frag<true>.
+// hundredth of BF16's, but 300 times FP32's.  Where that shows, the operands are widened to fp16 (exact)
+// for v_mfma_f32_16x16x32_f16, whose sums are FP32 (1e-8), at half the rate: Frag<true>.
 template <bool PREC>
 struct Frag;
 template <>
@@ -50,17 +50,17 @@ struct Frag<false> {
 };
 template <>
 struct Frag<true> {
-    v8b v[4];
+    v8h v[4];
     __device__ __forceinline__ void set(v8i f) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            v2b w[4];
+            v2h w[4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                w[2 * h] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)f[2 * i + h], 1.0f, false);
-                w[2 * h + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)f[2 * i + h], 1.0f, true);
+                w[2 * h] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((unsigned)f[2 * i + h], 1.0f, false);
+                w[2 * h + 1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((unsigned)f[2 * i + h], 1.0f, true);
             }
-            v[i] = v8b{w[0][0], w[0][1], w[1][0], w[1][1], w[2][0], w[2][1], w[3][0], w[3][1]};
+            v[i] = v8h{w[0][0], w[0][1], w[1][0], w[1][1], w[2][0], w[2][1], w[3][0], w[3][1]};
         }
     }
 };
@@ -71,7 +71,7 @@ __device__ __forceinline__ v4f block_product(const Frag<false>& a, const Frag<fa
 __device__ __forceinline__ v4f block_product(const Frag<true>& a, const Frag<true>& b) {
     v4f c = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b.v[i], c, 0, 0, 0);
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v[i], b.v[i], c, 0, 0, 0);
     return c;
 }
 

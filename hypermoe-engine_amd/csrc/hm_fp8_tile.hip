@@ -89,14 +89,25 @@ __device__ __forceinline__ void store_y(const Product& p, const TileAt& t, const
         }
     }
 }
+// Maximum over the lanes of one column, l % 16 (the four lane groups).
+__device__ __forceinline__ float column_max(float v) {
+    const unsigned u = __float_as_uint(v);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const unsigned w = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+    const auto b = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 // z = silu(gate) up and its quantisation (one block of 128 columns; s_amax: a maximum for each of the
-// four waves of a row).  Every wave of the workgroup calls it.
+// four waves of a row).  Every wave of the workgroup calls it.  The matrix instructions stand still
+// meanwhile, so it is kept short: z carries FP32 noise of a few units in the last place, and the scale
+// and the bytes' quotients go by one reciprocal instead of divisions.
 template <int XF, int WF, int BM>
 __device__ __forceinline__ void store_z(const Product& p, const TileAt& t, v4f (&acc)[XF][WF],
                                         float (&s_amax)[4][BM], uint8_t* zq, float* zs, int r0, int c0,
                                         int wn, int g) {
     constexpr int SH = WF / 2;
     const int N = (int)p.N, nbn = (int)hm_f8_blocks(p.N);
+    const bool whole = t.n0 + kF8Block <= N;
 #pragma unroll
     for (int i = 0; i < XF; ++i) {
         float amax = 0.0f, bad = 0.0f;
@@ -104,32 +115,37 @@ __device__ __forceinline__ void store_z(const Product& p, const TileAt& t, v4f (
         for (int q = 0; q < SH; ++q)
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-                const float z = c0 + 4 * q + v < N ? fast_silu(acc[i][q][v]) * acc[i][SH + q][v] : 0.0f;
+                float z = fast_silu(acc[i][q][v]) * acc[i][SH + q][v];
+                if (!whole) z = c0 + 4 * q + v < N ? z : 0.0f;
                 acc[i][q][v] = z;
                 amax = fmaxf(amax, fabsf(z));
                 bad = __builtin_fmaf(z, 0.0f, bad);  // NaN from an infinity or a NaN
             }
-        amax = bad == 0.0f ? amax : __builtin_inff();
-        amax = fmaxf(amax, __shfl_xor(amax, 16, 64));
-        amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+        amax = column_max(bad == 0.0f ? amax : __builtin_inff());
         if (g == 0) s_amax[wn][r0 + 16 * i] = amax;
     }
     lds_barrier();
 #pragma unroll
     for (int i = 0; i < XF; ++i) {
         const int r = r0 + 16 * i;
-        const hm_f8_scaler s = hm_f8_scaler_of(
-            fmaxf(fmaxf(s_amax[0][r], s_amax[1][r]), fmaxf(s_amax[2][r], s_amax[3][r])));
+        const float amax = fmaxf(fmaxf(s_amax[0][r], s_amax[1][r]), fmaxf(s_amax[2][r], s_amax[3][r]));
         if (r >= t.nrows) continue;
+        const bool finite = amax < __builtin_inff();
+        const float m = fmaxf(amax, kF8Tiny), inv = kF8Top * __builtin_amdgcn_rcpf(m);
         uint32_t w[SH];
 #pragma unroll
-        for (int q = 0; q < SH; ++q)
-            w[q] = hm_f8_pack4(s, acc[i][q][0], acc[i][q][1], acc[i][q][2], acc[i][q][3]);
+        for (int q = 0; q < SH; ++q) {
+            int b = __builtin_amdgcn_cvt_pk_fp8_f32(acc[i][q][0] * inv, acc[i][q][1] * inv, 0, false);
+            b = __builtin_amdgcn_cvt_pk_fp8_f32(acc[i][q][2] * inv, acc[i][q][3] * inv, b, true);
+            w[q] = finite ? (uint32_t)b : 0x7f7f7f7fu;
+        }
         const int64_t row = t.row0 + r;
-        uint32_t* to = reinterpret_cast<uint32_t*>(zq + row * (nbn * kF8Block) + c0);
+        hm_pack<uint32_t, SH> out;
 #pragma unroll
-        for (int q = 0; q < SH; ++q) to[q] = w[q];
-        if (wn == 0 && g == 0) zs[row * nbn + t.n0 / kF8Block] = s.scale;
+        for (int q = 0; q < SH; ++q) out.v[q] = w[q];
+        *reinterpret_cast<hm_pack<uint32_t, SH>*>(zq + row * (nbn * kF8Block) + c0) = out;
+        if (wn == 0 && g == 0)
+            zs[row * nbn + t.n0 / kF8Block] = finite ? m * (1.0f / kF8Top) : __builtin_nanf("");
     }
 }
 
@@ -417,9 +433,11 @@ int launch_plain(int bm, int bn, const Product& p, const int4* table, int64_t m_
     if constexpr (!PREC) {
         if (bm == 256) return launch<8, 4, 2, false, BROW, PREC, T>(p, table, m_tiles, out, nullptr, nullptr, s);
     }
-    if (bn == 256)
-        return bm == 128 ? launch<4, 4, 3, false, BROW, PREC, T>(p, table, m_tiles, out, nullptr, nullptr, s)
-                         : launch<2, 4, 3, false, BROW, PREC, T>(p, table, m_tiles, out, nullptr, nullptr, s);
+    if constexpr (!BROW) {  // the experts' down projection
+        if (bm == 64 && bn == 256)
+            return launch<2, 4, 3, false, BROW, PREC, T>(p, table, m_tiles, out, nullptr, nullptr, s);
+    }
+    if (bn == 256) return launch<4, 4, 3, false, BROW, PREC, T>(p, table, m_tiles, out, nullptr, nullptr, s);
     return bm == 128 ? launch<4, 2, 2, false, BROW, PREC, T>(p, table, m_tiles, out, nullptr, nullptr, s)
                      : launch<2, 2, 3, false, BROW, PREC, T>(p, table, m_tiles, out, nullptr, nullptr, s);
 }

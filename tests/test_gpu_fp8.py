@@ -313,7 +313,8 @@ def _check_experts(y, xv, w, perm, offsets, h, i, ydtype):
 @pytest.mark.parametrize("xdtype,ydtype", [("bf16", "bf16"), ("f16", "f16"), ("f16", "f32"), ("bf16", "f32")])
 @pytest.mark.parametrize("tokens,top_k,e,h,i", [(1, 2, 4, 256, 128), (3, 8, 16, 384, 256), (16, 4, 8, 200, 100),
                                                 (40, 3, 5, 512, 384), (150, 2, 3, 300, 500), (400, 4, 6, 512, 256),
-                                                (90, 2, 70, 640, 520), (300, 3, 5, 401, 600), (700, 2, 4, 520, 384)])
+                                                (90, 2, 70, 640, 520), (300, 3, 5, 401, 600), (700, 2, 4, 520, 384),
+                                                (900, 2, 4, 272, 300)])
 def test_experts(dev, xdtype, ydtype, tokens, top_k, e, h, i):
     print(f"[gpu] fp8 experts T={tokens} k={top_k} E={e} H={h} I={i} {xdtype}->{ydtype}", flush=True)
     rng = np.random.default_rng(tokens + e)
