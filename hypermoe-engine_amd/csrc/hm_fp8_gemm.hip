@@ -312,27 +312,29 @@ int launch_decode(const Decode& p, hipStream_t s) {
 // every CU where the form's LDS lets them.  The constants fit 14 shapes of K = 1024 and 4096 within 20 %.
 // 2048 x 2048 x 4096: 64 x 128 tiles 29 us, 128 x 128 34, 128 x 256 34, 256 x 256 50; 4096 x 4096: 111, 88,
 // 76 and 66.  The stream kernel has no ring to fill: 16 rows of 2048 x 2048 7 us against 8 for the smallest
-// tile, 333 x 777 x 4096 (FP32) 21 against 28.
+// tile, 333 x 777 x 4096 (FP32) 21 against 28, 16 x 2048 x 256 2.9 against 4.1 (kernel alone); but it reads
+// w again for every 64 rows: 4096 x 4096 x 256 76 us against 12.
 struct Form {
-    int bm, bn, per_cu;
+    int bm, bn, per_cu, min_blocks;
     double alone, every, shared;
 };
-constexpr Form kFast[] = {{256, 256, 1, 1.43, 1.95, 1.95}, {128, 256, 1, 0.92, 1.1, 1.1},
-                          {128, 128, 2, 0.58, 0.95, 1.3}, {64, 128, 2, 0.44, 0.47, 0.82}};
-constexpr Form kExact[] = {{128, 256, 1, 1.9, 2.1, 2.1}, {128, 128, 1, 1.2, 1.2, 1.2},
-                           {64, 128, 2, 0.8, 0.84, 1.27}};
+constexpr Form kFast[] = {{256, 256, 1, 1, 1.43, 1.95, 1.95}, {128, 256, 1, 2, 0.92, 1.1, 1.1},
+                          {128, 128, 2, 1, 0.58, 0.95, 1.3}, {64, 128, 2, 2, 0.44, 0.47, 0.82}};
+constexpr Form kExact[] = {{128, 256, 1, 2, 1.9, 2.1, 2.1}, {128, 128, 1, 1, 1.2, 1.2, 1.2},
+                           {64, 128, 2, 2, 0.8, 0.84, 1.27}};
 constexpr int kCus = 256;
 
 // nullptr: the stream kernel
 const Form* choose_form(const Product& p, bool exact) {
     const double steps = (double)hm_f8_blocks(p.K);
     const double groups = (double)((p.N + 15) / 16) * (double)((p.rows + 63) / 64);
-    double best = 4.7 + steps / 16 * (groups <= kCus ? 4.0 : groups / (2 * kCus) * 12.0);
+    double best = groups <= kCus ? 3.0 + steps / 16 * 4.0 : 4.7 + steps / 16 * groups / (2 * kCus) * 12.0;
     const Form* form = nullptr;
     if (!hm_f8_tile_ok(p, false)) return nullptr;
     const Form* forms = exact ? kExact : kFast;
     for (int i = 0; i < (exact ? 3 : 4); ++i) {
         const Form& f = forms[i];
+        if (steps < f.min_blocks) continue;
         const int64_t tiles = ((p.rows + f.bm - 1) / f.bm) * ((p.N + f.bn - 1) / f.bn);
         const int64_t rounds = (tiles + kCus * f.per_cu - 1) / (kCus * f.per_cu);
         const double t = 4.0 + steps * (tiles <= kCus ? f.alone + (f.every - f.alone) * tiles / kCus
@@ -395,7 +397,7 @@ ExpertsForm experts_form(const hm_layer* L, int64_t tokens, int64_t pairs, bool 
     gu.perm = &gathered;
     if (pairs <= kDecodePairs && decode_lds(16, (int)std::max(H, I)) <= 65536) {
         f.kind = Experts::kDecode;
-    } else if (hm_f8_tile_ok(gu, true) && hm_f8_tile_ok(dn, false)) {
+    } else if (hm_f8_tile_ok(gu, true) && hm_f8_tile_ok(dn, false) && I > kF8Block) {
         f.kind = Experts::kTiles;
         if (pairs >= 128 * L->experts) f.bm = !exact && pairs >= 384 * L->experts ? 256 : 128;
         f.cap = (int)(pairs / f.bm + std::min(L->experts, pairs));

@@ -147,7 +147,9 @@ __device__ __forceinline__ bool locate(const int32_t* __restrict__ offsets, int 
 
 // The tile kernels (hm_fp8_tile.hip).  table: the m-tiles of a grouped product (entry 0: their number
 // in x; then {expert, first row, rows}) and m_tiles an upper bound of them, or nullptr and the m-tiles of
-// one matrix.  bm: rows of x per tile, 64, 128 or (16-bit results) 256; bn: 128 or 256 rows of w.
+// one matrix.  bm: rows of x per tile, 64, 128 or (16-bit results) 256; bn: 128 or 256 rows of w.  Rings of
+// three stages (64 x 128, 64 x 256, 128 x 256) need two blocks of K, gathered rows three: a stage of the
+// next tile is the first to go out in the last two steps, gathered rows are fetched one step before.
 bool hm_f8_tile_ok(const Product& p, bool gu);
 int hm_f8_launch_tiles(int bm, int bn, bool brow, const Product& p, const int4* table, int64_t m_tiles,
                        void* y, int32_t dtype, hipStream_t s);

@@ -446,7 +446,7 @@ int launch_plain(int bm, int bn, const Product& p, const int4* table, int64_t m_
 
 bool hm_f8_tile_ok(const Product& p, bool gu) {
     const uint64_t pitch = (uint64_t)hm_f8_pitch(p.K), top = (uint64_t)1 << 32;
-    return p.K > 2 * kF8Block && p.rows < (int64_t)1 << 30 && p.N < (int64_t)1 << 28 &&
+    return (!gu || p.K > 2 * kF8Block) && p.rows < (int64_t)1 << 30 && p.N < (int64_t)1 << 28 &&
            (uint64_t)(gu ? 2 * p.N : p.N) * pitch < top && (!p.perm || (uint64_t)p.x_rows * pitch < top) &&
            256 * pitch < top;
 }

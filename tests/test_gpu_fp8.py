@@ -164,7 +164,8 @@ def _check_matmul(dev, rng, m, k, n, block_rows, dtype, offset=0):
 @pytest.mark.parametrize("block_rows", [1, 128])
 @pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 2048, 768), (2, 127, 130), (5, 128, 3), (16, 129, 257),
                                    (17, 384, 256), (33, 1000, 100), (64, 256, 128), (65, 640, 200),
-                                   (128, 512, 512), (130, 300, 515), (300, 1024, 260), (520, 700, 384)])
+                                   (128, 512, 512), (130, 300, 515), (300, 1024, 260), (520, 700, 384),
+                                   (700, 100, 1100), (900, 250, 1030), (2500, 128, 700), (2200, 200, 2100)])
 def test_matmul(dev, dtype, block_rows, m, k, n):
     print(f"[gpu] fp8 matmul {m}x{k}x{n} {dtype} block_rows={block_rows}", flush=True)
     _check_matmul(dev, np.random.default_rng(m * 7 + k + n), m, k, n, block_rows, dtype)
@@ -314,7 +315,8 @@ def _check_experts(y, xv, w, perm, offsets, h, i, ydtype):
 @pytest.mark.parametrize("tokens,top_k,e,h,i", [(1, 2, 4, 256, 128), (3, 8, 16, 384, 256), (16, 4, 8, 200, 100),
                                                 (40, 3, 5, 512, 384), (150, 2, 3, 300, 500), (400, 4, 6, 512, 256),
                                                 (90, 2, 70, 640, 520), (300, 3, 5, 401, 600), (700, 2, 4, 520, 384),
-                                                (900, 2, 4, 272, 300)])
+                                                (900, 2, 4, 272, 300), (16, 1, 2, 3840, 200), (2, 8, 9, 100, 3900),
+                                                (500, 2, 4, 400, 130)])
 def test_experts(dev, xdtype, ydtype, tokens, top_k, e, h, i):
     print(f"[gpu] fp8 experts T={tokens} k={top_k} E={e} H={h} I={i} {xdtype}->{ydtype}", flush=True)
     rng = np.random.default_rng(tokens + e)
