@@ -18,6 +18,7 @@ from dataclasses import dataclass, field
 import numpy as np
 
 from . import capi
+from .fp8 import check_on_device
 
 ROUTE_SOFTMAX = capi.HM_ROUTE_SOFTMAX
 ROUTE_RENORM = capi.HM_ROUTE_RENORM
@@ -81,6 +82,7 @@ class DeviceExpertLayer:
         torch = _torch()
         if isinstance(payload, np.ndarray):
             payload = torch.from_numpy(np.ascontiguousarray(payload)).to("cuda")
+        check_on_device(payload)
         experts = payload.shape[0]
         codes = {torch.float32: capi.HM_DTYPE_FP32, torch.float16: capi.HM_DTYPE_FP16,
                  torch.bfloat16: capi.HM_DTYPE_BF16}
@@ -93,6 +95,8 @@ class DeviceExpertLayer:
             blocks = -(-hidden // capi.HM_FP8_BLOCK) * -(-inter // capi.HM_FP8_BLOCK)
             scale = torch.empty((experts, 3, blocks), dtype=torch.float32, device=payload.device)
             s = torch.cuda.current_stream().cuda_stream if stream is None else stream
+            if stream is not None:
+                torch.cuda.current_stream().synchronize()  # the payload may still be on its way
             capi.call("hm_fp8_pack_layer", payload.data_ptr(), codes[payload.dtype], experts, hidden,
                       inter, packed.data_ptr(), scale.data_ptr(), s)
             torch.cuda.synchronize()
@@ -105,6 +109,7 @@ class DeviceExpertLayer:
         the float32 scale of each 128 x 128 block [E, ceil(out / 128),
         ceil(in / 128)]."""
         torch = _torch()
+        check_on_device(gate, up, down, gate_scale, up_scale, down_scale)
         experts, inter, hidden = gate.shape
         b = capi.HM_FP8_BLOCK
         per, scales = [], []

@@ -49,6 +49,18 @@ class Matrix:
     width: int
     block_rows: int
 
+    def __post_init__(self):
+        torch = _torch()
+        nb = -(-self.width // capi.HM_FP8_BLOCK)
+        if self.block_rows not in (1, capi.HM_FP8_BLOCK) or self.width <= 0:
+            raise ValueError("block_rows is 1 or 128 and the matrix has columns")
+        if self.q.dim() != 2 or self.q.element_size() != 1 or self.q.shape[1] != nb * capi.HM_FP8_BLOCK or \
+                not self.q.is_contiguous():
+            raise ValueError(f"the bytes are a contiguous [rows, {nb * capi.HM_FP8_BLOCK}] tensor")
+        if self.scale.dtype != torch.float32 or not self.scale.is_contiguous() or \
+                tuple(self.scale.shape) != (-(-self.q.shape[0] // self.block_rows), nb):
+            raise ValueError(f"the scales are a contiguous float32 [ceil(rows / {self.block_rows}), {nb}] tensor")
+
     @property
     def rows(self) -> int:
         return self.q.shape[0]
@@ -122,6 +134,8 @@ def experts(layer, x, offsets, perm_tokens, out_dtype=None, out=None, workspace=
         out = torch.empty((pairs, layer.hidden), dtype=out_dtype or x.dtype, device=device)
     elif tuple(out.shape) != (pairs, layer.hidden) or not out.is_contiguous() or out_dtype not in (None, out.dtype):
         raise ValueError(f"out must be a contiguous [{pairs}, {layer.hidden}] tensor")
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("the workspace must be contiguous")
     if pairs == 0 or tokens == 0:
         return out
     if workspace is None:

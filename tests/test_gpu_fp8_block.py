@@ -257,6 +257,53 @@ def test_python_entry_points(dev):
             bad()
 
 
+def test_python_refusals(dev):
+    """What the Python entry points refuse before a launch: operands that a kernel would read as something
+    they are not."""
+    from hmoe import fp8, rows
+    from hmoe.block import DeviceExpertLayer
+    torch = dev.torch
+    x = torch.ones((4, 256), device="cuda")
+    good = fp8.quantize(x)
+    for q, scale, width, block_rows in ((good.q[:, :128], good.scale, 256, 1), (good.q, good.scale[:3], 256, 1),
+                                        (good.q, good.scale.double(), 256, 1), (good.q, good.scale, 300, 1),
+                                        (good.q, good.scale, 256, 64), (good.q, good.scale, 256, 128),
+                                        (good.q.t().contiguous().t(), good.scale, 256, 1)):
+        with pytest.raises(ValueError):
+            fp8.Matrix(q, scale, width, block_rows)
+    with pytest.raises(ValueError):
+        fp8.quantize(x.cpu())
+    with pytest.raises(ValueError):
+        fp8.matmul(good, fp8.quantize(torch.ones((4, 128), device="cuda")))
+    with pytest.raises(ValueError):
+        fp8.matmul(fp8.quantize(x, block_rows=128), good)
+    with pytest.raises(ValueError):
+        fp8.matmul(good, good, out=torch.empty((4, 8), device="cuda")[:, ::2])
+    weights = [torch.zeros((2, 128, 128), dtype=torch.uint8) for _ in range(3)]
+    scales = [torch.ones((2, 1, 1)) for _ in range(3)]
+    on = [t.cuda() for t in weights + scales]
+    DeviceExpertLayer.from_fp8(*on)
+    for host in range(6):   # one operand left on the host
+        with pytest.raises(ValueError):
+            DeviceExpertLayer.from_fp8(*[t.cpu() if i == host else t for i, t in enumerate(on)])
+    with pytest.raises(ValueError):
+        DeviceExpertLayer.quantize_fp8(torch.zeros((2, 3, 128 * 128)), 128, 128)
+    layer = DeviceExpertLayer.from_fp8(*on)
+    offsets = torch.tensor([0, 4, 4], dtype=torch.int32, device="cuda")
+    perm = torch.arange(4, dtype=torch.int32, device="cuda")
+    xs = torch.ones((4, 128), device="cuda")
+    work = torch.empty(2 * fp8.workspace_bytes(layer, 4, 4), dtype=torch.uint8, device="cuda")
+    for args, kw in (((x, offsets, perm), {}), ((xs, offsets[:2], perm), {}), ((xs, offsets.long(), perm), {}),
+                     ((xs, offsets, perm), {"workspace": work[::2]}), ((xs.cpu(), offsets, perm), {}),
+                     ((xs, offsets, perm), {"out": torch.empty((3, 128), device="cuda")})):
+        with pytest.raises(ValueError):
+            fp8.experts(layer, *args, **kw)
+    slots = torch.zeros((4, 1), dtype=torch.int32, device="cuda")
+    for args in ((x[:3], slots, 4), (x, slots.long(), 4), (x.t(), slots, 4), (x, slots.cpu(), 4)):
+        with pytest.raises(ValueError):
+            rows.dispatch(*args)
+
+
 def test_training_step(dev):
     """One layer's rows forward and backward around the experts' products in FP8: out = sum_r s (x W_e^T),
     gradients of x, W and s through dispatch, the FP8 products and combine, against 64 bits from the same
