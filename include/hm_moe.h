@@ -375,9 +375,9 @@ int hm_limb_partials(const int8_t* digits, int64_t rows, int64_t inner,
  * transposed views of dY and x, both with a scale per row (w_block_rows 1).
  * y must not overlap the operands.
  *
- * HM_ERR_OVERFLOW: over 65535 x 64 rows (x 128 with block_rows 128) to
- * quantise, unless block_rows is 1 and the columns are contiguous, or to
- * multiply where w's bytes exceed 4 GiB. */
+ * HM_ERR_OVERFLOW: over 65535 x 128 rows to quantise, unless block_rows is 1
+ * and the columns are contiguous; over 65535 x 64 rows to multiply where w's
+ * bytes exceed 4 GiB. */
 int64_t hm_fp8_pitch(int64_t width);
 int hm_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t width,
                     int64_t row_stride, int64_t col_stride, int32_t block_rows,
