@@ -13,7 +13,9 @@
 //
 // Bound by the rows' bytes (one read or write each; the products are a few operations a value).  A
 // workgroup owns a token, or without dot products a column chunk of it, so every sum has one owner
-// and a fixed order (ranks ascending): no atomics, the same bits every run.
+// and a fixed order (ranks ascending): no atomics, the same bits every run.  4096 tokens, top-8, 2048 wide, BF16:
+// dispatch 26 us (151 MB), join 40 (168 MB), combine's gradient with both results 49 (285 MB): 4.2 to 5.8
+// TB/s where a large copy reaches 4.8.
 #include "hm_fp8.h"
 
 #include <limits.h>
@@ -23,7 +25,8 @@ namespace {
 constexpr int kRThreads = 256;
 constexpr int kRanks = 8;   // ranks walked at once: their row loads are in flight together
 
-// V consecutive values of a row; V = 1 where the rows are not 16-byte aligned.
+// V consecutive values of a row: 16 bytes where the rows are aligned to that, else 2 values (4096 tokens,
+// top-8, BF16, forward and backward: 2048 wide 155 us, 2046 226; by single values 336), else one.
 template <typename T, int V>
 struct Chunk {
     float v[V];
@@ -187,13 +190,19 @@ int spread(const void* src, const void* other, const int32_t* slots, const float
            hipStream_t s) {
     constexpr int V = 16 / sizeof(T);
     const bool vec = width % V == 0 && aligned(src, 16) && aligned(other, 16) && aligned(out, 16);
+    constexpr uintptr_t P = 2 * sizeof(T);
+    const bool pairs = width % 2 == 0 && aligned(src, P) && aligned(other, P) && aligned(out, P);
     auto run = [&](auto kernel, int v) {
         hipLaunchKernelGGL(kernel, rows_grid(tokens, width, v, dots != nullptr), dim3(kRThreads), 0, s,
                            static_cast<const T*>(src), static_cast<const T*>(other), slots, weights,
                            (int)top_k, rows, width, static_cast<T*>(out), dots);
     };
-    if (dots) vec ? run(rows_spread_kernel<T, V, true>, V) : run(rows_spread_kernel<T, 1, true>, 1);
-    else vec ? run(rows_spread_kernel<T, V, false>, V) : run(rows_spread_kernel<T, 1, false>, 1);
+    if (dots)
+        vec ? run(rows_spread_kernel<T, V, true>, V)
+        : pairs ? run(rows_spread_kernel<T, 2, true>, 2) : run(rows_spread_kernel<T, 1, true>, 1);
+    else
+        vec ? run(rows_spread_kernel<T, V, false>, V)
+        : pairs ? run(rows_spread_kernel<T, 2, false>, 2) : run(rows_spread_kernel<T, 1, false>, 1);
     HM_LAUNCHED();
     return HM_OK;
 }
@@ -205,14 +214,21 @@ int join(const void* src, const void* other, const int32_t* slots, const float* 
     constexpr int V = 16 / sizeof(T);
     const bool vec = width % V == 0 && aligned(src, 16) && aligned(other, 16) &&
                      aligned(residual, 16) && aligned(dst, 16);
+    constexpr uintptr_t P = 2 * sizeof(T);
+    const bool pairs = width % 2 == 0 && aligned(src, P) && aligned(other, P) &&
+                       aligned(residual, P) && aligned(dst, P);
     auto run = [&](auto kernel, int v) {
         hipLaunchKernelGGL(kernel, rows_grid(tokens, width, v, dots != nullptr), dim3(kRThreads), 0, s,
                            static_cast<const T*>(src), static_cast<const T*>(other), slots, weights,
                            static_cast<const T*>(residual), (int)top_k, rows, width,
                            static_cast<T*>(dst), dots);
     };
-    if (dots) vec ? run(rows_join_kernel<T, V, true>, V) : run(rows_join_kernel<T, 1, true>, 1);
-    else vec ? run(rows_join_kernel<T, V, false>, V) : run(rows_join_kernel<T, 1, false>, 1);
+    if (dots)
+        vec ? run(rows_join_kernel<T, V, true>, V)
+        : pairs ? run(rows_join_kernel<T, 2, true>, 2) : run(rows_join_kernel<T, 1, true>, 1);
+    else
+        vec ? run(rows_join_kernel<T, V, false>, V)
+        : pairs ? run(rows_join_kernel<T, 2, false>, 2) : run(rows_join_kernel<T, 1, false>, 1);
     HM_LAUNCHED();
     return HM_OK;
 }

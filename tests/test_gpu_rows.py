@@ -88,7 +88,8 @@ CASES = [dict(tokens=1, top_k=1, width=1), dict(tokens=1, top_k=8, width=2048), 
          dict(tokens=7, top_k=3, width=1001, dropped=0.5), dict(tokens=33, top_k=9, width=72, dropped=0.3),
          dict(tokens=5, top_k=20, width=4104), dict(tokens=300, top_k=2, width=256, dropped=0.1),
          dict(tokens=4, top_k=2, width=64, dropped=1.0), dict(tokens=6, top_k=4, width=136, offset=1, dropped=0.2),
-         dict(tokens=9, top_k=2, width=96, dropped=0.4, bad_slots=True)]
+         dict(tokens=9, top_k=2, width=96, dropped=0.4, bad_slots=True),
+         dict(tokens=19, top_k=3, width=1030, dropped=0.2), dict(tokens=6, top_k=9, width=520, offset=2)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
