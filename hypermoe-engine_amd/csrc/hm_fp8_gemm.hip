@@ -12,7 +12,8 @@ constexpr int kSWaves = 8;
 
 // Weights streamed from memory: a workgroup of 8 waves owns 16 MT rows x 16 outputs (GU: 16 gate and
 // 16 up outputs, z = silu(g) u), its waves split K by blocks and their sums meet in the LDS in wave
-// order.  BROW: w has a scale for each of its rows.
+// order.  BROW: w has a scale for each of its rows.  Bound by latency: one row of 2048 x 2048 3.6 us,
+// 333 x 1000 x 777 (FP32) 7.8.
 template <int MT, bool GU, bool BROW, typename T>
 __global__ __launch_bounds__(64 * kSWaves) void f8_stream_kernel(Product p, T* __restrict__ y) {
     constexpr int NP = GU ? 2 : 1;
@@ -116,7 +117,8 @@ int launch_stream(const Product& p, int64_t m_tiles16, T* y, hipStream_t s) {
 // of 8 waves owns 8 / KP x 16 outputs (GU: gate and up) of up to 16 rows of one expert.  Its weights are
 // sent for first (KP waves split K, two blocks each in flight), then its rows are cut to 8 bits into the
 // LDS, 16 lanes a block, so that nothing is launched before or between the products; the waves' sums
-// meet in the LDS in wave order.
+// meet in the LDS in wave order.  One token, top-8 of 128 experts of 2048 x 768: gate/up 8.4 us (25 MB),
+// down 5.1 (13 MB), 13.7 as called; by quantisation and tiles 19.4.
 struct Decode {
     const void* x;
     const uint8_t* w;

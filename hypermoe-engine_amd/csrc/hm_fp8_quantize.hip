@@ -18,8 +18,8 @@ namespace {
 constexpr int kQThreads = 256;
 
 // 8 consecutive values from p (VEC: 16-byte loads), zeros from column `left` on.  Unaligned 16-bit values
-// come as the words that hold them, shifted by half a word where p is odd (65536 x 4095 of a row of 4096: 206 us
-// against 342 value by value).
+// come as the words that hold them, shifted by half a word where p is odd (65536 x 4095 of rows of 4096:
+// 206 us against 342 value by value).
 template <typename T, bool VEC>
 __device__ __forceinline__ void load8(const T* __restrict__ p, int64_t left, float (&v)[8]) {
     if (VEC && left >= 8) {

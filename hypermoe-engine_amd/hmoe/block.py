@@ -160,6 +160,8 @@ class MoEBlock:
 
     def _buffers(self, tokens: int, exec_flags: int = 0):
         torch = _torch()
+        if self.layer.dtype == capi.HM_DTYPE_FP8 and self.layer.packed.device.index != torch.cuda.current_device():
+            raise ValueError(f"the layer is on {self.layer.packed.device}, not on the current device")
         nbytes = capi.load().hm_moe_block_workspace_bytes(
             C.byref(self.layer.desc), tokens, self.top_k, self.limbs_x, self.limbs_z, exec_flags)
         if nbytes == 0:
