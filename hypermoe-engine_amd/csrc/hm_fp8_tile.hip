@@ -136,7 +136,8 @@ __device__ __forceinline__ void store_z(const Product& p, const TileAt& t, v4f (
         const float amax = fmaxf(fmaxf(s_amax[0][r], s_amax[1][r]), fmaxf(s_amax[2][r], s_amax[3][r]));
         if (r >= t.nrows) continue;
         const bool finite = amax < __builtin_inff();
-        const float m = fmaxf(amax, kF8Tiny), inv = kF8Top * __builtin_amdgcn_rcpf(m);
+        const float m = fmaxf(amax, kF8Tiny);
+        const float inv = 0.875f * __builtin_amdgcn_rcpf(m * 0x1p-9f);  // 448 / m; 1 / m may be subnormal, 0 here
         uint32_t w[SH];
 #pragma unroll
         for (int q = 0; q < SH; ++q) {

@@ -362,9 +362,10 @@ int hm_limb_partials(const int8_t* digits, int64_t rows, int64_t inner,
  * k col_stride], one of the strides 1) to that form.  With amax = max(|x|,
  * 2^-100) over a block, scale = amax / 448 and each byte is the e4m3 value
  * nearest to 448 x / amax, ties to even (decided exactly for 16-bit x).  A
- * block that holds an infinity or a NaN becomes NaN throughout.  The blocks
- * of a transposed matrix are the transposed blocks, so quantising the
- * transposed view of a weight gives the operand of its input's gradient.
+ * block that holds an infinity or a NaN becomes NaN throughout.  q and scale
+ * must not overlap x.  The blocks of a transposed matrix are the transposed
+ * blocks, so quantising the transposed view of a weight gives the operand of
+ * its input's gradient.
  *
  * hm_fp8_matmul: y[m, n] = sum_b xs[m, b] ws[n / w_block_rows, b]
  * sum_{k in block b} x[m, k] w[n, k], x [rows x inner] with a scale per row

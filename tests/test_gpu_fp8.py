@@ -326,6 +326,22 @@ def test_experts(dev, xdtype, ydtype, tokens, top_k, e, h, i):
     _check_experts(y, xv, w, perm, offsets, h, i, ydtype)
 
 
+@pytest.mark.parametrize("tokens,ydtype", [(2, "f32"), (60, "f32"), (500, "bf16")])
+def test_experts_large_z(dev, tokens, ydtype):
+    """z up to 2.5e38, where the reciprocal of a block's maximum is a subnormal float."""
+    print(f"[gpu] fp8 experts, large z, T={tokens} {ydtype}", flush=True)
+    rng = np.random.default_rng(tokens)
+    e, h, i = 3, 400, 300
+    packed, scale, w = _layer(rng, e, h, i)
+    perm, offsets = _groups(rng, tokens, 1, e)
+    x = rng.standard_normal((tokens, h)).astype(np.float32).astype(np.float64)
+    grown = max(np.max(np.maximum(x[perm[lo:hi]] @ g.T, 0.0) * np.abs(x[perm[lo:hi]] @ u.T))
+                for (g, u, _), lo, hi in zip(w, offsets[:-1], offsets[1:]) if hi > lo)
+    y, xv = _experts(dev, packed, scale, x * np.sqrt(2.5e38 / grown), "f32", perm, offsets, e, h, i, ydtype)
+    with np.errstate(over="ignore"):          # e^-g of gates below -700
+        _check_experts(y, xv, w, perm, offsets, h, i, ydtype)
+
+
 @pytest.mark.parametrize("tokens", [5, 300])
 def test_experts_one_group(dev, tokens):
     """Every row to one expert, and a last group that ends before `pairs` (rows behind it stay)."""
