@@ -11,8 +11,8 @@
 //   w     fragment j's row i is w row 4 SH (i / 4) + 4 j + i % 4 of the wave's, so that a lane ends
 //         with 4 SH consecutive outputs of one row (SH: fragments side by side).
 //   order tiles are cut into 8 contiguous ranges, one per XCD (workgroup i runs on XCD i % 8); n-tiles
-//         of an m-tile lie together, for one matrix in groups of 4 m-tiles, so what is read by
-//         several workgroups at once is in one L2.
+//         of an m-tile lie together, for one matrix in groups of m-tiles, so what is read by several
+//         workgroups at once is in one L2.
 // Epilogue of gate/up (GU): z = silu(g) u for one block of 128 columns; its maximum over the block goes
 // over lanes, then through the LDS over the four waves of a row; the bytes and scale are stored.
 //
@@ -32,7 +32,6 @@ namespace {
 
 constexpr int kXcds = 8;
 constexpr int kTThreads = 512;
-constexpr int kSuper = 4;    // m-tiles walked together (one matrix)
 
 struct TileAt {
     int e, row0, nrows, n0;
@@ -45,10 +44,13 @@ __device__ __forceinline__ P* uni(P* p) {
     return reinterpret_cast<P*>(((uint64_t)(uint32_t)uni((int)(v >> 32)) << 32) | (uint32_t)uni((int)v));
 }
 
-// Tile j: n-tiles of an m-tile lie together, for one matrix in groups of kSuper m-tiles.  (Per lane.)
+// Tile j: n-tiles of an m-tile lie together, for one matrix in groups of m-tiles, so many that the tiles
+// which an XCD has at once cover about as many rows of x as of w (4096 x 4096 x 4096 by groups of 4 and 8:
+// 64 x 128 tiles 105.5 and 100 us, 256 x 256 63.4 and 64).  (Per lane.)
 template <int BM, int TN>
 __device__ __forceinline__ TileAt tile_at(const Product& p, const int4* __restrict__ table, int j, int mt,
                                           int ntn) {
+    constexpr int SUPER = BM == 256 ? 4 : 8;
     TileAt t;
     if (table) {
         const int m = j / ntn;
@@ -58,8 +60,8 @@ __device__ __forceinline__ TileAt tile_at(const Product& p, const int4* __restri
         t.nrows = e.z;
         t.n0 = (j - m * ntn) * TN;
     } else {
-        const int grp = j / (kSuper * ntn), first = grp * kSuper;
-        const int gm = min(mt - first, kSuper), r = j - first * ntn;
+        const int grp = j / (SUPER * ntn), first = grp * SUPER;
+        const int gm = min(mt - first, SUPER), r = j - first * ntn;
         t.e = 0;
         t.row0 = (first + r % gm) * BM;
         t.nrows = min(BM, (int)p.rows - t.row0);
