@@ -95,17 +95,30 @@ __global__ __launch_bounds__(64 * kSWaves) void f8_stream_kernel(Product p, T* _
     }
 }
 
+constexpr int kCus = 256;
+
+// Rows of a stream workgroup, in 16s: as few as leave no CU more than one workgroup (64 x 2048 x 4096: 32
+// rows 9.8 us, 64 15, 16 11; 32 x 2048 x 4096: 16 rows 7.5, 64 10.8).
+int stream_mt(int64_t rows, int64_t cols) {
+    const int64_t groups = (cols + 15) / 16;
+    for (int mt = 1; mt < 4; mt *= 2)
+        if (rows <= 16 * mt || groups * ((rows + 16 * mt - 1) / (16 * mt)) <= kCus) return mt;
+    return 4;
+}
+
 template <bool GU, bool BROW, typename T>
 int launch_stream(const Product& p, int64_t m_tiles16, T* y, hipStream_t s) {
     // m_tiles16: an upper bound of the 16-row tiles
     const int64_t cols = (p.N + 15) / 16;
-    const int mt = p.rows <= 16 ? 1 : 4;
+    const int mt = p.offsets ? (p.rows <= 16 ? 1 : 4) : stream_mt(p.rows, p.N);
     const int64_t rows_tiles = p.offsets ? (mt == 1 ? m_tiles16 : (p.rows + 63) / 64 + min((int64_t)p.experts, p.rows))
                                          : (p.rows + 16 * mt - 1) / (16 * mt);
     if (rows_tiles > 65535 || cols > INT_MAX / 512) return HM_ERR_OVERFLOW;
     const dim3 grid((unsigned)cols, (unsigned)rows_tiles);
     if (mt == 1)
         hipLaunchKernelGGL((f8_stream_kernel<1, GU, BROW, T>), grid, dim3(64 * kSWaves), 0, s, p, y);
+    else if (mt == 2)
+        hipLaunchKernelGGL((f8_stream_kernel<2, GU, BROW, T>), grid, dim3(64 * kSWaves), 0, s, p, y);
     else
         hipLaunchKernelGGL((f8_stream_kernel<4, GU, BROW, T>), grid, dim3(64 * kSWaves), 0, s, p, y);
     HM_LAUNCHED();
@@ -314,8 +327,8 @@ int launch_decode(const Decode& p, hipStream_t s) {
 // every CU where the form's LDS lets them.  The constants fit 14 shapes of K = 1024 and 4096 within 20 %.
 // 2048 x 2048 x 4096: 64 x 128 tiles 29 us, 128 x 128 34, 128 x 256 34, 256 x 256 50; 4096 x 4096: 111, 88,
 // 76 and 66.  The stream kernel has no ring to fill: 16 rows of 2048 x 2048 7 us against 8 for the smallest
-// tile, 333 x 777 x 4096 (FP32) 21 against 28, 16 x 2048 x 256 2.9 against 4.1 (kernel alone); but it reads
-// w again for every 64 rows: 4096 x 4096 x 256 76 us against 12.
+// tile, 333 x 777 x 4096 (FP32) 21 against 28, 16 x 2048 x 256 2.9 against 4.1 (kernel alone), 32 x 8192 x
+// 4096 17.4 against 14.5; but it reads w again for every 64 rows: 4096 x 4096 x 256 76 us against 12.
 struct Form {
     int bm, bn, per_cu, min_blocks;
     double alone, every, shared;
@@ -324,13 +337,14 @@ constexpr Form kFast[] = {{256, 256, 1, 1, 1.43, 1.95, 1.95}, {128, 256, 1, 2, 0
                           {128, 128, 2, 1, 0.58, 0.95, 1.3}, {64, 128, 2, 2, 0.44, 0.47, 0.82}};
 constexpr Form kExact[] = {{128, 256, 1, 2, 1.9, 2.1, 2.1}, {128, 128, 1, 1, 1.2, 1.2, 1.2},
                            {64, 128, 2, 2, 0.8, 0.84, 1.27}};
-constexpr int kCus = 256;
 
 // nullptr: the stream kernel
 const Form* choose_form(const Product& p, bool exact) {
     const double steps = (double)hm_f8_blocks(p.K);
-    const double groups = (double)((p.N + 15) / 16) * (double)((p.rows + 63) / 64);
-    double best = groups <= kCus ? 3.0 + steps / 16 * 4.0 : 4.7 + steps / 16 * groups / (2 * kCus) * 12.0;
+    const int mt = stream_mt(p.rows, p.N);
+    const double groups = (double)((p.N + 15) / 16) * (double)((p.rows + 16 * mt - 1) / (16 * mt));
+    const double each = steps / 16 * (mt == 1 ? 1.3 : mt == 2 ? 3.2 : 6.0);
+    double best = groups <= kCus ? 3.0 + each : 4.7 + each * groups / kCus;
     const Form* form = nullptr;
     if (!hm_f8_tile_ok(p, false)) return nullptr;
     const Form* forms = exact ? kExact : kFast;
@@ -339,8 +353,10 @@ const Form* choose_form(const Product& p, bool exact) {
         if (steps < f.min_blocks) continue;
         const int64_t tiles = ((p.rows + f.bm - 1) / f.bm) * ((p.N + f.bn - 1) / f.bn);
         const int64_t rounds = (tiles + kCus * f.per_cu - 1) / (kCus * f.per_cu);
-        const double t = 4.0 + steps * (tiles <= kCus ? f.alone + (f.every - f.alone) * tiles / kCus
-                                                      : rounds * f.shared);
+        // (a tile whose lower half has no rows takes 0.7 of a step)
+        const double t = 4.0 + steps * (p.rows <= f.bm / 2 ? 0.7 : 1.0) *
+                                   (tiles <= kCus ? f.alone + (f.every - f.alone) * tiles / kCus
+                                                  : rounds * f.shared);
         if (t < best) {
             best = t;
             form = &f;

@@ -165,7 +165,8 @@ def _check_matmul(dev, rng, m, k, n, block_rows, dtype, offset=0):
 @pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 2048, 768), (2, 127, 130), (5, 128, 3), (16, 129, 257),
                                    (17, 384, 256), (33, 1000, 100), (64, 256, 128), (65, 640, 200),
                                    (128, 512, 512), (130, 300, 515), (300, 1024, 260), (520, 700, 384),
-                                   (700, 100, 1100), (900, 250, 1030), (2500, 128, 700), (2200, 200, 2100)])
+                                   (700, 100, 1100), (900, 250, 1030), (2500, 128, 700), (2200, 200, 2100),
+                                   (60, 1500, 1000), (25, 1100, 4100), (100, 900, 1090)])
 def test_matmul(dev, dtype, block_rows, m, k, n):
     print(f"[gpu] fp8 matmul {m}x{k}x{n} {dtype} block_rows={block_rows}", flush=True)
     _check_matmul(dev, np.random.default_rng(m * 7 + k + n), m, k, n, block_rows, dtype)
