@@ -125,7 +125,7 @@ int launch_stream(const Product& p, int64_t m_tiles16, T* y, hipStream_t s) {
     return HM_OK;
 }
 
-// ---- Experts of a few rows: two launches, each quantising what it multiplies.
+// ---- Experts of a few rows (64 at most): two launches, each quantising what it multiplies.
 // A decode step reads every chosen expert's weights for a row or two; the rest is latency.  A workgroup
 // of 8 waves owns 8 / KP x 16 outputs (GU: gate and up) of up to 16 rows of one expert.  Its weights are
 // sent for first (KP waves split K, two blocks each in flight), then its rows are cut to 8 bits into the
@@ -392,11 +392,20 @@ struct ExpertsPlan {
     int4* table;
 };
 
-// Up to kDecodePairs rows take the decode kernels; others tiles of 64 rows, or 128 where an expert has
-// that many on average (128 experts top-8, 2048 tokens: 194 us against 211; 1024: 168 against 160), or, with
-// the FP8 instruction, 256 from 384 rows an expert (6144 tokens: 367 us against 395; 4096: 315 against 293;
-// 8 experts top-2 of 4096 x 2048, 16384 tokens: 932 us, 1.77 PFLOP/s, against 1079).
-constexpr int64_t kDecodePairs = 16;
+// The decode kernels take up to kDecodePairs rows, or four times as many where they go to experts of up to 8
+// on average and kDecodeBytes of weights at most: beyond, the weights' stream hides the tiles' extra
+// launch (16 tokens, top-2 of 8 experts of 2048 x 768, 38 MB: 16.7 us against 24.5 by tiles; top-8 of 128:
+// 3 tokens, 113 MB, 31.1 against 32.3; 4 tokens 37.8 against 36.4; 32 tokens, top-2 of 4, 26.3 against
+// 24.7).  Others take tiles of 64 rows, or 128 where an expert has that many on average (128 experts
+// top-8, 2048 tokens: 194 us against 211; 1024: 168 against 160), or, with the FP8 instruction, 256 from
+// 384 rows an expert (6144 tokens: 367 us against 395; 4096: 315 against 293; 8 experts top-2 of 4096 x
+// 2048, 16384 tokens: 932 us, 1.77 PFLOP/s, against 1079).
+constexpr int64_t kDecodePairs = 16, kDecodeBytes = (int64_t)1 << 27;
+bool decode_rows(const hm_layer* L, int64_t pairs) {
+    if (pairs <= kDecodePairs) return true;
+    return pairs <= 4 * kDecodePairs && pairs <= 8 * L->experts &&
+           std::min(pairs, L->experts) * 3 * L->hidden <= kDecodeBytes / L->intermediate;
+}
 enum class Experts { kDecode, kTiles, kStream };
 struct ExpertsForm {
     Experts kind;
@@ -413,7 +422,7 @@ ExpertsForm experts_form(const hm_layer* L, int64_t tokens, int64_t pairs, bool 
     gu.K = dn.N = H;
     gu.N = dn.K = I;
     gu.perm = &gathered;
-    if (pairs <= kDecodePairs && decode_lds(16, (int)std::max(H, I)) <= 65536) {
+    if (decode_rows(L, pairs) && decode_lds(16, (int)std::max(H, I)) <= 65536) {
         f.kind = Experts::kDecode;
     } else if (hm_f8_tile_ok(gu, true) && hm_f8_tile_ok(dn, false) && I > kF8Block) {
         f.kind = Experts::kTiles;

@@ -317,7 +317,7 @@ def _check_experts(y, xv, w, perm, offsets, h, i, ydtype):
                                                 (40, 3, 5, 512, 384), (150, 2, 3, 300, 500), (400, 4, 6, 512, 256),
                                                 (90, 2, 70, 640, 520), (300, 3, 5, 401, 600), (700, 2, 4, 520, 384),
                                                 (900, 2, 4, 272, 300), (16, 1, 2, 3840, 200), (2, 8, 9, 100, 3900),
-                                                (500, 2, 4, 400, 130)])
+                                                (500, 2, 4, 400, 130), (20, 2, 6, 300, 260), (64, 1, 64, 256, 128)])
 def test_experts(dev, xdtype, ydtype, tokens, top_k, e, h, i):
     print(f"[gpu] fp8 experts T={tokens} k={top_k} E={e} H={h} I={i} {xdtype}->{ydtype}", flush=True)
     rng = np.random.default_rng(tokens + e)
@@ -343,7 +343,7 @@ def test_experts_large_z(dev, tokens, ydtype):
         _check_experts(y, xv, w, perm, offsets, h, i, ydtype)
 
 
-@pytest.mark.parametrize("tokens", [5, 300])
+@pytest.mark.parametrize("tokens", [5, 50, 300])
 def test_experts_one_group(dev, tokens):
     """Every row to one expert, and a last group that ends before `pairs` (rows behind it stay)."""
     rng = np.random.default_rng(3)
