@@ -18,7 +18,7 @@ from dataclasses import dataclass, field
 import numpy as np
 
 from . import capi
-from .fp8 import check_on_device
+from .fp8 import check_e4m3, check_on_device
 
 ROUTE_SOFTMAX = capi.HM_ROUTE_SOFTMAX
 ROUTE_RENORM = capi.HM_ROUTE_RENORM
@@ -104,10 +104,10 @@ class DeviceExpertLayer:
 
     @classmethod
     def from_fp8(cls, gate, up, down, gate_scale, up_scale, down_scale):
-        """An FP8 layer of a checkpoint's tensors: e4m3 (or uint8) weights
-        [E, out, in] on the device, gate and up [E, I, H], down [E, H, I], with
-        the float32 scale of each 128 x 128 block [E, ceil(out / 128),
-        ceil(in / 128)]."""
+        """An FP8 layer of a checkpoint's tensors: weights in float8_e4m3fn (or
+        its bytes as uint8) [E, out, in] on the device, gate and up [E, I, H],
+        down [E, H, I], with the float32 scale of each 128 x 128 block
+        [E, ceil(out / 128), ceil(in / 128)]."""
         torch = _torch()
         check_on_device(gate, up, down, gate_scale, up_scale, down_scale)
         experts, inter, hidden = gate.shape
@@ -115,8 +115,9 @@ class DeviceExpertLayer:
         per, scales = [], []
         for w, s, (n, k) in ((gate, gate_scale, (inter, hidden)), (up, up_scale, (inter, hidden)),
                              (down, down_scale, (hidden, inter))):
-            if tuple(w.shape) != (experts, n, k) or w.element_size() != 1:
-                raise ValueError(f"FP8 weights must be [{experts}, {n}, {k}] bytes, got {tuple(w.shape)}")
+            check_e4m3(w, "FP8 weights")
+            if tuple(w.shape) != (experts, n, k):
+                raise ValueError(f"FP8 weights must be [{experts}, {n}, {k}], got {tuple(w.shape)}")
             if tuple(s.shape) != (experts, -(-n // b), -(-k // b)):
                 raise ValueError(f"block scales do not match [{experts}, {-(-n // b)}, {-(-k // b)}]")
             w = torch.nn.functional.pad(w.view(torch.uint8), (0, -k % b))

@@ -40,10 +40,17 @@ def check_on_device(*tensors):
     return next(iter(devices))
 
 
+def check_e4m3(t, what: str):
+    """`t` holds OCP e4m3 bytes: the other 8-bit types have a byte a value too, but stand for others."""
+    torch = _torch()
+    if t.dtype not in (torch.uint8, torch.float8_e4m3fn):
+        raise ValueError(f"{what} must be e4m3 (float8_e4m3fn, or its bytes as uint8), got {t.dtype}")
+
+
 @dataclass
 class Matrix:
-    """A matrix [rows, width] in FP8: bytes [rows, width rounded up to 128] and the float32 scale of
-    every block of block_rows rows x 128 columns."""
+    """A matrix [rows, width] in FP8: bytes [rows, width rounded up to 128] (uint8 or float8_e4m3fn) and
+    the float32 scale of every block of block_rows rows x 128 columns."""
     q: object
     scale: object
     width: int
@@ -54,8 +61,8 @@ class Matrix:
         nb = -(-self.width // capi.HM_FP8_BLOCK)
         if self.block_rows not in (1, capi.HM_FP8_BLOCK) or self.width <= 0:
             raise ValueError("block_rows is 1 or 128 and the matrix has columns")
-        if self.q.dim() != 2 or self.q.element_size() != 1 or self.q.shape[1] != nb * capi.HM_FP8_BLOCK or \
-                not self.q.is_contiguous():
+        check_e4m3(self.q, "the bytes")
+        if self.q.dim() != 2 or self.q.shape[1] != nb * capi.HM_FP8_BLOCK or not self.q.is_contiguous():
             raise ValueError(f"the bytes are a contiguous [rows, {nb * capi.HM_FP8_BLOCK}] tensor")
         if self.scale.dtype != torch.float32 or not self.scale.is_contiguous() or \
                 tuple(self.scale.shape) != (-(-self.q.shape[0] // self.block_rows), nb):
