@@ -91,15 +91,19 @@ def quantize(x, block_rows: int = 1) -> Matrix:
     device = check_on_device(x)
     if block_rows not in (1, capi.HM_FP8_BLOCK) or width == 0:
         raise ValueError("block_rows is 1 or 128 and the matrix has columns")
-    if x.stride(1) != 1 and x.stride(0) != 1 or min(x.stride()) <= 0:
+    # (the stride of a dimension of one is any number, and torch calls such a tensor contiguous)
+    col_stride = 1 if width == 1 else x.stride(1)
+    row_stride = width if rows == 1 and col_stride == 1 else x.stride(0)
+    if 1 not in (row_stride, col_stride) or min(row_stride, col_stride) <= 0:
         x = x.contiguous()
+        row_stride, col_stride = width, 1
     nb = -(-width // capi.HM_FP8_BLOCK)
     q = torch.empty((rows, nb * capi.HM_FP8_BLOCK), dtype=torch.uint8, device=device)
     scale = torch.empty((-(-rows // block_rows), nb), dtype=torch.float32, device=device)
     if rows == 0:
         return Matrix(q, scale, width, block_rows)
     with torch.cuda.device(device):
-        capi.call("hm_fp8_quantize", x.data_ptr(), code, rows, width, *x.stride(), block_rows,
+        capi.call("hm_fp8_quantize", x.data_ptr(), code, rows, width, row_stride, col_stride, block_rows,
                   q.data_ptr(), scale.data_ptr(), torch.cuda.current_stream().cuda_stream)
     return Matrix(q, scale, width, block_rows)
 

@@ -42,3 +42,48 @@ def test_checkpoint_of_other_bytes(on_host, dtype, which):
     for good in (torch.uint8, torch.float8_e4m3fn):
         layer = block.DeviceExpertLayer.from_fp8(*[t.view(good) for t in w], *s)
         assert (layer.experts, layer.hidden, layer.inter) == (2, 128, 128)
+
+
+@pytest.fixture
+def calls(on_host, monkeypatch):
+    """The library's calls, recorded instead of made; tensors pass as on a GPU."""
+    import contextlib
+    made = []
+    monkeypatch.setattr(fp8, "check_on_device", lambda *t: t[0].device)
+    monkeypatch.setattr(fp8.capi, "call", lambda *a: made.append(a))
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *d: type("S", (), {"cuda_stream": 0}))
+    return made
+
+
+def _views():
+    x = torch.randn(8, 12)
+    yield "a row of a strided block", x[::2, ::2][:1, :1]
+    yield "a column of one, any stride", x.as_strided((4, 1), (1, 7))
+    yield "a row, broadcast", torch.randn(12).as_strided((1, 12), (0, 1))
+    yield "a row, negative-free stride of a slice", x[:1, ::2]
+    yield "a row of a transposed view", x.t()[:1]
+    yield "a column", x[:, 3:4]
+    yield "a column of every third row", x[::3, 3:4]
+    yield "a whole matrix", x
+    yield "a transposed view", x.t()
+    yield "a block of a matrix", x[2:5, 4:9]
+    yield "every second column", x[:, ::2]
+    yield "one row repeated", torch.randn(12).expand(5, 12)
+    yield "one value repeated", torch.randn(1, 1).expand(5, 12)
+
+
+@pytest.mark.parametrize("what,x", list(_views()), ids=lambda v: v if isinstance(v, str) else "")
+def test_quantize_views(calls, what, x):
+    """Whatever the view, the library gets strides that it takes and that name the view's elements: the
+    stride of a dimension of one is any number, also one that the library would refuse."""
+    m = fp8.quantize(x)
+    (name, pointer, _, rows, width, row_stride, col_stride, *_), = calls
+    assert name == "hm_fp8_quantize" and (rows, width) == tuple(x.shape) == (m.rows, m.width)
+    assert row_stride > 0 and col_stride > 0 and 1 in (row_stride, col_stride)
+    at = torch.arange(rows)[:, None] * row_stride + torch.arange(width) * col_stride
+    if pointer == x.data_ptr():      # else a copy, whose strides are its shape's
+        own = x.as_strided((int(at.max()) + 1,), (1,))
+        assert torch.equal(own[at], x)
+    else:
+        assert (row_stride, col_stride) == (width, 1)
