@@ -134,7 +134,7 @@ def experts(layer, x, offsets, perm_tokens, out_dtype=None, out=None, workspace=
     layer (DeviceExpertLayer.quantize_fp8 or from_fp8), offsets and perm_tokens int32 as
     hm_permute gives them.  A workspace (uint8, workspace_bytes(...)) may be kept by the caller."""
     torch = _torch()
-    device = check_on_device(x, offsets, perm_tokens, layer.packed, out, workspace)
+    device = check_on_device(x, offsets, perm_tokens, layer.packed, layer.scale, out, workspace)
     tokens, pairs = x.shape[0], perm_tokens.numel()
     if x.dim() != 2 or x.shape[1] != layer.hidden or not x.is_contiguous():
         raise ValueError(f"x must be a contiguous [tokens, {layer.hidden}] tensor")

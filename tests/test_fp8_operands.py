@@ -87,3 +87,27 @@ def test_quantize_views(calls, what, x):
         assert torch.equal(own[at], x)
     else:
         assert (row_stride, col_stride) == (width, 1)
+
+
+def _one_device(*tensors):
+    """check_on_device with the host in the place of a GPU."""
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise ValueError(f"the operands must share one GPU, got {devices}")
+    return devices.pop()
+
+
+@pytest.mark.parametrize("part", ["packed", "scale"])
+def test_experts_of_a_layer_elsewhere(calls, monkeypatch, part):
+    """Both of a layer's arrays have to be where the rows are."""
+    monkeypatch.setattr(fp8, "check_on_device", _one_device)
+    monkeypatch.setattr(fp8, "workspace_bytes", lambda *a: 16)
+    w = [torch.zeros((2, 128, 128), dtype=torch.uint8) for _ in range(3)]
+    layer = block.DeviceExpertLayer.from_fp8(*w, *[torch.ones((2, 1, 1)) for _ in range(3)])
+    args = torch.ones((4, 128)), torch.tensor([0, 4, 4], dtype=torch.int32), torch.arange(4, dtype=torch.int32)
+    fp8.experts(layer, *args)
+    assert len(calls) == 1
+    setattr(layer, part, getattr(layer, part).to("meta"))
+    with pytest.raises(ValueError, match="share one GPU"):
+        fp8.experts(layer, *args)
+    assert len(calls) == 1
