@@ -127,6 +127,12 @@ class DeviceExpertLayer:
                         inter)
 
 
+def check_current_device(layer):
+    """Buffers and streams are the current device's; an FP8 layer (from_fp8) may be on another."""
+    if layer.dtype == capi.HM_DTYPE_FP8 and layer.packed.device.index != _torch().cuda.current_device():
+        raise ValueError(f"the layer is on {layer.packed.device}, not on the current device")
+
+
 @dataclass
 class ExpertBatch:
     """ExpertBatch (src/experts/ExpertBatch.hpp:10-18)."""
@@ -161,8 +167,7 @@ class MoEBlock:
 
     def _buffers(self, tokens: int, exec_flags: int = 0):
         torch = _torch()
-        if self.layer.dtype == capi.HM_DTYPE_FP8 and self.layer.packed.device.index != torch.cuda.current_device():
-            raise ValueError(f"the layer is on {self.layer.packed.device}, not on the current device")
+        check_current_device(self.layer)
         nbytes = capi.load().hm_moe_block_workspace_bytes(
             C.byref(self.layer.desc), tokens, self.top_k, self.limbs_x, self.limbs_z, exec_flags)
         if nbytes == 0:

@@ -20,7 +20,7 @@ import ctypes as C
 import numpy as np
 
 from . import capi
-from .block import DeviceExpertLayer
+from .block import DeviceExpertLayer, check_current_device
 
 
 def _torch():
@@ -40,6 +40,8 @@ class MoEStack:
         h0 = layers[0].hidden
         if any(l.hidden != h0 for l in layers):
             raise ValueError("all layers share the hidden size")
+        for l in layers:
+            check_current_device(l)
         self.layers, self.router_w = layers, router_w
         self.top_k, self.eps, self.flags = top_k, eps, flags
         self.limbs_x, self.limbs_z = limbs_x, limbs_z

@@ -6,7 +6,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from hmoe import block, fp8  # noqa: E402
+from hmoe import block, fp8, stack  # noqa: E402
 
 
 @pytest.fixture
@@ -14,6 +14,7 @@ def on_host(monkeypatch):
     """The entry points' checks on host tensors."""
     monkeypatch.setattr(fp8, "_torch", lambda: torch)
     monkeypatch.setattr(block, "_torch", lambda: torch)
+    monkeypatch.setattr(stack, "_torch", lambda: torch)
     monkeypatch.setattr(block, "check_on_device", lambda *t: t[0].device)
 
 
@@ -111,3 +112,18 @@ def test_experts_of_a_layer_elsewhere(calls, monkeypatch, part):
     with pytest.raises(ValueError, match="share one GPU"):
         fp8.experts(layer, *args)
     assert len(calls) == 1
+
+
+@pytest.mark.parametrize("entry", ["block", "stack"])
+def test_layer_on_another_device(on_host, monkeypatch, entry):
+    """A block and a stack refuse an FP8 layer that is not on the current device, whose memory their
+    buffers and their stream belong to."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    w = [torch.zeros((2, 128, 128), dtype=torch.uint8) for _ in range(3)]
+    layer = block.DeviceExpertLayer.from_fp8(*w, *[torch.ones((2, 1, 1)) for _ in range(3)])
+    layer.packed = type("Elsewhere", (), {"device": torch.device("cuda", 1)})()
+    with pytest.raises(ValueError, match="cuda:1"):
+        if entry == "block":
+            block.MoEBlock(layer, 1)._buffers(4)
+        else:
+            stack.MoEStack([layer], [torch.zeros((128, 2))], 1)
