@@ -20,11 +20,13 @@ __global__ __launch_bounds__(64 * kSWaves) void f8_stream_kernel(Product p, T* _
     __shared__ __attribute__((aligned(16))) v4f s_part[kSWaves][NP * MT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int j = lane & 15, g = lane >> 4;
-    Tile t = {0, (int64_t)blockIdx.y * 16 * MT, 0};
+    const int64_t tile = (int64_t)blockIdx.z * gridDim.y + blockIdx.y;
+    Tile t = {0, tile * 16 * MT, 0};
     if (p.offsets) {
-        if (!locate(p.offsets, p.experts, p.rows, 16 * MT, blockIdx.y, &t)) return;
+        if (!locate(p.offsets, p.experts, p.rows, 16 * MT, tile, &t)) return;
     } else {
         t.nrows = min((int64_t)16 * MT, p.rows - t.row0);
+        if (t.nrows <= 0) return;
     }
     const int64_t nb = hm_f8_blocks(p.K), pitch = nb * kF8Block;
     const int64_t n0 = 16 * (int64_t)blockIdx.x;
@@ -113,8 +115,10 @@ int launch_stream(const Product& p, int64_t m_tiles16, T* y, hipStream_t s) {
     const int mt = p.offsets ? (p.rows <= 16 ? 1 : 4) : stream_mt(p.rows, p.N);
     const int64_t rows_tiles = p.offsets ? (mt == 1 ? m_tiles16 : (p.rows + 63) / 64 + min((int64_t)p.experts, p.rows))
                                          : (p.rows + 16 * mt - 1) / (16 * mt);
-    if (rows_tiles > 65535 || cols > INT_MAX / 512) return HM_ERR_OVERFLOW;
-    const dim3 grid((unsigned)cols, (unsigned)rows_tiles);
+    // (a grid's second and third dimensions hold 65535 each)
+    const int64_t deep = (rows_tiles + 65534) / 65535;
+    if (deep > 65535 || cols > INT_MAX / 512) return HM_ERR_OVERFLOW;
+    const dim3 grid((unsigned)cols, (unsigned)((rows_tiles + deep - 1) / deep), (unsigned)deep);
     if (mt == 1)
         hipLaunchKernelGGL((f8_stream_kernel<1, GU, BROW, T>), grid, dim3(64 * kSWaves), 0, s, p, y);
     else if (mt == 2)

@@ -377,8 +377,8 @@ int hm_limb_partials(const int8_t* digits, int64_t rows, int64_t inner,
  * y must not overlap the operands.
  *
  * HM_ERR_OVERFLOW: over 65535 x 128 rows to quantise, unless block_rows is 1
- * and the columns are contiguous; over 65535 x 64 rows to multiply where w's
- * bytes exceed 4 GiB. */
+ * and the columns are contiguous; over 2^31 - 1 rows or inner columns to
+ * multiply, or over 67 million columns (rows of w). */
 int64_t hm_fp8_pitch(int64_t width);
 int hm_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t width,
                     int64_t row_stride, int64_t col_stride, int32_t block_rows,
