@@ -78,7 +78,7 @@ template <typename T, bool VEC>
 __global__ __launch_bounds__(kQThreads) void f8_quantize_rows_kernel(
     const T* __restrict__ x, int64_t rows, int64_t width, int64_t stride, uint8_t* __restrict__ q,
     float* __restrict__ scale) {
-    quantize_rows<T, VEC>(x, rows, width, stride, q, scale, blockIdx.x);
+    quantize_rows<T, VEC>(x, rows, width, stride, q, scale, (int64_t)blockIdx.y * gridDim.x + blockIdx.x);
 }
 
 // The rows of an expert batch, and (workgroup 0) the table of its m-tiles: entry 0 their number, then
@@ -266,11 +266,13 @@ int launch_quantize(const T* x, int64_t rows, int64_t width, int64_t row_stride,
     if (col_stride == 1) {
         const bool vec = (uintptr_t)x % 16 == 0 && row_stride % (16 / (int64_t)sizeof(T)) == 0;
         if (block_rows == 1) {
-            const int64_t grid = (rows * nb + kQThreads / 16 - 1) / (kQThreads / 16);
-            if (grid > INT_MAX / kQThreads) return HM_ERR_OVERFLOW;
+            // a grid's first dimension holds 2^31 - 1 lanes, its second 65535 times that
+            if (rows > ((int64_t)1 << 42) / nb) return HM_ERR_OVERFLOW;
+            const int64_t groups = (rows * nb + kQThreads / 16 - 1) / (kQThreads / 16);
+            const int64_t deep = (groups + INT_MAX / kQThreads - 1) / (INT_MAX / kQThreads);
             hipLaunchKernelGGL((vec ? f8_quantize_rows_kernel<T, true> : f8_quantize_rows_kernel<T, false>),
-                               dim3((unsigned)grid), dim3(kQThreads), 0, s, x, rows, width, row_stride,
-                               q, scale);
+                               dim3((unsigned)((groups + deep - 1) / deep), (unsigned)deep), dim3(kQThreads),
+                               0, s, x, rows, width, row_stride, q, scale);
         } else {
             const int64_t rb = hm_f8_blocks(rows);
             if (rb > 65535 || nb > INT_MAX / 512) return HM_ERR_OVERFLOW;

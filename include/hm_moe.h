@@ -376,9 +376,10 @@ int hm_limb_partials(const int8_t* digits, int64_t rows, int64_t inner,
  * transposed views of dY and x, both with a scale per row (w_block_rows 1).
  * y must not overlap the operands.
  *
- * HM_ERR_OVERFLOW: over 65535 x 128 rows to quantise, unless block_rows is 1
- * and the columns are contiguous; over 2^31 - 1 rows or inner columns to
- * multiply, or over 67 million columns (rows of w). */
+ * HM_ERR_OVERFLOW: to quantise rows of contiguous columns with block_rows 1,
+ * over 2^42 blocks, 2^40 rows or 2^31 columns; otherwise over 65535 x 128 rows
+ * or 2^29 - 128 columns.  To multiply, over 2^31 - 1 rows or inner columns or
+ * 67 million columns (rows of w). */
 int64_t hm_fp8_pitch(int64_t width);
 int hm_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t width,
                     int64_t row_stride, int64_t col_stride, int32_t block_rows,

@@ -79,3 +79,29 @@ def test_experts_many_pairs(dev):
     assert float(whole.abs().max()) > 0.0
     for lo, hi in ((0, 1 << 20), (pairs // 3 - 500, pairs // 3 + 900), (pairs - 3000, pairs)):
         assert torch.equal(run(lo, hi), whole[lo:hi]), (lo, hi)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_quantize_many_rows(dev, dtype):
+    """More blocks of contiguous rows than 2^31 - 1 lanes of 16 each hold: 2^27 rows and a few, of 1 column."""
+    torch = dev.torch
+    rows = (1 << 27) + 4999
+    print(f"[gpu] fp8 quantize {rows} x 1 {dtype}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    t, code = (torch.float32, capi.HM_DTYPE_FP32) if dtype == "f32" else (torch.bfloat16, capi.HM_DTYPE_BF16)
+    x = torch.randn((rows, 1), device="cuda", generator=g).to(t)
+    x[::1000003] = 0.0
+    q = torch.full((rows + 1, 128), 0xAA, dtype=torch.uint8, device="cuda")
+    scale = torch.full((rows + 1,), -5.0, device="cuda")
+    dev.call("hm_fp8_quantize", x.data_ptr(), code, rows, 1, 1, 1, 1, q.data_ptr(), scale.data_ptr(), dev.stream)
+    dev.sync()
+    assert bool((q[rows] == 0xAA).all()) and float(scale[rows]) == -5.0, "past the end"
+    v = x.double().flatten()
+    want = torch.where(v == 0.0, 0, 0x7e) + torch.where(torch.signbit(v), 0x80, 0)   # +-448: a block of one value
+    step = 1 << 24
+    for lo in range(0, rows, step):
+        part = q[lo:min(rows, lo + step)]
+        assert torch.equal(part[:, 0].long(), want[lo:lo + len(part)]), lo
+        assert not bool(part[:, 1:].any()), lo
+    s64 = v.abs().clamp_min(2.0 ** -100) / 448.0
+    assert bool(((scale[:rows].double() - s64).abs() <= U * s64).all())
