@@ -611,6 +611,30 @@ int hm_fp8_experts(const hm_layer* layer, const void* x, int32_t x_dtype, int64_
     return rc ? rc : hm_f8_experts_down(c, hm_stream(stream));
 }
 
+int hm_debug_fp8_matmul_form(int64_t rows, int64_t inner, int64_t cols, int32_t y_dtype) {
+    if (rows <= 0 || inner <= 0 || cols <= 0 || !hm_row_dtype(y_dtype)) return -1;
+    Product p = {};
+    p.rows = p.x_rows = rows;
+    p.K = inner;
+    p.N = cols;
+    const Form* f = choose_form(p, y_dtype == HM_DTYPE_FP32);
+    return f ? f->bm << 16 | f->bn : 0;
+}
+
+int hm_debug_fp8_experts_form(const hm_layer* layer, int64_t tokens, int64_t pairs, int32_t y_dtype) {
+    if (!layer || layer->dtype != HM_DTYPE_FP8 || layer->experts <= 0 || layer->hidden <= 0 ||
+        layer->intermediate <= 0 || tokens <= 0 || pairs <= 0 || !hm_row_dtype(y_dtype))
+        return -1;
+    hm_f8_experts_call c = {};
+    c.layer = layer;
+    c.pairs = pairs;
+    c.y_dtype = y_dtype;
+    const bool exact = exact_z(c);
+    const ExpertsForm f = experts_form(layer, tokens, pairs, exact);
+    if (f.kind != Experts::kTiles) return f.kind == Experts::kDecode ? 16 : 0;
+    return exact ? f.bm << 16 : f.bm;
+}
+
 int hm_fp8_pack_layer(const void* payload, int32_t dtype, int64_t experts, int64_t hidden,
                       int64_t intermediate, void* packed, float* scale, void* stream) {
     HM_REQUIRE(payload && packed && scale && payload != packed && experts > 0 && hidden > 0 &&

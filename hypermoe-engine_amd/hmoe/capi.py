@@ -105,6 +105,8 @@ SIGNATURES = {
     "hm_dispatch_rows_grad": (c_i32, [vp, vp, vp, vp, c_i64, c_i32, c_i64, c_i64, c_i32, vp, vp, vp]),
     "hm_combine_rows": (c_i32, [vp, vp, vp, vp, c_i64, c_i32, c_i64, c_i64, c_i32, vp, vp]),
     "hm_combine_rows_grad": (c_i32, [vp, vp, vp, vp, c_i64, c_i32, c_i64, c_i64, c_i32, vp, vp, vp]),
+    "hm_debug_fp8_matmul_form": (c_i32, [c_i64, c_i64, c_i64, c_i32]),
+    "hm_debug_fp8_experts_form": (c_i32, [C.POINTER(HmLayer), c_i64, c_i64, c_i32]),
     "hm_debug_expf": (c_i32, [vp, vp, c_i64, vp]),
 }
 

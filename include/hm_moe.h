@@ -460,6 +460,15 @@ int hm_combine_rows_grad(const void* dout, const void* y, const int32_t* slots,
  * The device restatement of glibc expf used by the router softmax and SiLU,
  * evaluated elementwise (parity of the libm boundary). */
 int hm_debug_expf(const float* x, float* y, int64_t n, void* stream);
+/* Which kernel an FP8 call of these sizes takes, so that a test of one is a
+ * test of that one.  Products: rows of x << 16 | rows of w of a tile, 0 the
+ * kernel that streams w.  Experts: 16 the kernels for few rows, 0 streamed
+ * weights, else the rows of a tile (<< 16 where gate and up use the exact
+ * products).  -1: not a call. */
+int hm_debug_fp8_matmul_form(int64_t rows, int64_t inner, int64_t cols,
+                             int32_t y_dtype);
+int hm_debug_fp8_experts_form(const hm_layer* layer, int64_t tokens,
+                              int64_t pairs, int32_t y_dtype);
 
 #ifdef __cplusplus
 }
