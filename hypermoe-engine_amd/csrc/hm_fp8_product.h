@@ -36,11 +36,13 @@ __device__ __forceinline__ v8i load_frag(const uint8_t* block, int g) {
                      *reinterpret_cast<const v4i*>(block + 16 * (g + 4)));
 }
 
-// The FP8 instruction aligns each eight consecutive products to the largest of them and drops what
-// lies more than 13 bits below it (measured: 2^16 + 2^2 is 2^16 inside a group of eight and exact
-// across groups), 1.3e-5 to 2.4e-5 of a sum's norm: under a sixth of FP16's rounding step and a
-// hundredth of BF16's, but 300 times FP32's.  Where that shows, the operands are widened to fp16 (exact)
-// for v_mfma_f32_16x16x32_f16, whose sums are FP32 (1e-8), at half the rate: Frag<true>.
+// The FP8 instruction aligns each eight consecutive products, by the sums of their exponents, to the
+// largest of them and cuts what lies more than 13 bits below it (measured: 2^16 + 2^2 is 2^16 inside a group
+// of eight and exact across groups): at most 2^-10 of sum |x w|.  Of a result's norm that is 1.5e-5 for
+// normally distributed operands, under a tenth of FP16's rounding and a hundredth of BF16's, and 5.1e-5 for
+// bytes spread evenly over the format, but 150 to 400 times FP32's sums.  Where that shows, the operands
+// are widened to fp16 (exact) for v_mfma_f32_16x16x32_f16, whose sums are FP32 (1.1e-7 over 4096 columns),
+// at half the rate: Frag<true>.
 template <bool PREC>
 struct Frag;
 template <>

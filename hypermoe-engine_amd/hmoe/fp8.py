@@ -109,7 +109,9 @@ def quantize(x, block_rows: int = 1) -> Matrix:
 
 
 def matmul(x: Matrix, w: Matrix, out_dtype=None, out=None):
-    """x w^T, [x.rows, w.rows] in out_dtype (default bfloat16)."""
+    """x w^T, [x.rows, w.rows] in out_dtype (default bfloat16).  float32 results are FP32 sums of the exact
+    products; 16-bit ones of many rows take the FP8 matrix instruction (twice the rate, about 1.5e-5 of
+    the result's norm off before the rounding)."""
     torch = _torch()
     device = check_on_device(x.q, x.scale, w.q, w.scale, out)
     if x.width != w.width:
@@ -132,7 +134,8 @@ def matmul(x: Matrix, w: Matrix, out_dtype=None, out=None):
 def experts(layer, x, offsets, perm_tokens, out_dtype=None, out=None, workspace=None):
     """The SwiGLU experts of a routed batch: grouped rows [pairs, H] of x [tokens, H] through an FP8
     layer (DeviceExpertLayer.quantize_fp8 or from_fp8), offsets and perm_tokens int32 as
-    hm_permute gives them.  A workspace (uint8, workspace_bytes(...)) may be kept by the caller."""
+    hm_permute gives them.  Rows from offsets[E] on keep what `out` held (of a new one: undefined).
+    A workspace (uint8, workspace_bytes(...)) may be kept by the caller."""
     torch = _torch()
     device = check_on_device(x, offsets, perm_tokens, layer.packed, layer.scale, out, workspace)
     tokens, pairs = x.shape[0], perm_tokens.numel()

@@ -370,11 +370,23 @@ int hm_limb_partials(const int8_t* digits, int64_t rows, int64_t inner,
  * hm_fp8_matmul: y[m, n] = sum_b xs[m, b] ws[n / w_block_rows, b]
  * sum_{k in block b} x[m, k] w[n, k], x [rows x inner] with a scale per row
  * and block, w [cols x inner] with w_block_rows 128 or 1, y [rows x cols] in
- * y_dtype (FP32, FP16, BF16).  Sums and scale products are FP32, in an order
- * that the sizes fix.  A layer's product: x W^T.  Its input's gradient: dY
- * times the quantised transposed view of W.  Its weight's gradient: the
- * transposed views of dY and x, both with a scale per row (w_block_rows 1).
- * y must not overlap the operands.
+ * y_dtype (FP32, FP16, BF16).  A layer's product: x W^T.  Its input's
+ * gradient: dY times the quantised transposed view of W.  Its weight's
+ * gradient: the transposed views of dY and x, both with a scale per row
+ * (w_block_rows 1).  y must not overlap the operands.
+ * Sums: the sizes and y_dtype fix their order, so a call repeats its bits, but
+ * a row's may differ with the number of rows beside it.  FP32 results are FP32
+ * sums of the exact products (1.1e-7 of the result's norm over 4096 columns).
+ * FP16 and BF16 results of many rows take the FP8 matrix instruction, which
+ * aligns eight consecutive products to the largest and drops what lies more
+ * than 13 bits below it: at most 2^-10 of sum |x w|; 1.5e-5 of the result's
+ * norm for normally distributed operands, 5.1e-5 for bytes spread evenly over
+ * the format (FP16's own rounding: 2.1e-4).  A caller that needs the FP32 sums
+ * asks for FP32 results, at half the rate.
+ * Scales: xs ws is one FP32 product.  Where it passes the largest float (the
+ * blocks' maxima multiply to over 6.8e43) the outputs that it enters are
+ * infinite or NaN, also where the block's sum is small enough for a finite
+ * one; below 2^-126 it has the bits of a subnormal.
  *
  * HM_ERR_OVERFLOW: to quantise rows of contiguous columns with block_rows 1,
  * over 2^42 blocks, 2^40 rows or 2^31 columns; otherwise over 65535 x 128 rows
@@ -394,8 +406,14 @@ int hm_fp8_matmul(const uint8_t* xq, const float* xs, const uint8_t* wq,
  * groups of MoERuntime.cpp:282-306) with the weights of an FP8 layer:
  * grouped row g of expert e, offsets[e] <= g < offsets[e + 1], is
  *   y[g] = z D_e^T,  z = silu(x[perm_tokens[g]] G_e^T) * (x[..] U_e^T),
- * x and z each quantised as by hm_fp8_quantize(block_rows 1) before their
- * product.  layer->packed holds, expert after expert, gate [I x pitch(H)],
+ * x and z each quantised to a scale per row and 128 columns before their
+ * product: x as by hm_fp8_quantize, z from FP32 values, scale and quotients
+ * within two units in the last place of hm_fp8_quantize's.  y's sums are those
+ * of F1.  z's are FP32 sums of the exact products, except for BF16 y and at
+ * least 128 pairs an expert: there gate and up take the FP8 instruction, and a
+ * byte of z next to a border may move by a step (an error of 2.0e-3 of y's
+ * norm in all, where FP32 sums leave 1.7e-3, BF16's own rounding; FP32 or FP16
+ * y avoids it).  layer->packed holds, expert after expert, gate [I x pitch(H)],
  * up [I x pitch(H)] and down [H x pitch(I)] bytes, layer->scale [E x 3 x
  * ceil(H / 128) ceil(I / 128)] their block scales, each projection's in its
  * own [ceil(N / 128) x ceil(K / 128)] order; zero_point is unused.  x
