@@ -6,10 +6,10 @@
 //                                                             dx[t] = sum_r w g[slot(t,r)]
 //   combine        out[t] = res[t] + sum_r w y[slot(t,r)]     dw = <g[t], y[slot(t,r)]>,
 //                                                             dy[slot(t,r)] = w g[t]
-// so there are two movements, each the other's gradient: `spread` writes a token's row to its slots,
-// `join` sums a token's slots, and either takes the dot products of the rows it walks in the same
-// pass.  A pair with a slot outside [0, rows) is one that no expert took: it is written nowhere, adds
-// nothing and has weight gradient 0.
+// so there are two movements, each the other's gradient: `spread` writes a token's row to its slots and
+// takes the dot products in the same pass; `join` sums a token's slots and takes theirs in a second pass
+// over the same rows.  A pair with a slot outside [0, rows) is one that no expert took: it is written
+// nowhere, adds nothing and has weight gradient 0.
 //
 // Bound by the rows' bytes (one read or write each; the products are a few operations a value).  A
 // workgroup owns a token, or without dot products a column chunk of it, so every sum has one owner
