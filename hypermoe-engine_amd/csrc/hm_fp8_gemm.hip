@@ -119,12 +119,10 @@ int launch_stream(const Product& p, int64_t m_tiles16, T* y, hipStream_t s) {
     const int64_t deep = (rows_tiles + 65534) / 65535;
     if (deep > 65535 || cols > INT_MAX / 512) return HM_ERR_OVERFLOW;
     const dim3 grid((unsigned)cols, (unsigned)((rows_tiles + deep - 1) / deep), (unsigned)deep);
-    if (mt == 1)
-        hipLaunchKernelGGL((f8_stream_kernel<1, GU, BROW, T>), grid, dim3(64 * kSWaves), 0, s, p, y);
-    else if (mt == 2)
-        hipLaunchKernelGGL((f8_stream_kernel<2, GU, BROW, T>), grid, dim3(64 * kSWaves), 0, s, p, y);
-    else
-        hipLaunchKernelGGL((f8_stream_kernel<4, GU, BROW, T>), grid, dim3(64 * kSWaves), 0, s, p, y);
+    auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * kSWaves), 0, s, p, y); };
+    if (mt == 1) run(f8_stream_kernel<1, GU, BROW, T>);
+    else if (mt == 4) run(f8_stream_kernel<4, GU, BROW, T>);
+    else if constexpr (!GU) run(f8_stream_kernel<2, GU, BROW, T>);   // (groups take 1 or 4)
     HM_LAUNCHED();
     return HM_OK;
 }

@@ -477,7 +477,7 @@ int hm_f8_launch_gateup_tiles(int bm, bool prec, const Product& p, const int4* t
     if (prec)
         return bm == 128 ? launch<4, 4, 3, true, false, true, float>(p, table, m_tiles, none, zq, zs, s)
                          : launch<2, 4, 3, true, false, true, float>(p, table, m_tiles, none, zq, zs, s);
-    if (bm == 256) return launch<8, 4, 2, true, false, false, float>(p, table, m_tiles, none, zq, zs, s);
-    return bm == 128 ? launch<4, 4, 3, true, false, false, float>(p, table, m_tiles, none, zq, zs, s)
-                     : launch<2, 4, 3, true, false, false, float>(p, table, m_tiles, none, zq, zs, s);
+    // (the FP8 instruction from 128 rows an expert on, which have no 64-row tiles)
+    return bm == 256 ? launch<8, 4, 2, true, false, false, float>(p, table, m_tiles, none, zq, zs, s)
+                     : launch<4, 4, 3, true, false, false, float>(p, table, m_tiles, none, zq, zs, s);
 }
