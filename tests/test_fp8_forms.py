@@ -13,7 +13,7 @@ from hmoe import capi
 def test_every_form_has_cases():
     fast, exact = ({c[i] for c in F.MATMULS} - {0} for i in (0, 1))
     assert fast == {F.F64, F.F128, F.FW, F.F256} and exact == {F.F64, F.F128, F.FW}
-    assert {c[0] for c in F.EXPERTS} == {0, 64, 128, 256}
+    assert {c[0] for c in F.EXPERTS} == {0, 16, 64, 128, 256}
 
 
 @pytest.mark.parametrize("fast,exact,m,k,n", F.MATMULS)
