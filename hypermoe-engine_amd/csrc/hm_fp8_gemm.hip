@@ -12,8 +12,9 @@ constexpr int kSWaves = 8;
 
 // Weights streamed from memory: a workgroup of 8 waves owns 16 MT rows x 16 outputs (GU: 16 gate and
 // 16 up outputs, z = silu(g) u), its waves split K by blocks and their sums meet in the LDS in wave
-// order.  BROW: w has a scale for each of its rows.  Bound by latency: one row of 2048 x 2048 3.6 us,
-// 333 x 1000 x 777 (FP32) 7.8.
+// order.  BROW: w has a scale for each of its rows.  Bound by latency: one row of 2048 x 2048 3.8 us,
+// 333 x 1000 x 777 (FP32) 8.0: eight blocks of K for eight waves, each of which widens five fragments for
+// four products, and 294 workgroups on 256 CUs.
 template <int MT, bool GU, bool BROW, typename T>
 __global__ __launch_bounds__(64 * kSWaves) void f8_stream_kernel(Product p, T* __restrict__ y) {
     constexpr int NP = GU ? 2 : 1;
@@ -132,8 +133,8 @@ int launch_stream(const Product& p, int64_t m_tiles16, T* y, hipStream_t s) {
 // of 8 waves owns 8 / KP x 16 outputs (GU: gate and up) of up to 16 rows of one expert.  Its weights are
 // sent for first (KP waves split K, two blocks each in flight), then its rows are cut to 8 bits into the
 // LDS, 16 lanes a block, so that nothing is launched before or between the products; the waves' sums
-// meet in the LDS in wave order.  One token, top-8 of 128 experts of 2048 x 768: gate/up 8.4 us (25 MB),
-// down 5.1 (13 MB), 13.7 as called; by quantisation and tiles 19.4.
+// meet in the LDS in wave order.  One token, top-8 of 128 experts of 2048 x 768: 13.6 us as called,
+// under the tracer gate/up 8.9 us (25 MB) and down 6.2 (13 MB); by quantisation and tiles 19.4.
 struct Decode {
     const void* x;
     const uint8_t* w;
@@ -401,7 +402,8 @@ struct ExpertsPlan {
 // 24.7).  Others take tiles of 64 rows, or 128 where an expert has that many on average (128 experts
 // top-8, 2048 tokens: 194 us against 211; 1024: 168 against 160), or, with the FP8 instruction, 256 from
 // 384 rows an expert (6144 tokens: 367 us against 395; 4096: 315 against 293; 8 experts top-2 of 4096 x
-// 2048, 16384 tokens: 932 us, 1.77 PFLOP/s, against 1079).
+// 2048, 16384 tokens: 932 us, 1.77 PFLOP/s, against 1079).  The decode kernels keep 16 rows in 64 KiB of LDS
+// (decode_lds), so that two workgroups share a CU: H and I up to 3840.
 constexpr int64_t kDecodePairs = 16, kDecodeBytes = (int64_t)1 << 27;
 bool decode_rows(const hm_layer* L, int64_t pairs) {
     if (pairs <= kDecodePairs) return true;

@@ -16,10 +16,12 @@
 // Epilogue of gate/up (GU): z = silu(g) u for one block of 128 columns; its maximum over the block goes
 // over lanes, then through the LDS over the four waves of a row; the bytes and scale are stored.
 //
-// Bound by the matrix instructions and the clock they leave: 4096 x 4096 x 4096 to BF16 63.5 us, 2.16
-// PFLOP/s (the library's product with one scale for all: 2.62), matrix pipes 56 % busy at 1.85 GHz, waves
-// waiting for operands 29 % and for an issue slot 35 % of their time.  FP32 results 136 us.  128 experts
-// top-8 of 2048 x 768, 4096 tokens: gate/up 190 us (403 MB of weights, 206 GFLOP), down 109.
+// Bound by the matrix instructions and the clock they leave: 4096 x 4096 x 4096 to BF16 65 us, 2.1
+// PFLOP/s (the library's product with one scale for all: 2.5 to 2.6), matrix pipes 55 % busy at 1.73 GHz,
+// waves waiting for operands 30 % and for an issue slot 35 % of their time.  FP32 results 139 us.  128
+// experts top-8 of 2048 x 768, 4096 tokens, to BF16: gate/up 182 us (206 GFLOP; 634 MB read where weights and
+// rows are 411, because m-tiles of an expert read them again), down 105.  Results off 16 bytes are stored
+// value by value: 4096 x 4096 x 2048 to BF16 41 us, 2044 to 2047 columns 62; to FP32 75, and 95 where odd.
 #include "hm_fp8_product.h"
 #include "hm_lds_dma.h"
 

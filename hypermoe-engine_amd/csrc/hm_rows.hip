@@ -14,8 +14,9 @@
 // Bound by the rows' bytes (one read or write each; the products are a few operations a value).  A
 // workgroup owns a token, or without dot products a column chunk of it, so every sum has one owner
 // and a fixed order (ranks ascending): no atomics, the same bits every run.  4096 tokens, top-8, 2048
-// wide, BF16: dispatch 26 us (151 MB), join 40 (168 MB), combine's gradient with both results 49 (285
-// MB): 4.2 to 5.8 TB/s where a large copy reaches 4.8.
+// wide, BF16: dispatch 26 us (151 MB), join 26 to 47 (168 MB; the least where the rows are still in the
+// caches), with dot products 49, combine's gradient with both results 49 (285 MB): 4.2 to 5.8 TB/s where a
+// large copy reaches 4.8.
 #include "hm_fp8.h"
 
 #include <limits.h>
