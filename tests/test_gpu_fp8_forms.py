@@ -266,3 +266,42 @@ def test_experts_form(dev, bm, ydtype, e, h, i, pairs):
     # step: 2 * 0.8 d * 0.09 of z's square for an error d of z's norm, which is sqrt(2) times a product's
     # 2.4e-5 (1.7e-6 where gate and up are FP32 sums of cancelling terms); and down's own window
     norms.check(2.2e-3 if not exact else 5e-4)
+
+
+@pytest.mark.parametrize("bm,ydtype,e,h,i,pairs", [(16, "bf16", 6, 300, 200, 40), (64, "f16", 6, 400, 300, 400),
+                                                   (128, "bf16", 4, 400, 300, 1400), (256, "bf16", 3, 400, 300, 1900),
+                                                   (0, "bf16", 6, 200, 300, 400)])
+def test_tokens_out_of_range(dev, bm, ydtype, e, h, i, pairs):
+    """A pair whose token is not one of the batch reads token 0, in every form; groups that begin after row
+    0 and end before the last leave the rows around them as they were."""
+    torch = dev.torch
+    tokens = 50
+    layer = capi.HmLayer(e, h, i, capi.HM_DTYPE_FP8, 16, 16, None)
+    form = dev.lib.hm_debug_fp8_experts_form(C.byref(layer), tokens, pairs, CODES[ydtype])
+    assert (form & 0xffff or form >> 16) == bm
+    print(f"[gpu] fp8 experts of tokens out of range, E={e} H={h} I={i} P={pairs} {ydtype}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(pairs)
+    packed = _random_bytes(torch, g, e, 2 * i * _pitch(h) + h * _pitch(i)).view(torch.uint8)
+    for at, n, k in ((0, 2 * i, h), (2 * i * _pitch(h), h, i)):   # zeros past the width
+        packed[:, at:at + n * _pitch(k)].view(e, n, _pitch(k))[:, :, k:] = 0
+    scale = torch.rand((e, 3, (_pitch(h) // 128) * (_pitch(i) // 128)), device="cuda", generator=g) * 1e-3
+    layer.packed, layer.scale = packed.data_ptr(), scale.data_ptr()
+    sizes = torch.full((e,), (pairs - 9) // e)
+    offsets = (torch.cat([torch.zeros(1), sizes.cumsum(0)]) + 4).int().cuda()
+    lo, hi = 4, int(offsets[-1])
+    perm = torch.randint(0, tokens, (pairs,), device="cuda", generator=g).int()
+    bad = perm.clone()
+    bad[::3], bad[1::7], bad[2::11] = -1, tokens, 2 ** 31 - 1
+    perm[(bad < 0) | (bad >= tokens)] = 0
+    x = torch.randn((tokens, h), device="cuda", generator=g).to(_type(torch, ydtype))
+    need = dev.lib.hm_fp8_experts_workspace_bytes(C.byref(layer), tokens, pairs)
+    work = torch.empty(need, dtype=torch.uint8, device="cuda")
+    got = []
+    for p in (perm, bad):
+        y = torch.full((pairs, h), -77.0, dtype=x.dtype, device="cuda")
+        dev.call("hm_fp8_experts", C.byref(layer), x.data_ptr(), CODES[ydtype], tokens, offsets.data_ptr(),
+                 p.data_ptr(), pairs, y.data_ptr(), CODES[ydtype], work.data_ptr(), need, dev.stream)
+        dev.sync()
+        got.append(y)
+    assert torch.equal(*got) and bool((got[0][:lo] == -77.0).all()) and bool((got[0][hi:] == -77.0).all())
+    assert bool(torch.isfinite(got[0]).all()) and not bool((got[0][lo:hi] == -77.0).all(1).any())
