@@ -22,6 +22,8 @@ HM_GEMV_MAX_PAIRS = 64
 HM_EXEC_ROUTE_SEQUENTIAL = 0x400
 HM_DTYPE_FP32, HM_DTYPE_FP16, HM_DTYPE_BF16, HM_DTYPE_INT8, HM_DTYPE_FP8 = 0, 1, 2, 3, 4
 HM_FP8_BLOCK = 128
+HM_GROUPED_MAX_GROUPS = 1024
+HM_ADAPTER_MAX_RANK = 256
 
 
 class HmLayer(C.Structure):
@@ -105,6 +107,17 @@ SIGNATURES = {
     "hm_dispatch_rows_grad": (c_i32, [vp, vp, vp, vp, c_i64, c_i32, c_i64, c_i64, c_i32, vp, vp, vp]),
     "hm_combine_rows": (c_i32, [vp, vp, vp, vp, c_i64, c_i32, c_i64, c_i64, c_i32, vp, vp]),
     "hm_combine_rows_grad": (c_i32, [vp, vp, vp, vp, c_i64, c_i32, c_i64, c_i64, c_i32, vp, vp, vp]),
+    "hm_grouped_matmul": (c_i32, [vp, c_i32, vp, c_i32, vp, c_i64, c_i64, c_i64, c_i64, vp, c_i32, vp]),
+    "hm_grouped_swiglu": (c_i32, [vp, c_i32, c_i64, vp, vp, vp, c_i64, c_i64, c_i64, c_i64, vp, vp, vp]),
+    "hm_grouped_swiglu_grad": (c_i32, [vp, c_i32, vp, vp, vp, c_i64, c_i64, c_i64, c_i64, vp, vp, vp]),
+    "hm_grouped_weight_grad_workspace_bytes": (c_sz, [c_i64, c_i64, c_i64, c_i64]),
+    "hm_grouped_weight_grad": (c_i32, [vp, vp, c_i32, vp, c_i64, c_i64, c_i64, c_i64, vp, c_i32, c_i32, vp,
+                                       c_sz, vp]),
+    "hm_adapter_matmul": (c_i32, [vp, c_i32, vp, c_i32, vp, vp, vp, vp, c_i64, c_i64, c_i64, c_i64, c_i64, vp,
+                                  vp, vp]),
+    "hm_adapter_weight_grad_workspace_bytes": (c_sz, [c_i64, c_i64, c_i64, c_i64]),
+    "hm_adapter_weight_grad": (c_i32, [vp, vp, c_i32, vp, c_i64, c_i64, c_i64, c_i64, vp, c_i32, c_i32, vp,
+                                       c_sz, vp]),
     "hm_debug_fp8_matmul_form": (c_i32, [c_i64, c_i64, c_i64, c_i32]),
     "hm_debug_fp8_experts_form": (c_i32, [C.POINTER(HmLayer), c_i64, c_i64, c_i32]),
     "hm_debug_expf": (c_i32, [vp, vp, c_i64, vp]),

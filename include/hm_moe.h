@@ -474,6 +474,100 @@ int hm_combine_rows_grad(const void* dout, const void* y, const int32_t* slots,
                          int64_t rows, int64_t width, int32_t dtype, void* dy,
                          float* dweights, void* stream);
 
+/* ---- F4  Experts held in 16 bits, and their training ---------------------
+ * Grouped products: rows in expert order (hm_dispatch_rows; offsets [groups +
+ * 1] as hm_permute gives them), each group times its own matrix.  Operands
+ * FP16 or BF16 (`dtype`), sums FP32, rounded once to the result's type: dtype,
+ * or FP32 where a result type is asked for.  Matrices are row-major, one after
+ * another: w [groups x cols x inner].  Rows before offsets[0] and from
+ * offsets[groups] on are read by nothing and their results left as they were;
+ * a group may have no rows.  Offsets ascend; what they name past `rows` is left
+ * out.  At most 1024 groups, 2^31 - 1 rows, 2^26 columns and 2^40 values a
+ * matrix.  Outputs must not overlap inputs.
+ *   hm_grouped_matmul       y[g] = x[g] w_e^T, x [rows x inner], y [rows x
+ *                           cols].  w_transposed: w [groups x inner x cols],
+ *                           y[g] = x[g] w_e, which is the input's gradient of
+ *                           the product by the same matrices
+ *   hm_grouped_swiglu       the gate and up products and z[g] = silu(gate) up,
+ *                           from FP32 sums: w [groups x 2 intermediate x
+ *                           hidden], gate rows first; z [rows x intermediate].
+ *                           perm_tokens [rows]: row g reads x[perm_tokens[g]],
+ *                           x [x_rows x hidden] (outside it: row 0); NULL: x's
+ *                           own rows.  pre [rows x 2 intermediate] receives
+ *                           gate | up for the backward pass; may be NULL
+ *   hm_grouped_swiglu_grad  dz[g] = dy[g] w_e (w the down matrices [groups x
+ *                           hidden x intermediate]) kept in FP32, and from it
+ *                           and pre, with s = 1 / (1 + e^-gate): dpre = dz up
+ *                           s (1 + gate (1 - s)) | dz gate s, and z = gate s up
+ *                           again for the down matrices' gradient (NULL: not)
+ *   hm_grouped_weight_grad  dw[e] = sum over the group's rows of dy[g]^T x[g]
+ *                           [cols x inner], zeros for a group without rows;
+ *                           accumulate: added to what dw holds (in FP32, then
+ *                           rounded once).  The workspace holds
+ *                           hm_grouped_weight_grad_workspace_bytes(...) bytes
+ *                           (may be 0); calls that overlap in time need one
+ *                           each.
+ * A sum's order is fixed by the sizes and offsets: no atomics, the same bits
+ * every run. */
+#define HM_GROUPED_MAX_GROUPS 1024
+int hm_grouped_matmul(const void* x, int32_t dtype, const void* w,
+                      int32_t w_transposed, const int32_t* offsets,
+                      int64_t groups, int64_t rows, int64_t inner, int64_t cols,
+                      void* y, int32_t y_dtype, void* stream);
+int hm_grouped_swiglu(const void* x, int32_t dtype, int64_t x_rows,
+                      const int32_t* perm_tokens, const void* w,
+                      const int32_t* offsets, int64_t groups, int64_t rows,
+                      int64_t hidden, int64_t intermediate, void* z, void* pre,
+                      void* stream);
+int hm_grouped_swiglu_grad(const void* dy, int32_t dtype, const void* w,
+                           const void* pre, const int32_t* offsets,
+                           int64_t groups, int64_t rows, int64_t hidden,
+                           int64_t intermediate, void* dpre, void* z,
+                           void* stream);
+size_t hm_grouped_weight_grad_workspace_bytes(int64_t groups, int64_t rows,
+                                              int64_t cols, int64_t inner);
+int hm_grouped_weight_grad(const void* dy, const void* x, int32_t dtype,
+                           const int32_t* offsets, int64_t groups, int64_t rows,
+                           int64_t cols, int64_t inner, void* dw,
+                           int32_t dw_dtype, int32_t accumulate,
+                           void* workspace, size_t workspace_bytes,
+                           void* stream);
+
+/* ---- F5  Low-rank adapters beside a shared projection --------------------
+ * A projection that all rows share, W, and for each row its own adapter a =
+ * ids[row] (outside 0 .. adapters - 1: none), in any order:
+ *   mid[t] = scale[a] x[t] A_a^T,   y[t] = x[t] W^T + mid[t] B_a^T
+ * x [rows x inner], W [cols x inner], down = A [adapters x rank x inner], up =
+ * B [adapters x cols x rank], FP16 or BF16 (`dtype`), scale [adapters] FP32.
+ * mid [rows x rank] (zeros for a row without adapter) and y [rows x cols] have
+ * that type; sums are FP32, mid is rounded once before its product.  Adapters
+ * of smaller rank are padded with zeros.
+ * w_transposed: W [inner x cols], down [adapters x inner x rank], up [adapters
+ * x rank x cols], y = x W + mid up_a.  That is the input's gradient: pass dy,
+ * the same W, B as `down` and A as `up`; mid is then the gradient of mid, with
+ * the scale.
+ * hm_adapter_weight_grad: dw[a] = sum over the rows t with ids[t] = a of
+ * left[t]^T right[t], [left_cols x right_cols]: A's gradient of the gradient of
+ * mid and x, B's of dy and mid.  Zeros for an adapter without rows; accumulate,
+ * dw_dtype and workspace as F4's.  mid and y must not overlap anything.  Rank
+ * up to 256, up to 65535 adapters and 2^23 - 1 rows.
+ * Rows of one adapter side by side are fastest. */
+#define HM_ADAPTER_MAX_RANK 256
+int hm_adapter_matmul(const void* x, int32_t dtype, const void* w,
+                      int32_t w_transposed, const void* down, const void* up,
+                      const float* scale, const int32_t* ids, int64_t adapters,
+                      int64_t rank, int64_t rows, int64_t inner, int64_t cols,
+                      void* mid, void* y, void* stream);
+size_t hm_adapter_weight_grad_workspace_bytes(int64_t adapters, int64_t rows,
+                                              int64_t left_cols,
+                                              int64_t right_cols);
+int hm_adapter_weight_grad(const void* left, const void* right, int32_t dtype,
+                           const int32_t* ids, int64_t adapters, int64_t rows,
+                           int64_t left_cols, int64_t right_cols, void* dw,
+                           int32_t dw_dtype, int32_t accumulate,
+                           void* workspace, size_t workspace_bytes,
+                           void* stream);
+
 /* ---- Test hooks --------------------------------------------------------
  * The device restatement of glibc expf used by the router softmax and SiLU,
  * evaluated elementwise (parity of the libm boundary). */
