@@ -6,44 +6,313 @@
 
 #include <limits.h>
 
+#include <algorithm>
+#include <type_traits>
+
 namespace {
 
 constexpr int kThreads = 256;
 
-// mid of one row: a wave for every fourth rank (k-major), or 256 threads over k and ranks.
+// ---- mid
+// Few rows, each perhaps with an adapter of its own: a wave takes one rank of one row (k-major), or a workgroup 16
+// ranks of one row, k in 16 parts.  Bound by the matrices' bytes and latency.
 template <typename T, bool KM>
-__global__ __launch_bounds__(kThreads) void adapter_mid_kernel(const T* __restrict__ x, const T* __restrict__ down,
-                                                               const float* __restrict__ scale,
-                                                               const int32_t* __restrict__ ids, int adapters,
-                                                               int rank, int64_t K, T* __restrict__ mid) {
+__global__ __launch_bounds__(kThreads) void adapter_mid_rows_kernel(const T* __restrict__ x,
+                                                                    const T* __restrict__ down,
+                                                                    const float* __restrict__ scale,
+                                                                    const int32_t* __restrict__ ids, int adapters,
+                                                                    int rank, int64_t K, T* __restrict__ mid) {
     const int64_t row = blockIdx.x;
     const int a = ids[row];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool has = a >= 0 && a < adapters;
     const T* xr = x + row * K;
     const T* d = down + (int64_t)(has ? a : 0) * rank * K;
-    const float s = has ? scale[a] : 0.0f;
-    for (int r = wave; r < rank; r += kThreads / 64) {
+    if constexpr (KM) {
+        const int lane = threadIdx.x & 63, r = (int)blockIdx.y * (kThreads / 64) + (threadIdx.x >> 6);
+        if (r >= rank) return;
         float v = 0.0f;
-        if (has)
-            for (int64_t k = lane; k < K; k += 64)
-                v = __builtin_fmaf((float)xr[k], (float)(KM ? d[r * K + k] : d[k * rank + r]), v);
+        if (has) {
+            const T* dr = d + (int64_t)r * K;
+#pragma unroll 4
+            for (int64_t k = 8 * lane; k < K; k += 512) {
+                float p[8], q[8];
+                load8(xr + k, (int)min(K - k, (int64_t)8), p);
+                load8(dr + k, (int)min(K - k, (int64_t)8), q);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v = __builtin_fmaf(p[i], q[i], v);
+            }
+        }
 #pragma unroll
         for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m, 64);
-        if (lane == 0) mid[row * rank + r] = has ? (T)(s * v) : (T)0.0f;
+        if (lane == 0) mid[row * rank + r] = has ? (T)(scale[a] * v) : (T)0.0f;
+    } else {
+        __shared__ float s_part[16][17];
+        const int c = threadIdx.x & 15, part = threadIdx.x >> 4, r = (int)blockIdx.y * 16 + c;
+        float v = 0.0f;
+        if (has && r < rank) {
+#pragma unroll 8
+            for (int64_t k = part; k < K; k += 16) v = __builtin_fmaf((float)xr[k], (float)d[k * rank + r], v);
+        }
+        s_part[part][c] = v;
+        __syncthreads();
+        if (part == 0 && r < rank) {
+            for (int i = 1; i < 16; ++i) v += s_part[i][c];
+            mid[row * rank + r] = has ? (T)(scale[a] * v) : (T)0.0f;
+        }
     }
 }
 
+// More rows: a workgroup takes 16 rows and 16 RF ranks, its 8 waves k in parts of 64, straight from memory into
+// fragments (x is read once; the adapters' matrices stay in the L2); once for each adapter that the rows name, its
+// own rows kept.  The waves' sums meet in the LDS in wave order.
+template <typename T, bool KM, int RF>
+__global__ __launch_bounds__(512) void adapter_mid_tile_kernel(const T* __restrict__ x, const T* __restrict__ down,
+                                                               const float* __restrict__ scale,
+                                                               const int32_t* __restrict__ ids, int adapters,
+                                                               int rank, int64_t rows, int64_t K,
+                                                               T* __restrict__ mid) {
+    typedef typename Elem16<T>::v8 v8;
+    __shared__ v4f s_part[8][RF][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i16 = lane & 15, g = lane >> 4;
+    const int64_t row0 = (int64_t)blockIdx.x * 16, row = row0 + i16;
+    const int r0 = (int)blockIdx.y * 16 * RF;
+    int mine = row < rows ? ids[row] : -1;
+    if (mine < 0 || mine >= adapters) mine = -1;
+    const T* xr = x + min(row, rows - 1) * K;
+    // rows without adapter
+    for (int q = threadIdx.x; q < 16 * 16 * RF; q += 512) {
+        const int r = r0 + q % (16 * RF), m = q / (16 * RF);
+        if (row0 + m >= rows || r >= rank) continue;
+        const int id = ids[row0 + m];
+        if (id < 0 || id >= adapters) mid[(row0 + m) * rank + r] = (T)0.0f;
+    }
+    int cur = -1;
+    while (true) {
+        cur = wave_min(mine > cur ? mine : INT_MAX);
+        if (cur == INT_MAX) break;
+        const T* d = down + (int64_t)cur * rank * K;
+        v4f acc[RF] = {};
+        int64_t k0 = 64 * wave;
+        // U parts at a time, all their loads in flight; `whole`: within K
+        auto parts = [&](auto u_, bool whole) __attribute__((always_inline)) {
+            constexpr int U = decltype(u_)::value;
+            v8 xf[U][2], df[U][2][RF];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int64_t k = k0 + 512 * u + 32 * h + 8 * g, n = whole ? 8 : K - k;
+                    xf[u][h] = load_frag8<T>(xr + k, n);
+#pragma unroll
+                    for (int f = 0; f < RF; ++f) {
+                        const int r = min(r0 + 16 * f + i16, rank - 1);   // (ranks past the last are dropped)
+                        if constexpr (KM) {
+                            df[u][h][f] = load_frag8<T>(d + (int64_t)r * K + k, n);
+                        } else {
+                            Loose8<T> w;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) w.v[i] = whole || i < n ? d[(k + i) * rank + r] : (T)0.0f;
+                            df[u][h][f] = __builtin_bit_cast(v8, w);
+                        }
+                    }
+                }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int f = 0; f < RF; ++f) acc[f] = Elem16<T>::mfma(df[u][h][f], xf[u][h], acc[f]);
+            k0 += 512 * U;
+        };
+        constexpr int U = RF == 4 ? 2 : KM ? 4 : 2;
+        while (k0 + 512 * (U - 1) + 64 <= K) parts(std::integral_constant<int, U>{}, true);
+        while (k0 < K) parts(std::integral_constant<int, 1>{}, false);
+#pragma unroll
+        for (int f = 0; f < RF; ++f) s_part[wave][f][lane] = acc[f];
+        __syncthreads();
+        // lane (row i16, ranks 4 g ..) of fragment f
+        const int f = threadIdx.x >> 6;
+        if (f < RF && mine == cur) {
+            v4f v = s_part[0][f][lane];
+#pragma unroll
+            for (int w = 1; w < 8; ++w) v += s_part[w][f][lane];
+            const float s = scale[cur];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = r0 + 16 * f + 4 * g + i;
+                if (r < rank) mid[row * rank + r] = (T)(s * v[i]);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+constexpr int64_t kMidRows = 256;   // rows up to which mid is taken row by row
+
 template <typename T>
-int launch_mid(const void* x, bool km, const void* down, const float* scale, const int32_t* ids, int adapters,
-               int rank, int64_t rows, int64_t K, void* mid, hipStream_t s) {
-    auto run = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(kThreads), 0, s, static_cast<const T*>(x),
-                           static_cast<const T*>(down), scale, ids, adapters, rank, K, static_cast<T*>(mid));
-    };
-    if (km) run(adapter_mid_kernel<T, true>);
-    else run(adapter_mid_kernel<T, false>);
+int launch_mid(const void* x_, bool km, const void* down_, const float* scale, const int32_t* ids, int adapters,
+               int rank, int64_t rows, int64_t K, void* mid_, hipStream_t s) {
+    const T *x = static_cast<const T*>(x_), *down = static_cast<const T*>(down_);
+    T* mid = static_cast<T*>(mid_);
+    if (rows <= kMidRows) {
+        const dim3 grid((unsigned)rows, (unsigned)((rank + (km ? 3 : 15)) / (km ? 4 : 16)));
+        auto run = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, x, down, scale, ids, adapters, rank, K, mid);
+        };
+        if (km) run(adapter_mid_rows_kernel<T, true>);
+        else run(adapter_mid_rows_kernel<T, false>);
+    } else {
+        const int rf = rank <= 16 ? 1 : rank <= 32 ? 2 : 4;
+        const dim3 grid((unsigned)((rows + 15) / 16), (unsigned)((rank + 16 * rf - 1) / (16 * rf)));
+        auto run = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, grid, dim3(512), 0, s, x, down, scale, ids, adapters, rank, rows, K, mid);
+        };
+        if (rf == 1) km ? run(adapter_mid_tile_kernel<T, true, 1>) : run(adapter_mid_tile_kernel<T, false, 1>);
+        else if (rf == 2) km ? run(adapter_mid_tile_kernel<T, true, 2>) : run(adapter_mid_tile_kernel<T, false, 2>);
+        else km ? run(adapter_mid_tile_kernel<T, true, 4>) : run(adapter_mid_tile_kernel<T, false, 4>);
+    }
     HM_LAUNCHED();
+    return HM_OK;
+}
+
+// ---- the matrices' gradients
+// A workgroup takes a 64 x 64 tile of one adapter's gradient over one part of the rows: it collects the rows that are
+// the adapter's, 64 at a time (in ascending order, so sums have one order), moves those rows' columns to the LDS and
+// multiplies them transposed.  Parts meet in a second kernel.  LDS rows are 64 columns of one row, 128 bytes, piece c at
+// c ^ s(row): the 8 rows that the LDS serves at once lie on all of its banks.
+// Bound by the rows' bytes and, for a part, one round trip for each 64 rows.
+constexpr int kGT = 64;
+constexpr int kScan = 1024;   // ids that a wave looks at at once
+
+template <typename T, typename O>
+__global__ __launch_bounds__(kThreads) void adapter_grad_kernel(const T* __restrict__ left, const T* __restrict__ right,
+                                                                const int32_t* __restrict__ ids, int64_t rows,
+                                                                int64_t L, int64_t R, int64_t part_rows,
+                                                                float* __restrict__ parts, O* __restrict__ dw,
+                                                                int accumulate) {
+    typedef typename Elem16<T>::v8 v8;
+    __shared__ __attribute__((aligned(16))) uint8_t s_l[kGT * 128], s_r[kGT * 128];
+    __shared__ int s_list[4][128];   // (each wave its own)
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int wm = wave >> 1, wn = wave & 1, i16 = lane & 15, g = lane >> 4;
+    const int adapter = blockIdx.y;
+    const int64_t ntr = (R + kGT - 1) / kGT;
+    const int64_t l0 = (int64_t)blockIdx.x / ntr * kGT, c0 = (int64_t)blockIdx.x % ntr * kGT;
+    const int64_t beg = (int64_t)blockIdx.z * part_rows, end = min(beg + part_rows, rows);
+    auto swz = [](int r) { return (r & 2) | ((r & 8) >> 1); };
+    const int trow = 8 * g + (i16 >> 2), tc = i16 & 3;
+    const int at0 = trow * 128 + 8 * (tc & 1), pc = tc >> 1;
+    v4f acc[2][2] = {};
+    int head = 0, count = 0;
+    auto stage = [&](int n) __attribute__((always_inline)) {   // the first n of the list
+        Loose8<T> v[2][2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int q = t + kThreads * u, k = q >> 3, col = 8 * (q & 7);
+            const int64_t row = k < n ? s_list[wave][(head + k) & 127] : -1;
+            v[0][u] = __builtin_bit_cast(Loose8<T>, load_frag8<T>(left + row * L + l0 + col,
+                                                                  row >= 0 ? min(L - l0 - col, (int64_t)8) : 0));
+            v[1][u] = __builtin_bit_cast(Loose8<T>, load_frag8<T>(right + row * R + c0 + col,
+                                                                  row >= 0 ? min(R - c0 - col, (int64_t)8) : 0));
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int q = t + kThreads * u, k = q >> 3, at = k * 128 + 16 * ((q & 7) ^ swz(k));
+            *reinterpret_cast<v8*>(s_l + at) = __builtin_bit_cast(v8, v[0][u]);
+            *reinterpret_cast<v8*>(s_r + at) = __builtin_bit_cast(v8, v[1][u]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (32 * h >= n) break;
+            v8 a[2], b[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                b[i] = read_transposed<v8>(s_l + at0 + 32 * h * 128 + 16 * ((4 * wm + 2 * i + pc) ^ swz(trow)), 4 * 128);
+                a[i] = read_transposed<v8>(s_r + at0 + 32 * h * 128 + 16 * ((4 * wn + 2 * i + pc) ^ swz(trow)), 4 * 128);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[i][j] = Elem16<T>::mfma(a[j], b[i], acc[i][j]);
+        }
+        head += n;
+        count -= n;
+    };
+    for (int64_t p0 = beg; p0 < end; p0 += kScan) {
+        int id[kScan / 64];
+#pragma unroll
+        for (int i = 0; i < kScan / 64; ++i) {
+            const int64_t r = p0 + 64 * i + lane;
+            id[i] = r < end ? ids[r] : -1;
+        }
+        for (int i = 0; i < kScan / 64; ++i) {
+            int here = -1;
+#pragma unroll
+            for (int q = 0; q < kScan / 64; ++q) here = q == i ? id[q] : here;
+            const uint64_t m = __ballot(here == adapter);
+            if (!m) continue;
+            if (here == adapter)
+                s_list[wave][(head + count + __popcll(m & ((1ull << lane) - 1))) & 127] = (int)(p0 + 64 * i + lane);
+            count += __popcll(m);
+            if (count >= kGT) stage(kGT);
+        }
+    }
+    if (count > 0) stage(count);
+    // lane: row 16 i + i16 of the wave's 32, columns 4 g .. of its 16 j
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int64_t l = l0 + 32 * wm + 16 * i + i16;
+        if (l >= L) continue;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const int64_t c = c0 + 32 * wn + 16 * j + 4 * g + v;
+                if (c >= R) continue;
+                const int64_t at = ((int64_t)adapter * L + l) * R + c;
+                if (parts) parts[(int64_t)blockIdx.z * gridDim.y * L * R + at] = acc[i][j][v];
+                else dw[at] = (O)(acc[i][j][v] + (accumulate ? (float)dw[at] : 0.0f));
+            }
+    }
+}
+
+template <typename O>
+__global__ __launch_bounds__(kThreads) void adapter_grad_join_kernel(const float* __restrict__ parts, int n,
+                                                                     int64_t size, O* __restrict__ dw,
+                                                                     int accumulate) {
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < size; i += (int64_t)gridDim.x * kThreads) {
+        float v = 0.0f;
+        for (int s = 0; s < n; ++s) v += parts[s * size + i];
+        dw[i] = (O)(v + (accumulate ? (float)dw[i] : 0.0f));
+    }
+}
+
+// Parts that the rows are cut into: so many that about 1024 workgroups share the work, 128 rows a part at least.
+int grad_parts(int64_t adapters, int64_t rows, int64_t L, int64_t R) {
+    const int64_t tiles = ((L + kGT - 1) / kGT) * ((R + kGT - 1) / kGT) * adapters;
+    return (int)std::max((int64_t)1, std::min(std::min((int64_t)1024 / tiles, (rows + 127) / 128), (int64_t)64));
+}
+
+template <typename T, typename O>
+int launch_grad(const void* left, const void* right, const int32_t* ids, int64_t adapters, int64_t rows, int64_t L,
+                int64_t R, void* dw, int accumulate, void* workspace, hipStream_t s) {
+    const int n = grad_parts(adapters, rows, L, R);
+    const int64_t tiles = ((L + kGT - 1) / kGT) * ((R + kGT - 1) / kGT), size = adapters * L * R;
+    if (tiles > INT_MAX / kThreads) return HM_ERR_OVERFLOW;
+    float* parts = n > 1 ? static_cast<float*>(workspace) : nullptr;
+    hipLaunchKernelGGL((adapter_grad_kernel<T, O>), dim3((unsigned)tiles, (unsigned)adapters, (unsigned)n),
+                       dim3(kThreads), 0, s, static_cast<const T*>(left), static_cast<const T*>(right), ids, rows, L, R,
+                       (rows + n - 1) / n, parts, static_cast<O*>(dw), accumulate);
+    HM_LAUNCHED();
+    if (n > 1) {
+        hipLaunchKernelGGL((adapter_grad_join_kernel<O>),
+                           dim3((unsigned)std::min((size + kThreads - 1) / kThreads, (int64_t)4096)), dim3(kThreads), 0, s,
+                           parts, n, size, static_cast<O*>(dw), accumulate);
+        HM_LAUNCHED();
+    }
     return HM_OK;
 }
 
@@ -91,13 +360,16 @@ int hm_adapter_matmul(const void* x, int32_t dtype, const void* w, int32_t w_tra
     p.up = up;
     p.adapters = (int)adapters;
     p.rank = (int)rank;
-    return hm_g_launch_generic(G_ADAPTER, !w_transposed, dtype, dtype, p, s);
+    return hm_g_launch(G_ADAPTER, !w_transposed, dtype, dtype, p, s);
 }
 
 size_t hm_adapter_weight_grad_workspace_bytes(int64_t adapters, int64_t rows, int64_t left_cols,
                                               int64_t right_cols) {
-    (void)adapters, (void)rows, (void)left_cols, (void)right_cols;
-    return 0;
+    if (adapters < 1 || adapters > kMaxAdapters || rows < 0 || left_cols < 1 || right_cols < 1 ||
+        left_cols > kMaxDim || right_cols > kMaxDim || left_cols * right_cols > kMaxMatrix)
+        return 0;
+    const int n = grad_parts(adapters, rows, left_cols, right_cols);
+    return n > 1 ? (size_t)n * adapters * left_cols * right_cols * sizeof(float) : 0;
 }
 
 int hm_adapter_weight_grad(const void* left, const void* right, int32_t dtype, const int32_t* ids,
@@ -113,19 +385,17 @@ int hm_adapter_weight_grad(const void* left, const void* right, int32_t dtype, c
                aligned(ids, 4) && aligned(dw, dw_dtype == HM_DTYPE_FP32 ? 4 : 2));
     const int64_t nw = adapters * left_cols * right_cols * (dw_dtype == HM_DTYPE_FP32 ? 4 : 2);
     HM_REQUIRE(!hm_overlap(dw, nw, left, 2 * rows * left_cols) && !hm_overlap(dw, nw, right, 2 * rows * right_cols));
-    if (workspace_bytes < hm_adapter_weight_grad_workspace_bytes(adapters, rows, left_cols, right_cols))
-        return HM_ERR_INVALID;
-    GProduct p = {};
-    p.x = left;
-    p.w = right;
-    p.y = dw;
-    p.ids = ids;
-    p.rows = rows;
-    p.M = left_cols;
-    p.N = right_cols;
-    p.groups = (int)adapters;
-    p.accumulate = accumulate;
-    return hm_g_launch_generic(G_WEIGHT_GRAD, false, dtype, dw_dtype, p, hm_stream(stream));
+    const size_t need = hm_adapter_weight_grad_workspace_bytes(adapters, rows, left_cols, right_cols);
+    HM_REQUIRE(workspace_bytes >= need && (!need || (workspace && aligned(workspace, 4))));
+    HM_REQUIRE(!need || (!hm_overlap(workspace, need, dw, nw) && !hm_overlap(workspace, need, left, 2 * rows * left_cols) &&
+                         !hm_overlap(workspace, need, right, 2 * rows * right_cols)));
+    const hipStream_t s = hm_stream(stream);
+    auto run = [&](auto launcher) {
+        return launcher(left, right, ids, adapters, rows, left_cols, right_cols, dw, accumulate, workspace, s);
+    };
+    if (dtype == HM_DTYPE_FP16)
+        return dw_dtype == HM_DTYPE_FP32 ? run(launch_grad<hm_f16, float>) : run(launch_grad<hm_f16, hm_f16>);
+    return dw_dtype == HM_DTYPE_FP32 ? run(launch_grad<hm_bf16, float>) : run(launch_grad<hm_bf16, hm_bf16>);
 }
 
 }  // extern "C"

@@ -60,6 +60,7 @@ struct GProduct {
     const void* up;            // adapters matrices [N x rank] or [rank x N]
     int adapters;
     int rank;
+    bool wide;                 // results are aligned to 4 elements
 };
 
 // The SwiGLU's gradient for one value: dz, gate and up to the gradients of both, and z.
@@ -73,6 +74,75 @@ __device__ __forceinline__ void swiglu_grad(float dz, float g, float u, float* d
     *z = a * u;
 }
 
+template <typename T>
+struct __attribute__((packed, aligned(2))) Loose8 {  // 16 bytes aligned to an element
+    T v[8];
+};
+template <>
+struct __attribute__((packed, aligned(4))) Loose8<float> {
+    float v[8];
+};
+// n values (8 at most) from and to rows of any alignment
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int n, float (&f)[8]) {
+    if (n >= 8) {
+        const Loose8<T> w = *reinterpret_cast<const Loose8<T>*>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = (float)w.v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = i < n ? (float)p[i] : 0.0f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int n, const float (&f)[8]) {
+    if (n >= 8) {
+        Loose8<T> w;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w.v[i] = (T)f[i];
+        *reinterpret_cast<Loose8<T>*>(p) = w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = (T)f[i];
+    }
+}
+
+// n values (8 at most) of a row as a fragment's 8, zeros behind them.
+template <typename T>
+__device__ __forceinline__ typename Elem16<T>::v8 load_frag8(const T* p, int64_t n) {
+    typedef typename Elem16<T>::v8 v8;
+    Loose8<T> w;
+    if (n >= 8) {
+        w = *reinterpret_cast<const Loose8<T>*>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w.v[i] = i < n ? p[i] : (T)0.0f;
+    }
+    return __builtin_bit_cast(v8, w);
+}
+
+// A fragment's 8 values of k from the LDS, `next4` bytes from one 4 of them to the next: ds_read_b64_tr_b16, in
+// which lane i of 16 gives the place of 4 consecutive values of row i / 4 and gets the values of 4 rows in column i.
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s* lds_v4s;
+template <typename V>
+__device__ __forceinline__ V read_transposed(const uint8_t* at, int next4) {
+    const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)at);
+    const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s)(at + next4));
+    return __builtin_bit_cast(V, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// The minimum over the wave, in every lane.
+__device__ __forceinline__ int wave_min(int v) {
+    v = min(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));
+    v = min(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
+    v = min(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false));
+    v = min(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false));
+    return min(min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+               min(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+
 // Whether two arrays of so many bytes share memory.
 static inline bool hm_overlap(const void* a, int64_t na, const void* b, int64_t nb) {
     const uint64_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
@@ -80,3 +150,12 @@ static inline bool hm_overlap(const void* a, int64_t na, const void* b, int64_t 
 }
 
 int hm_g_launch_generic(GKind kind, bool w_kmajor, int32_t dtype, int32_t y_dtype, const GProduct& p, hipStream_t s);
+// The tile kernels (hm_grouped_tile.h) for operands aligned to 16 bytes throughout.  form 256: tiles of 256 x 256
+// results, 128: of 128 x 256, 64: of 128 x 128.
+int hm_g_launch_tiles_f16(GKind kind, int form, bool w_kmajor, bool f32, const GProduct& p, hipStream_t s);
+int hm_g_launch_tiles_bf16(GKind kind, int form, bool w_kmajor, bool f32, const GProduct& p, hipStream_t s);
+// The kernel for few rows (hm_grouped_stream.hip): x w^T, SwiGLU or adapters, 16 mt rows a workgroup (1, 2, 4; 8 but
+// for SwiGLU).
+int hm_g_launch_stream(GKind kind, int mt, int32_t dtype, bool f32, const GProduct& p, hipStream_t s);
+// The kernel that a product's sizes and alignment ask for (hm_grouped.hip).
+int hm_g_launch(GKind kind, bool w_kmajor, int32_t dtype, int32_t y_dtype, const GProduct& p, hipStream_t s);

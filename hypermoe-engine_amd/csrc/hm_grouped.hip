@@ -2,6 +2,7 @@
 // SwiGLU's gradient behind the down matrix's, and the weights' gradients; entry points and the kernel for
 // operands of any size and alignment.
 #include "hm_grouped.h"
+#include "hm_lds_dma.h"
 
 #include <limits.h>
 
@@ -13,12 +14,6 @@ constexpr int kBT = 64;        // tile edge
 constexpr int kBK = 32;        // k a step
 constexpr int kPitch = 40;     // values from one row of a staged operand to the next (16-byte pieces)
 constexpr int kThreads = 256;
-
-// 8 values from p, which is aligned to its element only.
-template <typename T>
-struct __attribute__((packed, aligned(2))) Loose8 {
-    T v[8];
-};
 
 // One thread's 8 values of an operand tile [64 x 32]: k-major row t / 4, k 8 (t % 4) ..; else k t / 8, rows
 // 8 (t % 8) .. .  `at(r, k)` is the place of a value, -1 a row that counts as zeros.
@@ -97,9 +92,9 @@ __global__ __launch_bounds__(kThreads) void grouped_generic_kernel(GProduct p) {
     }
     // the rows that are summed over, for the weight gradient
     int64_t kbeg = 0, kend = p.K;
-    if (KIND == G_WEIGHT_GRAD) {  // (with adapters' ids, which may be nullptr where there are no rows: all of them)
-        kbeg = p.offsets ? max(0, p.offsets[e]) : 0;
-        kend = p.offsets ? min((int64_t)p.offsets[e + 1], p.rows) : p.rows;
+    if (KIND == G_WEIGHT_GRAD) {
+        kbeg = max(0, p.offsets[e]);
+        kend = min((int64_t)p.offsets[e + 1], p.rows);
     }
     w += KIND == G_WEIGHT_GRAD ? 0 : (int64_t)e * p.w_group;
 
@@ -138,11 +133,7 @@ __global__ __launch_bounds__(kThreads) void grouped_generic_kernel(GProduct p) {
     if constexpr (KIND == G_WEIGHT_GRAD) {
         for (int64_t k0 = kbeg; k0 < kend; k0 += kBK) {
             const int64_t k = k0 + (t >> 3);
-            bool mine = k < kend;
-            if (p.ids) {
-                mine = mine && p.ids[k] == e;
-                if (!__syncthreads_or(mine)) continue;
-            }
+            const bool mine = k < kend;
             Stage<T, false> sx, sw;
             sx.load_k(mine ? x + k * p.M : nullptr, row0 + 8 * (t & 7), p.M);
             sw.load_k(mine ? w + k * p.N : nullptr, n0 + 8 * (t & 7), p.N);
@@ -294,6 +285,41 @@ int hm_g_launch_generic(GKind kind, bool w_kmajor, int32_t dtype, int32_t y_dtyp
                                   : launch_kind<hm_bf16>(kind, w_kmajor, f32, p, s);
 }
 
+// Whether a product fits the tile kernels: everything that they move in 16 bytes is aligned to that, and offsets
+// from a tile's first row (x's first row where rows are gathered) stay below HM_BUF_RANGE.
+static bool tile_ok(GKind kind, bool w_kmajor, const GProduct& p) {
+    const int64_t top = HM_BUF_RANGE;
+    if (!aligned(p.x, 16) || !aligned(p.w, 16) || p.rows > INT_MAX - 256) return false;
+    if (kind == G_WEIGHT_GRAD) return p.M % 8 == 0 && p.N % 8 == 0;
+    if (p.K % 8 || (!w_kmajor && p.N % 8) || p.K > (int64_t)1 << 22) return false;
+    if (kind == G_ADAPTER) return p.rank % 8 == 0 && aligned(p.mid, 16) && aligned(p.up, 16);
+    return kind != G_SWIGLU || ((p.N + 256) * p.K * 2 < top && (!p.perm || p.x_rows * p.K * 2 < top));
+}
+
+// Which kernel: rows << 16 of a stream workgroup, the form of a tile, 0 for operands off 16 bytes.
+static int pick(GKind kind, bool w_kmajor, const GProduct& p) {
+    const bool nt = w_kmajor && kind != G_WEIGHT_GRAD;
+    const int64_t groups = p.offsets ? p.groups : 1, each = (p.rows + groups - 1) / groups;
+    if (nt && (each <= 16 || p.rows <= 64)) return (p.rows <= 16 || each <= 4 ? 1 : p.rows <= 32 || each <= 8 ? 2 : 4) << 16;
+    if (kind == G_ADAPTER && nt && p.rows <= 128) return 8 << 16;
+    if (!tile_ok(kind, w_kmajor, p)) return 0;
+    const int64_t tm = kind == G_WEIGHT_GRAD ? p.groups * ((p.M + 127) / 128) : p.rows / 128 + groups;
+    if (tm * ((p.N + 255) / 256) < 256) return 64;
+    if (kind == G_WEIGHT_GRAD || each >= 384) return 256;
+    return 128;
+}
+
+int hm_g_launch(GKind kind, bool w_kmajor, int32_t dtype, int32_t y_dtype, const GProduct& p_, hipStream_t s) {
+    GProduct p = p_;
+    const bool f32 = y_dtype == HM_DTYPE_FP32;
+    p.wide = aligned(p.y, f32 ? 16 : 8) && aligned(p.pre_out, 8);
+    const int form = pick(kind, w_kmajor, p);
+    if (!form) return hm_g_launch_generic(kind, w_kmajor, dtype, y_dtype, p, s);
+    if (form >> 16) return hm_g_launch_stream(kind, form >> 16, dtype, f32, p, s);
+    return dtype == HM_DTYPE_FP16 ? hm_g_launch_tiles_f16(kind, form, w_kmajor, f32, p, s)
+                                  : hm_g_launch_tiles_bf16(kind, form, w_kmajor, f32, p, s);
+}
+
 extern "C" {
 
 int hm_grouped_matmul(const void* x, int32_t dtype, const void* w, int32_t w_transposed,
@@ -316,7 +342,7 @@ int hm_grouped_matmul(const void* x, int32_t dtype, const void* w, int32_t w_tra
     p.N = cols;
     p.w_group = inner * cols;
     p.groups = (int)groups;
-    return hm_g_launch_generic(G_MATMUL, !w_transposed, dtype, y_dtype, p, hm_stream(stream));
+    return hm_g_launch(G_MATMUL, !w_transposed, dtype, y_dtype, p, hm_stream(stream));
 }
 
 int hm_grouped_swiglu(const void* x, int32_t dtype, int64_t x_rows, const int32_t* perm_tokens, const void* w,
@@ -346,7 +372,7 @@ int hm_grouped_swiglu(const void* x, int32_t dtype, int64_t x_rows, const int32_
     p.N = intermediate;
     p.w_group = 2 * hidden * intermediate;
     p.groups = (int)groups;
-    return hm_g_launch_generic(G_SWIGLU, true, dtype, dtype, p, hm_stream(stream));
+    return hm_g_launch(G_SWIGLU, true, dtype, dtype, p, hm_stream(stream));
 }
 
 int hm_grouped_swiglu_grad(const void* dy, int32_t dtype, const void* w, const void* pre,
@@ -373,7 +399,7 @@ int hm_grouped_swiglu_grad(const void* dy, int32_t dtype, const void* w, const v
     p.N = intermediate;
     p.w_group = hidden * intermediate;
     p.groups = (int)groups;
-    return hm_g_launch_generic(G_SWIGLU_GRAD, false, dtype, dtype, p, hm_stream(stream));
+    return hm_g_launch(G_SWIGLU_GRAD, false, dtype, dtype, p, hm_stream(stream));
 }
 
 size_t hm_grouped_weight_grad_workspace_bytes(int64_t groups, int64_t rows, int64_t cols, int64_t inner) {
@@ -401,7 +427,7 @@ int hm_grouped_weight_grad(const void* dy, const void* x, int32_t dtype, const i
     p.N = inner;
     p.groups = (int)groups;
     p.accumulate = accumulate;
-    return hm_g_launch_generic(G_WEIGHT_GRAD, false, dtype, dw_dtype, p, hm_stream(stream));
+    return hm_g_launch(G_WEIGHT_GRAD, false, dtype, dw_dtype, p, hm_stream(stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,579 @@
+// hm_grouped_tile.h -- tiles of the 16-bit products (hm_grouped.h) through an LDS ring; one source for each type
+// (hm_grouped_tile_f16.hip, hm_grouped_tile_bf16.hip).
+//
+// Persistent workgroups of 4 waves, 2 (rows of x) x 2 (columns); a wave owns 16 XF x 16 WF results, a tile is
+// BM = 32 XF rows x BN = 32 WF columns.  A stage is 64 of k of both operands, 128 (BM + BN) bytes, moved to the
+// LDS by DMA; the stages of consecutive tiles form one stream, so a tile's first stages load while its
+// predecessor ends.  A stage is two steps of 32 k.  A step multiplies fragments that the step before read from
+// the LDS, so no matrix instruction waits for the LDS; between the two steps lies the one barrier of a stage:
+// the next stage has landed, and this one, which every wave now has in registers, is refilled.
+//   k-major operand   LDS row r is 64 k of one row; its 16-byte piece c sits at position c ^ s(r), and s
+//                     separates the 16 rows that a read takes of one piece.
+//   other operands    LDS row k is BM or BN consecutive values; piece c sits at c ^ s(k).  Read by
+//                     ds_read_b64_tr_b16: 16 lanes read 4 rows of k x 16 values and get them transposed.  The LDS
+//                     serves 32 lanes, 8 rows, at once; s spreads those over all of its banks.
+//   w                 fragment j's row i is column 32 (j / 2) + 8 (i / 4) + 4 (j % 2) + i % 4 of the wave's, so that a
+//                     lane ends with 8 consecutive results of a row from two fragments, and four lanes with 32.  In
+//                     the transposed form j % 2 is (j + i / 4) % 2, or half of the banks would stand idle.
+//   order             tiles are cut into 8 contiguous ranges, one per XCD (workgroup i runs on XCD i % 8); within
+//                     a group m-tiles by SUPER, so what is read by several workgroups at once is in one L2.
+#pragma once
+
+#include "hm_grouped.h"
+#include "hm_lds_dma.h"
+
+#include <limits.h>
+
+#include <algorithm>
+
+namespace {
+
+constexpr int kXcds = 8;
+constexpr int kThreads = 256;
+constexpr int kBK = 64;
+constexpr int kSuper = 4;
+
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+template <typename P>
+__device__ __forceinline__ P* uni(P* p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<P*>(((uint64_t)(uint32_t)uni((int)(v >> 32)) << 32) | (uint32_t)uni((int)v));
+}
+
+struct TileAt {
+    int e;              // group
+    int row0, nrows;    // rows of the tile (weight gradient: of the result)
+    int n0;
+    int k0, kn;         // weight gradient: the group's rows
+    int nb;             // stages of k
+};
+
+template <int WMC, int WNC, int XF, int WF, int NS, GKind KIND, bool WK, typename T, typename O>
+__global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
+    typedef typename Elem16<T>::v8 v8;
+    constexpr bool WG = KIND == G_WEIGHT_GRAD, XK = !WG, GU = KIND == G_SWIGLU;
+    constexpr int NW = WMC * WNC, BM = 16 * XF * WMC, BN = 16 * WF * WNC, SH = GU ? WF / 2 : WF, TN = GU ? BN / 2 : BN;
+    constexpr int STAGE = 128 * (BM + BN), WOFF = 128 * BM;
+    constexpr int XL = BM / 8 / NW, LPW = (BM + BN) / 8 / NW;   // a wave's 1 KB loads a stage, of x first
+    static_assert(XF % 2 == 0 && (SH == 2 || SH == 4 || SH == 8) && BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "tile");
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * STAGE];
+    __shared__ int s_pre[WG ? 1 : HM_GROUPED_MAX_GROUPS + 1];  // m-tiles before each group
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WNC, wn = wave % WNC, i16 = lane & 15, g = lane >> 4;
+    const int N = (int)p.N, K = (int)p.K;
+    const int ntn = (N + TN - 1) / TN;
+    const T* xp = static_cast<const T*>(p.x);
+    const T* wp = static_cast<const T*>(p.w);
+
+    // ---- tiles
+    int total;
+    if constexpr (WG) {
+        total = p.groups * (int)((p.M + BM - 1) / BM) * ntn;
+    } else {
+        if (p.offsets) {
+            // 4 groups a thread; a group's rows are cut to 0 .. rows, and none where its offsets descend
+            const int e0 = 4 * threadIdx.x;
+            int cnt[4], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                cnt[i] = 0;
+                if (e0 + i < p.groups) {
+                    const int lo = max(0, p.offsets[e0 + i]);
+                    const int hi = (int)min((int64_t)p.offsets[e0 + i + 1], p.rows);
+                    cnt[i] = hi > lo ? (hi - lo - 1) / BM + 1 : 0;
+                }
+                sum += cnt[i];
+            }
+            int incl = sum;
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) {
+                const int o = __shfl_up(incl, m, 64);
+                if (lane >= m) incl += o;
+            }
+            int* s_wave = reinterpret_cast<int*>(ring);
+            if (lane == 63) s_wave[wave] = incl;
+            __syncthreads();
+            int base = incl - sum;
+            for (int i = 0; i < wave; ++i) base += s_wave[i];
+            if (threadIdx.x == 0) s_pre[0] = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                base += cnt[i];
+                if (e0 + i < p.groups) s_pre[e0 + i + 1] = base;
+            }
+            __syncthreads();
+            total = s_pre[p.groups] * ntn;
+        } else {
+            total = (int)((p.rows + BM - 1) / BM) * ntn;
+        }
+    }
+    total = uni(total);
+    const int per = (total + kXcds - 1) / kXcds;
+    const int step = gridDim.x / kXcds;
+    const int jbeg = (blockIdx.x % kXcds) * per + blockIdx.x / kXcds;
+    const int jend = min((int)(blockIdx.x % kXcds + 1) * per, total);
+    if (jbeg >= jend) return;
+
+    // Tile j (the same in every lane).
+    auto tile_at = [&](int j) __attribute__((always_inline)) {
+        TileAt t;
+        int mt, jl = j;
+        if constexpr (WG) {
+            mt = (int)((p.M + BM - 1) / BM);
+            t.e = j / (mt * ntn);
+            jl = j - t.e * mt * ntn;
+            const int lo = max(0, p.offsets[t.e]);
+            const int hi = (int)min((int64_t)p.offsets[t.e + 1], p.rows);
+            t.k0 = uni(lo);
+            t.kn = uni(max(0, hi - lo));
+            t.nb = max(1, (t.kn + kBK - 1) / kBK);
+        } else if (p.offsets) {
+            const int m = j / ntn;
+            int e = 0;
+            for (int c = 0; c < p.groups; c += 64)
+                e += __popcll(__ballot(c + lane < p.groups && s_pre[min(c + lane, p.groups - 1) + 1] <= m));
+            t.e = min(uni(e), p.groups - 1);
+            mt = uni(s_pre[t.e + 1]) - uni(s_pre[t.e]);
+            jl = j - uni(s_pre[t.e]) * ntn;
+        } else {
+            t.e = 0;
+            mt = (int)((p.rows + BM - 1) / BM);
+        }
+        const int grp = jl / (kSuper * ntn), first = grp * kSuper;
+        const int gm = max(1, min(mt - first, kSuper)), r = jl - first * ntn;
+        const int m = first + r % gm;
+        t.n0 = r / gm * TN;
+        if constexpr (WG) {
+            t.row0 = m * BM;
+            t.nrows = min(BM, (int)p.M - t.row0);
+        } else {
+            const int lo = p.offsets ? uni(max(0, p.offsets[t.e])) : 0;
+            const int hi = p.offsets ? uni((int)min((int64_t)p.offsets[t.e + 1], p.rows)) : (int)p.rows;
+            t.row0 = lo + m * BM;
+            t.nrows = min(BM, hi - t.row0);
+            t.k0 = 0;
+            t.kn = K;
+            t.nb = (K + kBK - 1) / kBK;
+        }
+        t.row0 = uni(t.row0);
+        t.nrows = uni(t.nrows);
+        t.n0 = uni(t.n0);
+        return t;
+    };
+
+    // ---- the producer: the next stage that is loaded
+    TileAt pt;
+    int pj = jbeg, pks = 0;   // (its tile, its stage)
+    uint32_t voff[LPW];
+    const uint8_t *xbase, *wbase;
+    auto x_swz = [](int r) __attribute__((always_inline)) {
+        return XK ? (r >> 1) & 7 : ((r & 3) << 1) | (r & 8);
+    };
+    auto w_swz = [](int r) __attribute__((always_inline)) {
+        return WK ? ((r >> 1) & 1) | (((r >> 3) & 3) << 1) : (r & 1) | ((r & 2) << 1) | (r & 8);
+    };
+    // byte offset of the row of x that tile row r reads (from xbase)
+    auto x_off = [&](const TileAt& t, int r) __attribute__((always_inline)) -> uint32_t {
+        if (r >= t.nrows) return HM_BUF_RANGE;
+        int row = r;
+        if constexpr (GU) {
+            if (p.perm) {
+                row = p.perm[t.row0 + r];
+                if (row < 0 || row >= (int)p.x_rows) row = 0;
+            }
+        }
+        return (uint32_t)row * (uint32_t)K * 2;
+    };
+    // of the row of the group's matrix that row r of the staged w is (from wbase, the matrix's row n0)
+    auto w_off = [&](const TileAt& t, int r) __attribute__((always_inline)) -> uint32_t {
+        const bool up = GU && r >= TN;
+        const int n = up ? r - TN : r;
+        if (t.n0 + n >= N) return HM_BUF_RANGE;
+        return (uint32_t)(up ? N + n : n) * (uint32_t)K * 2;
+    };
+    // where the stage is the last of k: what lies past it counts as zeros in both operands
+    auto cut = [&]() __attribute__((always_inline)) {
+        const int left = uni(pt.kn - pks * kBK);
+        if (left >= kBK) return;
+        int l = lane;
+        asm volatile("" : "+v"(l));
+#pragma unroll
+        for (int c = 0; c < LPW; ++c) {
+            const bool isx = c < XL;
+            const int b = wave + NW * (isx ? c : c - XL);
+            int k;
+            if ((isx && XK) || (!isx && WK)) {
+                const int r = 8 * b + (l >> 3);
+                k = 8 * ((l & 7) ^ (isx ? x_swz(r) : w_swz(r)));
+            } else {
+                const int pcs = isx ? BM / 8 : BN / 8;
+                k = b * (64 / pcs) + l / pcs;
+            }
+            if (k >= left) voff[c] = HM_BUF_RANGE;
+        }
+    };
+    // ---- adapters: behind a tile's stages of k, for each adapter that its rows name (ascending) the stages of its
+    // rank: mid, with the rows of other adapters as zeros, and the adapter's matrix.  A lane knows the adapters of the
+    // tile's rows lane + 64 i.
+    constexpr int IDS = KIND == G_ADAPTER ? BM / 64 : 1;
+    int ids[IDS];
+    int low = -1;              // the adapter whose stages are loaded, -1: k's; INT_MAX: past the last tile
+    int lows = 0;              // its stage
+    auto read_ids = [&]() __attribute__((always_inline)) {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+#pragma unroll
+        for (int i = 0; i < IDS; ++i) {
+            const int r = 64 * i + l;
+            ids[i] = r < pt.nrows ? p.ids[pt.row0 + r] : -1;
+        }
+        low = -1;
+    };
+    auto next_low = [&]() __attribute__((always_inline)) {
+        if (low == INT_MAX) return false;
+        if (low >= 0 && (lows + 1) * kBK < p.rank) {
+            ++lows;
+            xbase += 2 * kBK;
+            wbase = uni(wbase + (WK ? 2 * kBK : 2 * (int64_t)kBK * N));
+        } else {
+            int v = INT_MAX;
+#pragma unroll
+            for (int i = 0; i < IDS; ++i) v = min(v, ids[i] > low && ids[i] < p.adapters ? ids[i] : INT_MAX);
+            v = wave_min(v);
+            if (v == INT_MAX) return false;
+            low = v;
+            lows = 0;
+            xbase = uni(static_cast<const uint8_t*>(p.mid) + (int64_t)pt.row0 * p.rank * 2);
+            wbase = uni(static_cast<const uint8_t*>(p.up) +
+                        2 * ((int64_t)low * N * p.rank + (WK ? (int64_t)pt.n0 * p.rank : (int64_t)pt.n0)));
+        }
+        const int left = p.rank - lows * kBK;
+        int l = lane;
+        asm volatile("" : "+v"(l));
+#pragma unroll
+        for (int c = 0; c < LPW; ++c) {
+            const bool isx = c < XL;
+            const int b = wave + NW * (isx ? c : c - XL);
+            if (isx || WK) {
+                const int r = 8 * b + (l >> 3), pc = (l & 7) ^ (isx ? x_swz(r) : w_swz(r));
+                const bool mine = isx ? __shfl(ids[NW * c / 8 % IDS], r & 63, 64) == low : pt.n0 + r < N;
+                voff[c] = mine && 8 * pc < left ? (uint32_t)r * (uint32_t)p.rank * 2 + 16 * pc : HM_BUF_RANGE;
+            } else {
+                const int r = b * (512 / BN) + l / (BN / 8), col = 8 * ((l % (BN / 8)) ^ w_swz(r));
+                voff[c] = r < left && pt.n0 + col < N ? (uint32_t)r * (uint32_t)N * 2 + 2 * (uint32_t)col : HM_BUF_RANGE;
+            }
+        }
+        pt.nb = 0;   // (each of these stages asks for the next one)
+        return true;
+    };
+    auto make_src = [&]() __attribute__((always_inline)) {
+        const TileAt& t = pt;
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        if constexpr (WG) {
+            xbase = uni(reinterpret_cast<const uint8_t*>(xp + (int64_t)t.k0 * p.M + t.row0));
+            wbase = uni(reinterpret_cast<const uint8_t*>(wp + (int64_t)t.k0 * N + t.n0));
+        } else {
+            xbase = uni(reinterpret_cast<const uint8_t*>(xp + (GU && p.perm ? 0 : (int64_t)t.row0 * K)));
+            wbase = uni(reinterpret_cast<const uint8_t*>(wp + (int64_t)t.e * p.w_group +
+                                                         (WK ? (int64_t)t.n0 * K : (int64_t)t.n0)));
+        }
+#pragma unroll
+        for (int c = 0; c < LPW; ++c) {
+            const bool isx = c < XL;
+            const int b = wave + NW * (isx ? c : c - XL);
+            if ((isx && XK) || (!isx && WK)) {
+                const int r = 8 * b + (l >> 3);
+                const uint32_t row = isx ? x_off(t, r) : w_off(t, r);
+                voff[c] = row + 16 * ((l & 7) ^ (isx ? x_swz(r) : w_swz(r)));
+            } else {
+                const int pcs = isx ? BM / 8 : BN / 8;   // pieces a row
+                const int ld = isx ? (int)p.M : N;
+                const int r = b * (64 / pcs) + l / pcs;
+                const int col = 8 * ((l % pcs) ^ (isx ? x_swz(r) : w_swz(r)));
+                voff[c] = (isx ? t.row0 : t.n0) + col < ld ? (uint32_t)r * (uint32_t)ld * 2 + 2 * (uint32_t)col
+                                                          : HM_BUF_RANGE;
+            }
+        }
+        cut();
+        if constexpr (KIND == G_ADAPTER) read_ids();
+    };
+    // bytes from one stage's values to the next one's
+    const int64_t xstep = XK ? 2 * kBK : 2 * (int64_t)kBK * p.M;
+    const int64_t wstep = WK ? 2 * kBK : 2 * (int64_t)kBK * N;
+    // load c of the producer's stage into a slot
+    hm_buf xbuf, wbuf;
+    auto issue = [&](int slot, int c) __attribute__((always_inline)) {
+        const bool isx = c < XL;
+        const int b = wave + NW * (isx ? c : c - XL);
+        dma16_buf(isx ? xbuf : wbuf, voff[c], ring + slot * STAGE + (isx ? 0 : WOFF) + 1024 * b);
+    };
+    // The descriptors of the producer's stage, ahead of its loads: a scalar register that the vector unit wrote may
+    // be read by a memory instruction five wait states later, and the compiler does not look into theirs.
+    auto describe = [&]() __attribute__((always_inline)) {
+        xbuf = make_buf(xbase);
+        wbuf = make_buf(wbase);
+        asm volatile("s_nop 4" : "+s"(xbuf), "+s"(wbuf));
+    };
+    uint32_t last = 0;         // bit s: the stage in slot s is its tile's last
+    // to the stage after the one that went to `slot`
+    auto advance = [&](int slot) __attribute__((always_inline)) {
+        last &= ~(1u << slot);
+        // (readfirstlane: the compiler does not see by itself that these are the same in every lane)
+        pks = uni(pks + 1);
+        if (pks < uni(pt.nb)) {
+            xbase = uni(xbase + xstep);
+            wbase = uni(wbase + wstep);
+            cut();
+            return;
+        }
+        if constexpr (KIND == G_ADAPTER) {
+            if (next_low()) return;
+        }
+        last |= 1u << slot;
+        pks = 0;
+        if (uni(pj) + step < jend) {
+            pj += step;
+            pt = tile_at(pj);
+            make_src();
+        } else {   // past the last tile: stages of nothing, so that loads and waits have no conditions
+            pt.nb = INT_MAX;
+            pt.kn = INT_MAX;
+            low = INT_MAX;
+#pragma unroll
+            for (int c = 0; c < LPW; ++c) voff[c] = HM_BUF_RANGE;
+        }
+    };
+
+    // ---- fragments
+    // k-major: one 16-byte read; otherwise two transposing reads of 8 bytes, in which lane i16 gives the place of 4
+    // values of row i16 / 4 and gets the values of column i16
+    int xrd, wrd[WK ? 1 : WF];
+    const int trow = 8 * g + (i16 >> 2), tc = i16 & 3;
+    if constexpr (XK) xrd = (wm * 16 * XF + i16) * 128 + 16 * (g ^ x_swz(i16));
+    else xrd = trow * 2 * BM + 16 * ((wm * 2 * XF + (tc >> 1)) ^ x_swz(trow)) + 8 * (tc & 1);
+    if constexpr (WK) {
+        const int r = 8 * (i16 >> 2) + (i16 & 3);
+        wrd[0] = WOFF + (wn * 16 * SH + r) * 128 + 16 * (g ^ w_swz(r));
+    } else {
+        const int at = WOFF + trow * 2 * BN + 16 * ((wn * 2 * WF + tc) ^ w_swz(trow)) + 8 * (tc & 1);
+#pragma unroll
+        for (int j = 0; j < WF; ++j) wrd[j] = at ^ (64 * (j >> 1)) ^ (8 * (j & 1));
+    }
+    auto read_x = [&](const uint8_t* st, int h, int i) __attribute__((always_inline)) {
+        if constexpr (XK) {
+            return *reinterpret_cast<const v8*>(st + (xrd ^ (64 * h)) + i * 16 * 128);
+        } else {
+            const uint8_t* at = st + (xrd ^ (32 * i)) + 32 * h * 2 * BM;
+            return read_transposed<v8>(at, 4 * 2 * BM);
+        }
+    };
+    auto read_w = [&](const uint8_t* st, int h, int j) __attribute__((always_inline)) {
+        if constexpr (WK) {
+            return *reinterpret_cast<const v8*>(st + (wrd[0] ^ (64 * h)) +
+                                                ((j / SH) * TN + 32 * ((j % SH) >> 1) + 4 * (j & 1)) * 128);
+        } else {
+            const uint8_t* at = st + wrd[j] + 32 * h * 2 * BN;
+            return read_transposed<v8>(at, 4 * 2 * BN);
+        }
+    };
+
+    v4f acc[XF][WF];
+    struct Frags {
+        v8 x[XF], w[WF];
+    };
+    // One step: the products of `f`, and among them the reads of the next step's fragments (half h of the stage at
+    // st) and, if LOAD, the loads of the producer's stage.
+    constexpr int NT = XF * WF, NR = XF + WF;
+    constexpr int RS = std::max(1, NT * 3 / 4 / NR), DS = std::max(1, NT / 2 / LPW);
+    auto mma = [&](const Frags& f, Frags& n, const uint8_t* st, int h, bool load, int slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int i = t / WF, j = t % WF;
+            acc[i][j] = Elem16<T>::mfma(f.w[j], f.x[i], acc[i][j]);
+            if (t % RS == 0 && t / RS < NR) {
+                // x 0, all of w, the rest of x: the order of their use
+                const int q = t / RS;
+                if (q == 0) n.x[0] = read_x(st, h, 0);
+                else if (q <= WF) n.w[q - 1] = read_w(st, h, q - 1);
+                else n.x[q - WF] = read_x(st, h, q - WF);
+            }
+            if (load && t % DS == 0 && t / DS < LPW) issue(slot, t / DS);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    // ---- results
+    // (lanes are taken anew, or the compiler keeps every address of it through the main loop and spills)
+    auto finish = [&](const TileAt& t) __attribute__((always_inline)) {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        const int gg = l >> 4;
+        const bool odd = !WK && (gg & 1);   // transposed reads: the two fragments of 8 columns in the other order
+        const int c0 = t.n0 + wn * 16 * SH + 8 * gg;
+#pragma unroll
+        for (int i = 0; i < XF; ++i) {
+            const int r = wm * 16 * XF + 16 * i + (l & 15);
+            if (r >= t.nrows) continue;
+            const int64_t row = t.row0 + r;
+#pragma unroll
+            for (int q = 0; q < SH; q += 2) {
+                const int c = c0 + 16 * q, n = N - c;
+                if (n <= 0) continue;
+                float a[8], b[8], d[8];
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    a[v] = odd ? acc[i][q + 1][v] : acc[i][q][v];
+                    a[4 + v] = odd ? acc[i][q][v] : acc[i][q + 1][v];
+                }
+                if constexpr (GU) {
+#pragma unroll
+                    for (int v = 0; v < 8; ++v) {
+                        b[v] = acc[i][SH + q + v / 4][v % 4];
+                        d[v] = fast_silu(a[v]) * b[v];
+                    }
+                    store8(static_cast<T*>(p.y) + row * N + c, n, d);
+                    if (p.pre_out) {
+                        T* pre = static_cast<T*>(p.pre_out) + row * 2 * N + c;
+                        store8(pre, n, a);
+                        store8(pre + N, n, b);
+                    }
+                } else if constexpr (KIND == G_SWIGLU_GRAD) {
+                    const T* pre = static_cast<const T*>(p.pre_in) + row * 2 * N + c;
+                    load8(pre, n, b);
+                    load8(pre + N, n, d);
+                    float z[8];
+#pragma unroll
+                    for (int v = 0; v < 8; ++v) swiglu_grad(a[v], b[v], d[v], &a[v], &d[v], &z[v]);
+                    T* to = static_cast<T*>(p.y) + row * 2 * N + c;
+                    store8(to, n, a);
+                    store8(to + N, n, d);
+                    if (p.z) store8(static_cast<T*>(p.z) + row * N + c, n, z);
+                } else if constexpr (WG) {
+                    O* y = static_cast<O*>(p.y) + ((int64_t)t.e * p.M + row) * N + c;
+                    if (p.accumulate) {
+                        load8(y, n, b);
+#pragma unroll
+                        for (int v = 0; v < 8; ++v) a[v] += b[v];
+                    }
+                    store8(y, n, a);
+                } else {
+                    store8(static_cast<O*>(p.y) + row * N + c, n, a);
+                }
+            }
+        }
+    };
+    // memory instructions that finish() issues at least for a tile whose rows and columns of this wave are whole
+    constexpr int STORES = XF * (GU ? SH / 2 : KIND == G_SWIGLU_GRAD ? 4 * SH / 2 : (int)sizeof(O) / 2 * SH / 2);
+    auto whole = [&](const TileAt& t) __attribute__((always_inline)) {
+        return t.nrows >= (wm + 1) * 16 * XF && t.n0 + TN <= N;
+    };
+    auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < XF; ++i)
+#pragma unroll
+            for (int j = 0; j < WF; ++j) acc[i][j] = v4f{};
+    };
+
+    // ---- the stream
+    TileAt cur = tile_at(jbeg);
+    int cj = jbeg, slot = 0;
+    bool stored = false;
+    pt = cur;
+    make_src();
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+        describe();
+#pragma unroll
+        for (int c = 0; c < LPW; ++c) issue(s, c);
+        advance(s);
+    }
+    clear();
+    Frags fa, fb;
+    wait_vmcnt<(NS - 1) * LPW>();
+    lds_barrier();
+    fa.x[0] = read_x(ring, 0, 0);
+#pragma unroll
+    for (int j = 0; j < WF; ++j) fa.w[j] = read_w(ring, 0, j);
+#pragma unroll
+    for (int i = 1; i < XF; ++i) fa.x[i] = read_x(ring, 0, i);
+    while (true) {
+        describe();
+        mma(fa, fb, ring + slot * STAGE, 1, false, 0);
+        // this wave's loads of the next stage have landed, then every wave's; and every wave has read this stage
+        // (after a whole tile's stores, which are younger, they may be in flight too)
+        if (stored) wait_vmcnt<std::min(60, (NS - 2) * LPW + STORES)>();
+        else wait_vmcnt<(NS - 2) * LPW>();
+        stored = false;
+        lds_barrier();
+        const int next = slot == NS - 1 ? 0 : slot + 1;
+        mma(fb, fa, ring + next * STAGE, 0, true, slot);
+        const bool done = uni((int)(last >> slot)) & 1;
+        advance(slot);
+        slot = next;
+        if (!done) continue;
+        finish(cur);
+        stored = whole(cur);
+        cj += step;
+        if (cj >= jend) break;
+        cur = tile_at(cj);
+        clear();
+    }
+    wait_vmcnt<0>();  // the LDS is not given back under a load
+}
+
+int cu_count() {
+    static int cached[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) dev = 0;
+    if (cached[dev] == 0) {
+        int cus = 0;
+        if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < kXcds)
+            cus = 256;
+        cached[dev] = cus;
+    }
+    return cached[dev];
+}
+
+// per_cu workgroups share a CU (their LDS)
+template <int WMC, int WNC, int XF, int WF, int NS, GKind KIND, bool WK, typename T, typename O>
+int launch(const GProduct& p, hipStream_t s) {
+    constexpr int BM = 16 * XF * WMC, BN = 16 * WF * WNC, TN = KIND == G_SWIGLU ? BN / 2 : BN;
+    const int64_t n = (p.N + TN - 1) / TN;
+    const int64_t m = KIND == G_WEIGHT_GRAD ? p.groups * ((p.M + BM - 1) / BM)
+                      : p.offsets           ? p.rows / BM + std::min((int64_t)p.groups, p.rows)
+                                            : (p.rows + BM - 1) / BM;
+    if (m * n > INT_MAX / 2) return HM_ERR_OVERFLOW;
+    const int64_t slots = (int64_t)cu_count() / kXcds * (NS * 128 * (BM + BN) > 76 * 1024 ? 1 : 2);
+    const int64_t grid = kXcds * std::min((m * n + kXcds - 1) / kXcds, slots);
+    hipLaunchKernelGGL((g_tile_kernel<WMC, WNC, XF, WF, NS, KIND, WK, T, O>), dim3((unsigned)grid),
+                       dim3(64 * WMC * WNC), 0, s, p);
+    HM_LAUNCHED();
+    return HM_OK;
+}
+
+template <int WMC, int WNC, int XF, int WF, int NS, typename T>
+int launch_kind(GKind kind, bool wk, bool f32, const GProduct& p, hipStream_t s) {
+#define HM_G(KIND, WK, O) launch<WMC, WNC, XF, WF, NS, KIND, WK, T, O>(p, s)
+    switch (kind) {
+    case G_SWIGLU: return HM_G(G_SWIGLU, true, T);
+    case G_SWIGLU_GRAD: return HM_G(G_SWIGLU_GRAD, false, T);
+    case G_WEIGHT_GRAD: return f32 ? HM_G(G_WEIGHT_GRAD, false, float) : HM_G(G_WEIGHT_GRAD, false, T);
+    case G_ADAPTER: return wk ? HM_G(G_ADAPTER, true, T) : HM_G(G_ADAPTER, false, T);
+    default: break;
+    }
+    if (wk) return f32 ? HM_G(G_MATMUL, true, float) : HM_G(G_MATMUL, true, T);
+    return f32 ? HM_G(G_MATMUL, false, float) : HM_G(G_MATMUL, false, T);
+#undef HM_G
+}
+
+template <typename T>
+int launch_tiles(int form, GKind kind, bool wk, bool f32, const GProduct& p, hipStream_t s) {
+    if (form == 256) return launch_kind<2, 4, 8, 4, 2, T>(kind, wk, f32, p, s);
+    if (form == 128) return launch_kind<2, 4, 4, 4, 3, T>(kind, wk, f32, p, s);
+    return launch_kind<2, 2, 4, 4, 2, T>(kind, wk, f32, p, s);
+}
+
+}  // namespace

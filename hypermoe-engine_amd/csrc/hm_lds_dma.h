@@ -72,4 +72,18 @@ __device__ __forceinline__ void dma4_off(const void* base, uint32_t off, void* l
     asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1"
                  :: "v"(off), "s"(base), "s"(m0) : "memory", "m0");
 }
+// dma16 through a buffer descriptor: the same, and a lane whose offset is at or past HM_BUF_RANGE reads
+// nothing and leaves zeros in its place of the LDS.
+#define HM_BUF_RANGE 0xf0000000u
+typedef int hm_buf __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ hm_buf make_buf(const void* base) {
+    const uint64_t a = reinterpret_cast<uint64_t>(base);
+    return hm_buf{__builtin_amdgcn_readfirstlane((int)(uint32_t)a), __builtin_amdgcn_readfirstlane((int)(a >> 32)),
+                  (int)HM_BUF_RANGE, 0x00020000};
+}
+__device__ __forceinline__ void dma16_buf(hm_buf buf, uint32_t off, void* lds_base) {
+    const unsigned m0 = (unsigned)(uintptr_t)(lds_ptr_t)lds_base;
+    asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                 :: "v"(off), "s"(buf), "s"(m0) : "memory", "m0");
+}
 #pragma clang diagnostic pop
