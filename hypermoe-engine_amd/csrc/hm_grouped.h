@@ -108,17 +108,24 @@ __device__ __forceinline__ void store8(T* p, int n, const float (&f)[8]) {
     }
 }
 
+// 16 bytes from a place aligned to 2.
+typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u64x2 load16(const void* p) {
+    typedef uint64_t loose __attribute__((ext_vector_type(2), aligned(2)));
+    return *(const __attribute__((address_space(1))) loose*)p;   // (never the LDS: no flat load)
+}
+
 // n values (8 at most) of a row as a fragment's 8, zeros behind them.
 template <typename T>
 __device__ __forceinline__ typename Elem16<T>::v8 load_frag8(const T* p, int64_t n) {
     typedef typename Elem16<T>::v8 v8;
-    Loose8<T> w;
-    if (n >= 8) {
-        w = *reinterpret_cast<const Loose8<T>*>(p);
-    } else {
+    typedef short v8s __attribute__((ext_vector_type(8)));
+    typedef const __attribute__((address_space(1))) short* global_t;
+    if (n >= 8) return __builtin_bit_cast(v8, load16(p));
+    v8s w = {};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w.v[i] = i < n ? p[i] : (T)0.0f;
-    }
+    for (int i = 0; i < 8; ++i)
+        if (i < n) w[i] = ((global_t)p)[i];
     return __builtin_bit_cast(v8, w);
 }
 
@@ -150,8 +157,8 @@ static inline bool hm_overlap(const void* a, int64_t na, const void* b, int64_t 
 }
 
 int hm_g_launch_generic(GKind kind, bool w_kmajor, int32_t dtype, int32_t y_dtype, const GProduct& p, hipStream_t s);
-// The tile kernels (hm_grouped_tile.h) for operands aligned to 16 bytes throughout.  form 256: tiles of 256 x 256
-// results, 128: of 128 x 256, 64: of 128 x 128.
+// The tile kernels (hm_grouped_tile.h).  form 256: tiles of 256 x 256 results, 128: of 128 x 256, 64: of 128 x 128,
+// these three for operands aligned to 16 bytes throughout; 32: of 128 x 128 for others.
 int hm_g_launch_tiles_f16(GKind kind, int form, bool w_kmajor, bool f32, const GProduct& p, hipStream_t s);
 int hm_g_launch_tiles_bf16(GKind kind, int form, bool w_kmajor, bool f32, const GProduct& p, hipStream_t s);
 // The kernel for few rows (hm_grouped_stream.hip): x w^T, SwiGLU or adapters, 16 mt rows a workgroup (1, 2, 4; 8 but

@@ -285,24 +285,32 @@ int hm_g_launch_generic(GKind kind, bool w_kmajor, int32_t dtype, int32_t y_dtyp
                                   : launch_kind<hm_bf16>(kind, w_kmajor, f32, p, s);
 }
 
-// Whether a product fits the tile kernels: everything that they move in 16 bytes is aligned to that, and offsets
-// from a tile's first row (x's first row where rows are gathered) stay below HM_BUF_RANGE.
-static bool tile_ok(GKind kind, bool w_kmajor, const GProduct& p) {
+// Whether a product fits the tile kernels: offsets from a tile's first row (x's first row where rows are gathered)
+// stay below HM_BUF_RANGE.
+static bool tile_ok(GKind kind, const GProduct& p) {
     const int64_t top = HM_BUF_RANGE;
-    if (!aligned(p.x, 16) || !aligned(p.w, 16) || p.rows > INT_MAX - 256) return false;
-    if (kind == G_WEIGHT_GRAD) return p.M % 8 == 0 && p.N % 8 == 0;
-    if (p.K % 8 || (!w_kmajor && p.N % 8) || p.K > (int64_t)1 << 22) return false;
-    if (kind == G_ADAPTER) return p.rank % 8 == 0 && aligned(p.mid, 16) && aligned(p.up, 16);
+    if (p.rows > INT_MAX - 256) return false;
+    if (kind == G_WEIGHT_GRAD) return true;
+    if (p.K > (int64_t)1 << 22) return false;
     return kind != G_SWIGLU || ((p.N + 256) * p.K * 2 < top && (!p.perm || p.x_rows * p.K * 2 < top));
 }
 
-// Which kernel: rows << 16 of a stream workgroup, the form of a tile, 0 for operands off 16 bytes.
+// Whether everything that a tile moves in 16 bytes is aligned to that.
+static bool dma_ok(GKind kind, bool w_kmajor, const GProduct& p) {
+    if (!aligned(p.x, 16) || !aligned(p.w, 16)) return false;
+    if (kind == G_WEIGHT_GRAD) return p.M % 8 == 0 && p.N % 8 == 0;
+    if (p.K % 8 || (!w_kmajor && p.N % 8)) return false;
+    return kind != G_ADAPTER || (p.rank % 8 == 0 && aligned(p.mid, 16) && aligned(p.up, 16));
+}
+
+// Which kernel: rows << 16 of a stream workgroup, the form of a tile, 0: the generic kernel.
 static int pick(GKind kind, bool w_kmajor, const GProduct& p) {
     const bool nt = w_kmajor && kind != G_WEIGHT_GRAD;
     const int64_t groups = p.offsets ? p.groups : 1, each = (p.rows + groups - 1) / groups;
     if (nt && (each <= 16 || p.rows <= 64)) return (p.rows <= 16 || each <= 4 ? 1 : p.rows <= 32 || each <= 8 ? 2 : 4) << 16;
     if (kind == G_ADAPTER && nt && p.rows <= 128) return 8 << 16;
-    if (!tile_ok(kind, w_kmajor, p)) return 0;
+    if (!tile_ok(kind, p)) return 0;
+    if (!dma_ok(kind, w_kmajor, p)) return 32;
     const int64_t tm = kind == G_WEIGHT_GRAD ? p.groups * ((p.M + 127) / 128) : p.rows / 128 + groups;
     if (tm * ((p.N + 255) / 256) < 256) return 64;
     if (kind == G_WEIGHT_GRAD || each >= 384) return 256;

@@ -25,6 +25,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -48,17 +49,21 @@ struct TileAt {
     int nb;             // stages of k
 };
 
-template <int WMC, int WNC, int XF, int WF, int NS, GKind KIND, bool WK, typename T, typename O>
+template <int WMC, int WNC, int XF, int WF, int NS, bool DMA, GKind KIND, bool WK, typename T, typename O>
 __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     typedef typename Elem16<T>::v8 v8;
     constexpr bool WG = KIND == G_WEIGHT_GRAD, XK = !WG, GU = KIND == G_SWIGLU;
     constexpr int NW = WMC * WNC, BM = 16 * XF * WMC, BN = 16 * WF * WNC, SH = GU ? WF / 2 : WF, TN = GU ? BN / 2 : BN;
     constexpr int STAGE = 128 * (BM + BN), WOFF = 128 * BM;
     constexpr int XL = BM / 8 / NW, LPW = (BM + BN) / 8 / NW;   // a wave's 1 KB loads a stage, of x first
+    static_assert(DMA || NW == 4, "fetch() takes the swizzles to be the same for every c");
     static_assert(XF % 2 == 0 && (SH == 2 || SH == 4 || SH == 8) && BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "tile");
     __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * STAGE];
     __shared__ int s_pre[WG ? 1 : HM_GROUPED_MAX_GROUPS + 1];  // m-tiles before each group
 
+    // (the barriers are hand-written: without this the compiler may take the ring, whose address would leave the
+    // function nowhere where there is no DMA, to be out of their reach)
+    asm volatile("" : : "s"((unsigned)(uintptr_t)(lds_ptr_t)ring) : "memory");
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WNC, wn = wave % WNC, i16 = lane & 15, g = lane >> 4;
@@ -168,6 +173,8 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     int pj = jbeg, pks = 0;   // (its tile, its stage)
     uint32_t voff[LPW];
     const uint8_t *xbase, *wbase;
+    int left = 0;              // k from the stage's first on
+    int xcols = 0, wcols = 0;  // without DMA, operands that are not k-major: columns from this lane's on
     auto x_swz = [](int r) __attribute__((always_inline)) {
         return XK ? (r >> 1) & 7 : ((r & 3) << 1) | (r & 8);
     };
@@ -195,8 +202,8 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     };
     // where the stage is the last of k: what lies past it counts as zeros in both operands
     auto cut = [&]() __attribute__((always_inline)) {
-        const int left = uni(pt.kn - pks * kBK);
-        if (left >= kBK) return;
+        left = uni(pt.kn - pks * kBK);
+        if (left >= kBK || (!DMA && XK && WK)) return;
         int l = lane;
         asm volatile("" : "+v"(l));
 #pragma unroll
@@ -205,6 +212,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
             const int b = wave + NW * (isx ? c : c - XL);
             int k;
             if ((isx && XK) || (!isx && WK)) {
+                if (!DMA) continue;   // (these count what is left of a piece)
                 const int r = 8 * b + (l >> 3);
                 k = 8 * ((l & 7) ^ (isx ? x_swz(r) : w_swz(r)));
             } else {
@@ -249,7 +257,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
             wbase = uni(static_cast<const uint8_t*>(p.up) +
                         2 * ((int64_t)low * N * p.rank + (WK ? (int64_t)pt.n0 * p.rank : (int64_t)pt.n0)));
         }
-        const int left = p.rank - lows * kBK;
+        left = uni(p.rank - lows * kBK);
         int l = lane;
         asm volatile("" : "+v"(l));
 #pragma unroll
@@ -259,7 +267,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
             if (isx || WK) {
                 const int r = 8 * b + (l >> 3), pc = (l & 7) ^ (isx ? x_swz(r) : w_swz(r));
                 const bool mine = isx ? __shfl(ids[NW * c / 8 % IDS], r & 63, 64) == low : pt.n0 + r < N;
-                voff[c] = mine && 8 * pc < left ? (uint32_t)r * (uint32_t)p.rank * 2 + 16 * pc : HM_BUF_RANGE;
+                voff[c] = mine && (!DMA || 8 * pc < left) ? (uint32_t)r * (uint32_t)p.rank * 2 + 16 * pc : HM_BUF_RANGE;
             } else {
                 const int r = b * (512 / BN) + l / (BN / 8), col = 8 * ((l % (BN / 8)) ^ w_swz(r));
                 voff[c] = r < left && pt.n0 + col < N ? (uint32_t)r * (uint32_t)N * 2 + 2 * (uint32_t)col : HM_BUF_RANGE;
@@ -293,6 +301,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
                 const int ld = isx ? (int)p.M : N;
                 const int r = b * (64 / pcs) + l / pcs;
                 const int col = 8 * ((l % pcs) ^ (isx ? x_swz(r) : w_swz(r)));
+                (isx ? xcols : wcols) = ld - (isx ? t.row0 : t.n0) - col;   // (the same for every c)
                 voff[c] = (isx ? t.row0 : t.n0) + col < ld ? (uint32_t)r * (uint32_t)ld * 2 + 2 * (uint32_t)col
                                                           : HM_BUF_RANGE;
             }
@@ -305,14 +314,64 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     const int64_t wstep = WK ? 2 * kBK : 2 * (int64_t)kBK * N;
     // load c of the producer's stage into a slot
     hm_buf xbuf, wbuf;
+    v8 regs[DMA ? 1 : LPW];
     auto issue = [&](int slot, int c) __attribute__((always_inline)) {
         const bool isx = c < XL;
         const int b = wave + NW * (isx ? c : c - XL);
-        dma16_buf(isx ? xbuf : wbuf, voff[c], ring + slot * STAGE + (isx ? 0 : WOFF) + 1024 * b);
+        uint8_t* to = ring + slot * STAGE + (isx ? 0 : WOFF) + 1024 * b;
+        if constexpr (DMA) dma16_buf(isx ? xbuf : wbuf, voff[c], to);
+        else *reinterpret_cast<v8*>(to + 16 * lane) = regs[c];
+    };
+    // Without DMA (operands off 16 bytes): the stage goes through registers, loaded one step ahead of the write.  A
+    // piece that ends past its row's last value is loaded so far before that it ends there, and shifted.
+    auto fetch = [&]() __attribute__((always_inline)) {
+        if (left <= 0 || low == INT_MAX) {
+#pragma unroll
+            for (int c = 0; c < LPW; ++c) regs[c] = v8{};
+            return;
+        }
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        // values of a row, and from the stage's first piece on; whether every piece is whole
+        const int xrow = XK ? (low >= 0 ? p.rank : K) : (int)p.M, wrow = WK ? (low >= 0 ? p.rank : K) : N;
+        const int xleft = XK ? left : (int)p.M - pt.row0, wleft = WK ? left : N - pt.n0;
+        const bool whole = xleft >= (XK ? kBK : BM) && wleft >= (WK ? kBK : BN);
+        auto load = [&](auto kind) __attribute__((always_inline)) {
+#pragma unroll
+            for (int c = 0; c < LPW; ++c) {
+                const bool isx = c < XL;
+                const int r = 8 * (wave + NW * (isx ? c : c - XL)) + (l >> 3);
+                const uint8_t* base = isx ? xbase : wbase;
+                const bool in = voff[c] < HM_BUF_RANGE;
+                int n = (isx && XK) || (!isx && WK) ? left - 8 * ((l & 7) ^ (isx ? x_swz(r) : w_swz(r)))
+                        : isx                       ? xcols
+                                                    : wcols;
+                if constexpr (decltype(kind)::value == 2) {   // rows of fewer than 8 values
+                    regs[c] = load_frag8<T>(reinterpret_cast<const T*>(base + voff[c]), in ? n : 0);
+                    continue;
+                }
+                const bool some = in && n > 0;
+                uint32_t off = some ? voff[c] : 0;
+                u64x2 v;
+                if constexpr (decltype(kind)::value == 0) {
+                    v = load16(base + off);
+                } else {
+                    const uint32_t back = 16 * (8 - min(8, some ? n : isx ? xleft : wleft));   // bits
+                    v = load16(base + (int64_t)off - back / 8);
+                    if (back >= 64) v = u64x2{v[1] >> (back & 63), 0};
+                    else if (back) v = u64x2{v[0] >> back | v[1] << (64 - back), v[1] >> back};
+                }
+                regs[c] = __builtin_bit_cast(v8, some ? v : u64x2{});
+            }
+        };
+        if (xrow < 8 || wrow < 8) load(std::integral_constant<int, 2>{});
+        else if (whole) load(std::integral_constant<int, 0>{});
+        else load(std::integral_constant<int, 1>{});
     };
     // The descriptors of the producer's stage, ahead of its loads: a scalar register that the vector unit wrote may
     // be read by a memory instruction five wait states later, and the compiler does not look into theirs.
     auto describe = [&]() __attribute__((always_inline)) {
+        if constexpr (!DMA) return;
         xbuf = make_buf(xbase);
         wbuf = make_buf(wbase);
         asm volatile("s_nop 4" : "+s"(xbuf), "+s"(wbuf));
@@ -485,14 +544,16 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     make_src();
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-        describe();
+        if constexpr (DMA) describe();
+        else fetch();
 #pragma unroll
         for (int c = 0; c < LPW; ++c) issue(s, c);
         advance(s);
     }
     clear();
     Frags fa, fb;
-    wait_vmcnt<(NS - 1) * LPW>();
+    if constexpr (DMA) wait_vmcnt<(NS - 1) * LPW>();
+    else fetch();
     lds_barrier();
     fa.x[0] = read_x(ring, 0, 0);
 #pragma unroll
@@ -504,14 +565,17 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
         mma(fa, fb, ring + slot * STAGE, 1, false, 0);
         // this wave's loads of the next stage have landed, then every wave's; and every wave has read this stage
         // (after a whole tile's stores, which are younger, they may be in flight too)
-        if (stored) wait_vmcnt<std::min(60, (NS - 2) * LPW + STORES)>();
-        else wait_vmcnt<(NS - 2) * LPW>();
-        stored = false;
+        if constexpr (DMA) {
+            if (stored) wait_vmcnt<std::min(60, (NS - 2) * LPW + STORES)>();
+            else wait_vmcnt<(NS - 2) * LPW>();
+            stored = false;
+        }
         lds_barrier();
         const int next = slot == NS - 1 ? 0 : slot + 1;
         mma(fb, fa, ring + next * STAGE, 0, true, slot);
         const bool done = uni((int)(last >> slot)) & 1;
         advance(slot);
+        if constexpr (!DMA) fetch();
         slot = next;
         if (!done) continue;
         finish(cur);
@@ -538,7 +602,7 @@ int cu_count() {
 }
 
 // per_cu workgroups share a CU (their LDS)
-template <int WMC, int WNC, int XF, int WF, int NS, GKind KIND, bool WK, typename T, typename O>
+template <int WMC, int WNC, int XF, int WF, int NS, bool DMA, GKind KIND, bool WK, typename T, typename O>
 int launch(const GProduct& p, hipStream_t s) {
     constexpr int BM = 16 * XF * WMC, BN = 16 * WF * WNC, TN = KIND == G_SWIGLU ? BN / 2 : BN;
     const int64_t n = (p.N + TN - 1) / TN;
@@ -548,15 +612,15 @@ int launch(const GProduct& p, hipStream_t s) {
     if (m * n > INT_MAX / 2) return HM_ERR_OVERFLOW;
     const int64_t slots = (int64_t)cu_count() / kXcds * (NS * 128 * (BM + BN) > 76 * 1024 ? 1 : 2);
     const int64_t grid = kXcds * std::min((m * n + kXcds - 1) / kXcds, slots);
-    hipLaunchKernelGGL((g_tile_kernel<WMC, WNC, XF, WF, NS, KIND, WK, T, O>), dim3((unsigned)grid),
+    hipLaunchKernelGGL((g_tile_kernel<WMC, WNC, XF, WF, NS, DMA, KIND, WK, T, O>), dim3((unsigned)grid),
                        dim3(64 * WMC * WNC), 0, s, p);
     HM_LAUNCHED();
     return HM_OK;
 }
 
-template <int WMC, int WNC, int XF, int WF, int NS, typename T>
+template <int WMC, int WNC, int XF, int WF, int NS, bool DMA, typename T>
 int launch_kind(GKind kind, bool wk, bool f32, const GProduct& p, hipStream_t s) {
-#define HM_G(KIND, WK, O) launch<WMC, WNC, XF, WF, NS, KIND, WK, T, O>(p, s)
+#define HM_G(KIND, WK, O) launch<WMC, WNC, XF, WF, NS, DMA, KIND, WK, T, O>(p, s)
     switch (kind) {
     case G_SWIGLU: return HM_G(G_SWIGLU, true, T);
     case G_SWIGLU_GRAD: return HM_G(G_SWIGLU_GRAD, false, T);
@@ -571,9 +635,10 @@ int launch_kind(GKind kind, bool wk, bool f32, const GProduct& p, hipStream_t s)
 
 template <typename T>
 int launch_tiles(int form, GKind kind, bool wk, bool f32, const GProduct& p, hipStream_t s) {
-    if (form == 256) return launch_kind<2, 4, 8, 4, 2, T>(kind, wk, f32, p, s);
-    if (form == 128) return launch_kind<2, 4, 4, 4, 3, T>(kind, wk, f32, p, s);
-    return launch_kind<2, 2, 4, 4, 2, T>(kind, wk, f32, p, s);
+    if (form == 256) return launch_kind<2, 4, 8, 4, 2, true, T>(kind, wk, f32, p, s);
+    if (form == 128) return launch_kind<2, 4, 4, 4, 3, true, T>(kind, wk, f32, p, s);
+    if (form == 64) return launch_kind<2, 2, 4, 4, 2, true, T>(kind, wk, f32, p, s);
+    return launch_kind<2, 2, 4, 4, 2, false, T>(kind, wk, f32, p, s);
 }
 
 }  // namespace
