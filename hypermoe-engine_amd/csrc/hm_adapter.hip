@@ -62,26 +62,36 @@ __global__ __launch_bounds__(kThreads) void adapter_mid_rows_kernel(const T* __r
     }
 }
 
-// More rows: a workgroup takes 16 rows and 16 RF ranks, its 8 waves k in parts of 64, straight from memory into
-// fragments (x is read once; the adapters' matrices stay in the L2); once for each adapter that the rows name, its
-// own rows kept.  The waves' sums meet in the LDS in wave order.
+// More rows: a workgroup takes 16 MT rows and 16 RF ranks, its 8 waves k in parts of 64, straight from memory into
+// fragments (x is read once; the adapters' matrices, read by every workgroup, stay in the L2 and bound it); once for
+// each adapter that the rows name, its own rows kept.  The waves' sums meet in the LDS in wave order.
+constexpr int kMidWaves = 8;
+
 template <typename T, bool KM, int RF>
-__global__ __launch_bounds__(512) void adapter_mid_tile_kernel(const T* __restrict__ x, const T* __restrict__ down,
-                                                               const float* __restrict__ scale,
-                                                               const int32_t* __restrict__ ids, int adapters,
-                                                               int rank, int64_t rows, int64_t K,
-                                                               T* __restrict__ mid) {
+__global__ __launch_bounds__(64 * kMidWaves, 2) void adapter_mid_tile_kernel(const T* __restrict__ x,
+                                                                          const T* __restrict__ down,
+                                                                          const float* __restrict__ scale,
+                                                                          const int32_t* __restrict__ ids,
+                                                                          int adapters, int rank, int64_t rows,
+                                                                          int64_t K, T* __restrict__ mid) {
     typedef typename Elem16<T>::v8 v8;
-    __shared__ v4f s_part[8][RF][64];
+    constexpr int MT = 1, kPart = 64 * kMidWaves;
+    __shared__ v4f s_part[kMidWaves][MT * RF][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i16 = lane & 15, g = lane >> 4;
-    const int64_t row0 = (int64_t)blockIdx.x * 16, row = row0 + i16;
+    const int64_t row0 = (int64_t)blockIdx.x * 16 * MT;
     const int r0 = (int)blockIdx.y * 16 * RF;
-    int mine = row < rows ? ids[row] : -1;
-    if (mine < 0 || mine >= adapters) mine = -1;
-    const T* xr = x + min(row, rows - 1) * K;
+    int mine[MT];
+    const T* xr[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int64_t row = row0 + 16 * i + i16;
+        mine[i] = row < rows ? ids[row] : -1;
+        if (mine[i] >= adapters) mine[i] = -1;
+        xr[i] = x + min(row, rows - 1) * K;
+    }
     // rows without adapter
-    for (int q = threadIdx.x; q < 16 * 16 * RF; q += 512) {
+    for (int q = threadIdx.x; q < 16 * MT * 16 * RF; q += 64 * kMidWaves) {
         const int r = r0 + q % (16 * RF), m = q / (16 * RF);
         if (row0 + m >= rows || r >= rank) continue;
         const int id = ids[row0 + m];
@@ -89,21 +99,25 @@ __global__ __launch_bounds__(512) void adapter_mid_tile_kernel(const T* __restri
     }
     int cur = -1;
     while (true) {
-        cur = wave_min(mine > cur ? mine : INT_MAX);
+        int next = INT_MAX;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) next = min(next, mine[i] > cur ? mine[i] : INT_MAX);
+        cur = wave_min(next);
         if (cur == INT_MAX) break;
         const T* d = down + (int64_t)cur * rank * K;
-        v4f acc[RF] = {};
+        v4f acc[MT][RF] = {};
         int64_t k0 = 64 * wave;
         // U parts at a time, all their loads in flight; `whole`: within K
         auto parts = [&](auto u_, bool whole) __attribute__((always_inline)) {
             constexpr int U = decltype(u_)::value;
-            v8 xf[U][2], df[U][2][RF];
+            v8 xf[U][2][MT], df[U][2][RF];
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int64_t k = k0 + 512 * u + 32 * h + 8 * g, n = whole ? 8 : K - k;
-                    xf[u][h] = load_frag8<T>(xr + k, n);
+                    const int64_t k = k0 + kPart * u + 32 * h + 8 * g, n = whole ? 8 : K - k;
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) xf[u][h][i] = load_frag8<T>(xr[i] + k, n);
 #pragma unroll
                     for (int f = 0; f < RF; ++f) {
                         const int r = min(r0 + 16 * f + i16, rank - 1);   // (ranks past the last are dropped)
@@ -122,26 +136,33 @@ __global__ __launch_bounds__(512) void adapter_mid_tile_kernel(const T* __restri
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int f = 0; f < RF; ++f) acc[f] = Elem16<T>::mfma(df[u][h][f], xf[u][h], acc[f]);
-            k0 += 512 * U;
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int f = 0; f < RF; ++f)
+                            acc[i][f] = Elem16<T>::mfma(df[u][h][f], xf[u][h][i], acc[i][f]);
+            k0 += kPart * U;
         };
-        constexpr int U = RF == 4 ? 2 : KM ? 4 : 2;
-        while (k0 + 512 * (U - 1) + 64 <= K) parts(std::integral_constant<int, U>{}, true);
+        constexpr int U = KM ? 4 : 2;
+        while (k0 + kPart * (U - 1) + 64 <= K) parts(std::integral_constant<int, U>{}, true);
         while (k0 < K) parts(std::integral_constant<int, 1>{}, false);
 #pragma unroll
-        for (int f = 0; f < RF; ++f) s_part[wave][f][lane] = acc[f];
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int f = 0; f < RF; ++f) s_part[wave][i * RF + f][lane] = acc[i][f];
         __syncthreads();
-        // lane (row i16, ranks 4 g ..) of fragment f
-        const int f = threadIdx.x >> 6;
-        if (f < RF && mine == cur) {
-            v4f v = s_part[0][f][lane];
+        // entry (i, f, lane): row 16 i + i16, ranks 4 g .. of fragment f; a wave each
+        if (wave < MT * RF) {
+            const int i = wave / RF, f = wave % RF;
+            v4f v = s_part[0][wave][lane];
 #pragma unroll
-            for (int w = 1; w < 8; ++w) v += s_part[w][f][lane];
-            const float s = scale[cur];
+            for (int w = 1; w < kMidWaves; ++w) v += s_part[w][wave][lane];
+            if (mine[MT == 1 ? 0 : i] == cur) {
+                const float s = scale[cur];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = r0 + 16 * f + 4 * g + i;
-                if (r < rank) mid[row * rank + r] = (T)(s * v[i]);
+                for (int j = 0; j < 4; ++j) {
+                    const int r = r0 + 16 * f + 4 * g + j;
+                    if (r < rank) mid[(row0 + 16 * i + i16) * rank + r] = (T)(s * v[j]);
+                }
             }
         }
         __syncthreads();
@@ -166,7 +187,7 @@ int launch_mid(const void* x_, bool km, const void* down_, const float* scale, c
         const int rf = rank <= 16 ? 1 : rank <= 32 ? 2 : 4;
         const dim3 grid((unsigned)((rows + 15) / 16), (unsigned)((rank + 16 * rf - 1) / (16 * rf)));
         auto run = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, grid, dim3(512), 0, s, x, down, scale, ids, adapters, rank, rows, K, mid);
+            hipLaunchKernelGGL(kernel, grid, dim3(64 * kMidWaves), 0, s, x, down, scale, ids, adapters, rank, rows, K, mid);
         };
         if (rf == 1) km ? run(adapter_mid_tile_kernel<T, true, 1>) : run(adapter_mid_tile_kernel<T, false, 1>);
         else if (rf == 2) km ? run(adapter_mid_tile_kernel<T, true, 2>) : run(adapter_mid_tile_kernel<T, false, 2>);
@@ -177,26 +198,29 @@ int launch_mid(const void* x_, bool km, const void* down_, const float* scale, c
 }
 
 // ---- the matrices' gradients
-// A workgroup takes a 64 x 64 tile of one adapter's gradient over one part of the rows: it collects the rows that are
-// the adapter's, 64 at a time (in ascending order, so sums have one order), moves those rows' columns to the LDS and
-// multiplies them transposed.  Parts meet in a second kernel.  LDS rows are 64 columns of one row, 128 bytes, piece c at
-// c ^ s(row): the 8 rows that the LDS serves at once lie on all of its banks.
-// Bound by the rows' bytes and, for a part, one round trip for each 64 rows.
+// A workgroup takes a 64 x 64 tile of the gradients over one part of the rows, for every gridDim.y-th adapter in turn:
+// it collects the rows that are the adapter's, up to 256 at a time (in ascending order, so sums have one order), loads those rows' columns, and takes
+// them 64 at a time through the LDS, where they are read transposed.  Parts meet in a second kernel; a part without rows
+// of an adapter is a flag and no more.  LDS rows are 64 columns of one row, 128 bytes, piece c at c ^ s(row): the 8 rows
+// that the LDS serves at once lie on all of its banks.
+// Bound by round trips: the ids, the rows, and the parts' sums.
 constexpr int kGT = 64;
 constexpr int kScan = 1024;   // ids that a wave looks at at once
+constexpr int kRound = 256;   // rows that are loaded at once
 
-template <typename T, typename O>
+// EVEN: L and R are multiples of 8, so every piece is whole or absent and loads have no branches.  (The kernel runs
+// through its code about once, so the time goes with the code's length: instructions come from the L2.)
+template <typename T, typename O, bool EVEN>
 __global__ __launch_bounds__(kThreads) void adapter_grad_kernel(const T* __restrict__ left, const T* __restrict__ right,
                                                                 const int32_t* __restrict__ ids, int64_t rows,
                                                                 int64_t L, int64_t R, int64_t part_rows,
-                                                                float* __restrict__ parts, O* __restrict__ dw,
-                                                                int accumulate) {
+                                                                float* __restrict__ parts, int32_t* __restrict__ flags,
+                                                                O* __restrict__ dw, int adapters, int accumulate) {
     typedef typename Elem16<T>::v8 v8;
     __shared__ __attribute__((aligned(16))) uint8_t s_l[kGT * 128], s_r[kGT * 128];
-    __shared__ int s_list[4][128];   // (each wave its own)
+    __shared__ int s_list[4][2 * kRound];   // (each wave its own)
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wm = wave >> 1, wn = wave & 1, i16 = lane & 15, g = lane >> 4;
-    const int adapter = blockIdx.y;
     const int64_t ntr = (R + kGT - 1) / kGT;
     const int64_t l0 = (int64_t)blockIdx.x / ntr * kGT, c0 = (int64_t)blockIdx.x % ntr * kGT;
     const int64_t beg = (int64_t)blockIdx.z * part_rows, end = min(beg + part_rows, rows);
@@ -205,95 +229,147 @@ __global__ __launch_bounds__(kThreads) void adapter_grad_kernel(const T* __restr
     const int at0 = trow * 128 + 8 * (tc & 1), pc = tc >> 1;
     v4f acc[2][2] = {};
     int head = 0, count = 0;
-    auto stage = [&](int n) __attribute__((always_inline)) {   // the first n of the list
-        Loose8<T> v[2][2];
+    bool any = false;
+    auto round = [&](int n) __attribute__((always_inline)) {   // the first n of the list
+        constexpr int S = kRound / kGT;
+        v8 v[S][2][2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int q = t + kThreads * u, k = q >> 3, col = 8 * (q & 7);
-            const int64_t row = k < n ? s_list[wave][(head + k) & 127] : -1;
-            v[0][u] = __builtin_bit_cast(Loose8<T>, load_frag8<T>(left + row * L + l0 + col,
-                                                                  row >= 0 ? min(L - l0 - col, (int64_t)8) : 0));
-            v[1][u] = __builtin_bit_cast(Loose8<T>, load_frag8<T>(right + row * R + c0 + col,
-                                                                  row >= 0 ? min(R - c0 - col, (int64_t)8) : 0));
-        }
-        __syncthreads();
+        for (int s = 0; s < S; ++s) {
+            if (kGT * s >= n) break;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int q = t + kThreads * u, k = q >> 3, at = k * 128 + 16 * ((q & 7) ^ swz(k));
-            *reinterpret_cast<v8*>(s_l + at) = __builtin_bit_cast(v8, v[0][u]);
-            *reinterpret_cast<v8*>(s_r + at) = __builtin_bit_cast(v8, v[1][u]);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (32 * h >= n) break;
-            v8 a[2], b[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                b[i] = read_transposed<v8>(s_l + at0 + 32 * h * 128 + 16 * ((4 * wm + 2 * i + pc) ^ swz(trow)), 4 * 128);
-                a[i] = read_transposed<v8>(s_r + at0 + 32 * h * 128 + 16 * ((4 * wn + 2 * i + pc) ^ swz(trow)), 4 * 128);
+            for (int u = 0; u < 2; ++u) {
+                const int q = t + kThreads * u, k = kGT * s + (q >> 3), col = 8 * (q & 7);
+                const int64_t row = k < n ? s_list[wave][(head + k) & (2 * kRound - 1)] : -1;
+                if constexpr (EVEN) {
+                    const bool il = row >= 0 && l0 + col < L, ir = row >= 0 && c0 + col < R;
+                    const u64x2 vl = load16(left + (il ? row * L + l0 + col : 0));
+                    const u64x2 vr = load16(right + (ir ? row * R + c0 + col : 0));
+                    v[s][0][u] = __builtin_bit_cast(v8, il ? vl : u64x2{});
+                    v[s][1][u] = __builtin_bit_cast(v8, ir ? vr : u64x2{});
+                } else {
+                    const T *pl = left + row * L + l0 + col, *pr = right + row * R + c0 + col;
+                    v[s][0][u] = load_frag8<T>(pl, row >= 0 ? min(L - l0 - col, (int64_t)8) : 0);
+                    v[s][1][u] = load_frag8<T>(pr, row >= 0 ? min(R - c0 - col, (int64_t)8) : 0);
+                }
             }
+        }
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+        for (int s = 0; s < S; ++s) {
+            if (kGT * s >= n) break;
+            __syncthreads();
 #pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = Elem16<T>::mfma(a[j], b[i], acc[i][j]);
+            for (int u = 0; u < 2; ++u) {
+                const int q = t + kThreads * u, k = q >> 3, at = k * 128 + 16 * ((q & 7) ^ swz(k));
+                *reinterpret_cast<v8*>(s_l + at) = v[s][0][u];
+                *reinterpret_cast<v8*>(s_r + at) = v[s][1][u];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (kGT * s + 32 * h >= n) break;
+                v8 a[2], b[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int at = at0 + 32 * h * 128;
+                    b[i] = read_transposed<v8>(s_l + at + 16 * ((4 * wm + 2 * i + pc) ^ swz(trow)), 4 * 128);
+                    a[i] = read_transposed<v8>(s_r + at + 16 * ((4 * wn + 2 * i + pc) ^ swz(trow)), 4 * 128);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) acc[i][j] = Elem16<T>::mfma(a[j], b[i], acc[i][j]);
+            }
         }
         head += n;
         count -= n;
+        any = true;
     };
-    for (int64_t p0 = beg; p0 < end; p0 += kScan) {
-        int id[kScan / 64];
+    int id[kScan / 64];
+    int64_t loaded = -1;   // the first row whose ids are in registers
+    for (int adapter = blockIdx.y; adapter < adapters; adapter += gridDim.y) {
+        int64_t p0 = beg;
+        int i = 0;         // of the ids from p0 on, the next 64
+        any = false;
+        for (bool more = true; more;) {
+            while (count < kRound) {
+                if (i == kScan / 64) {
+                    i = 0;
+                    p0 += kScan;
+                }
+                if (p0 + 64 * i >= end) {
+                    more = false;
+                    break;
+                }
+                if (loaded != p0) {
 #pragma unroll
-        for (int i = 0; i < kScan / 64; ++i) {
-            const int64_t r = p0 + 64 * i + lane;
-            id[i] = r < end ? ids[r] : -1;
-        }
-        for (int i = 0; i < kScan / 64; ++i) {
-            int here = -1;
+                    for (int q = 0; q < kScan / 64; ++q) {
+                        const int64_t r = p0 + 64 * q + lane;
+                        id[q] = r < end ? ids[r] : -1;
+                    }
+                    loaded = p0;
+                }
+                int here = -1;
 #pragma unroll
-            for (int q = 0; q < kScan / 64; ++q) here = q == i ? id[q] : here;
-            const uint64_t m = __ballot(here == adapter);
-            if (!m) continue;
-            if (here == adapter)
-                s_list[wave][(head + count + __popcll(m & ((1ull << lane) - 1))) & 127] = (int)(p0 + 64 * i + lane);
-            count += __popcll(m);
-            if (count >= kGT) stage(kGT);
-        }
-    }
-    if (count > 0) stage(count);
-    // lane: row 16 i + i16 of the wave's 32, columns 4 g .. of its 16 j
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int64_t l = l0 + 32 * wm + 16 * i + i16;
-        if (l >= L) continue;
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const int64_t c = c0 + 32 * wn + 16 * j + 4 * g + v;
-                if (c >= R) continue;
-                const int64_t at = ((int64_t)adapter * L + l) * R + c;
-                if (parts) parts[(int64_t)blockIdx.z * gridDim.y * L * R + at] = acc[i][j][v];
-                else dw[at] = (O)(acc[i][j][v] + (accumulate ? (float)dw[at] : 0.0f));
+                for (int q = 0; q < kScan / 64; ++q) here = q == i ? id[q] : here;
+                const uint64_t m = __ballot(here == adapter);
+                if (here == adapter)
+                    s_list[wave][(head + count + __popcll(m & ((1ull << lane) - 1))) & (2 * kRound - 1)] =
+                        (int)(p0 + 64 * i + lane);
+                count += __popcll(m);
+                ++i;
             }
+            if (count > 0) round(min(count, kRound));
+        }
+        if (flags) {
+            if (blockIdx.x == 0 && t == 0) flags[(int64_t)blockIdx.z * adapters + adapter] = any;
+            if (!any) continue;
+        }
+        // lane: row 16 i + i16 of the wave's 32, columns 4 g .. of its 16 j
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int64_t l = l0 + 32 * wm + 16 * i + i16;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int64_t c = c0 + 32 * wn + 16 * j + 4 * g, at = ((int64_t)adapter * L + l) * R + c;
+                v4f v = acc[i][j];
+                acc[i][j] = v4f{};
+                if (l >= L) continue;
+                if (parts) {
+                    store4(parts + (int64_t)blockIdx.z * adapters * L * R + at - c, c, R, v, false);
+                } else {
+                    if (accumulate) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (c + k < R) v[k] += (float)dw[at + k];
+                    }
+                    store4(dw + at - c, c, R, v, false);
+                }
+            }
+        }
     }
 }
 
+// The parts' sums, in their order; blockIdx.y: the adapter.
 template <typename O>
-__global__ __launch_bounds__(kThreads) void adapter_grad_join_kernel(const float* __restrict__ parts, int n,
+__global__ __launch_bounds__(kThreads) void adapter_grad_join_kernel(const float* __restrict__ parts,
+                                                                     const int32_t* __restrict__ flags, int n,
                                                                      int64_t size, O* __restrict__ dw,
                                                                      int accumulate) {
+    const int a = blockIdx.y, lane = threadIdx.x & 63;
+    uint64_t has = __ballot(lane < n && flags[(int64_t)min(lane, n - 1) * gridDim.y + a]);   // n <= 64
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < size; i += (int64_t)gridDim.x * kThreads) {
-        float v = 0.0f;
-        for (int s = 0; s < n; ++s) v += parts[s * size + i];
-        dw[i] = (O)(v + (accumulate ? (float)dw[i] : 0.0f));
+        const int64_t at = a * size + i;
+        float v = accumulate ? (float)dw[at] : 0.0f;
+        float sum = 0.0f;
+        for (uint64_t m = has; m; m &= m - 1) sum += parts[(__ffsll((long long)m) - 1) * gridDim.y * size + at];
+        dw[at] = (O)(sum + v);
     }
 }
 
-// Parts that the rows are cut into: so many that about 1024 workgroups share the work, 128 rows a part at least.
+// Parts that the rows are cut into: so many that about 512 workgroups share the work, 256 rows a part at least.
 int grad_parts(int64_t adapters, int64_t rows, int64_t L, int64_t R) {
-    const int64_t tiles = ((L + kGT - 1) / kGT) * ((R + kGT - 1) / kGT) * adapters;
-    return (int)std::max((int64_t)1, std::min(std::min((int64_t)1024 / tiles, (rows + 127) / 128), (int64_t)64));
+    const int64_t tiles = ((L + kGT - 1) / kGT) * ((R + kGT - 1) / kGT);
+    return (int)std::max((int64_t)1, std::min(std::min((int64_t)512 / tiles, (rows + 255) / 256), (int64_t)64));
 }
 
 template <typename T, typename O>
@@ -303,14 +379,21 @@ int launch_grad(const void* left, const void* right, const int32_t* ids, int64_t
     const int64_t tiles = ((L + kGT - 1) / kGT) * ((R + kGT - 1) / kGT), size = adapters * L * R;
     if (tiles > INT_MAX / kThreads) return HM_ERR_OVERFLOW;
     float* parts = n > 1 ? static_cast<float*>(workspace) : nullptr;
-    hipLaunchKernelGGL((adapter_grad_kernel<T, O>), dim3((unsigned)tiles, (unsigned)adapters, (unsigned)n),
-                       dim3(kThreads), 0, s, static_cast<const T*>(left), static_cast<const T*>(right), ids, rows, L, R,
-                       (rows + n - 1) / n, parts, static_cast<O*>(dw), accumulate);
+    int32_t* flags = n > 1 ? reinterpret_cast<int32_t*>(parts + n * size) : nullptr;
+    const int64_t share = std::max((int64_t)1, std::min(adapters, 1024 / (tiles * n)));
+    auto run = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, (unsigned)share, (unsigned)n), dim3(kThreads), 0, s,
+                           static_cast<const T*>(left), static_cast<const T*>(right), ids, rows, L, R, (rows + n - 1) / n,
+                           parts, flags, static_cast<O*>(dw), (int)adapters, accumulate);
+    };
+    if (L % 8 == 0 && R % 8 == 0) run(adapter_grad_kernel<T, O, true>);
+    else run(adapter_grad_kernel<T, O, false>);
     HM_LAUNCHED();
     if (n > 1) {
+        const int64_t each = L * R;
         hipLaunchKernelGGL((adapter_grad_join_kernel<O>),
-                           dim3((unsigned)std::min((size + kThreads - 1) / kThreads, (int64_t)4096)), dim3(kThreads), 0, s,
-                           parts, n, size, static_cast<O*>(dw), accumulate);
+                           dim3((unsigned)std::min((each + kThreads - 1) / kThreads, (int64_t)4096), (unsigned)adapters),
+                           dim3(kThreads), 0, s, parts, flags, n, each, static_cast<O*>(dw), accumulate);
         HM_LAUNCHED();
     }
     return HM_OK;
@@ -369,7 +452,8 @@ size_t hm_adapter_weight_grad_workspace_bytes(int64_t adapters, int64_t rows, in
         left_cols > kMaxDim || right_cols > kMaxDim || left_cols * right_cols > kMaxMatrix)
         return 0;
     const int n = grad_parts(adapters, rows, left_cols, right_cols);
-    return n > 1 ? (size_t)n * adapters * left_cols * right_cols * sizeof(float) : 0;
+    // the parts' sums, then a flag for each part and adapter
+    return n > 1 ? (size_t)n * adapters * (left_cols * right_cols + 1) * 4 : 0;
 }
 
 int hm_adapter_weight_grad(const void* left, const void* right, int32_t dtype, const int32_t* ids,

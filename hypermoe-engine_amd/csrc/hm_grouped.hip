@@ -310,11 +310,16 @@ static int pick(GKind kind, bool w_kmajor, const GProduct& p) {
     if (nt && (each <= 16 || p.rows <= 64)) return (p.rows <= 16 || each <= 4 ? 1 : p.rows <= 32 || each <= 8 ? 2 : 4) << 16;
     if (kind == G_ADAPTER && nt && p.rows <= 128) return 8 << 16;
     if (!tile_ok(kind, p)) return 0;
-    if (!dma_ok(kind, w_kmajor, p)) return 32;
-    const int64_t tm = kind == G_WEIGHT_GRAD ? p.groups * ((p.M + 127) / 128) : p.rows / 128 + groups;
-    if (tm * ((p.N + 255) / 256) < 256) return 64;
-    if (kind == G_WEIGHT_GRAD || each >= 384) return 256;
-    return 128;
+    const bool wg = kind == G_WEIGHT_GRAD;
+    const int64_t m128 = wg ? p.groups * ((p.M + 127) / 128) : p.rows / 128 + groups;
+    // Off 16 bytes (128 x 128 tiles through registers against the generic kernel's 64 x 64): 16 groups of 512 rows,
+    // 1001 x 1333, 70 us and 190, but 8 of 100, 1001 x 777, transposed 44 and 36: few tiles leave most of the chip idle.
+    if (!dma_ok(kind, w_kmajor, p)) return nt || m128 * ((p.N + 127) / 128) >= 128 ? 32 : 0;
+    // 128 x 128 where larger tiles are fewer than the chip's CUs: 2048 x 2048 x 2048 27 us, 128 x 256 34, 256 x 256 48.
+    if (m128 * ((p.N + 255) / 256) < 256) return 64;
+    // 256 x 256 from 384 rows a group on: 8 groups of 4096 rows, 2048 x 1536, 195 us against 219 of 128 x 256; but 128
+    // of 256 rows on average, uneven, 196 and 164: half of the second tile of a group is empty.
+    return wg || each >= 384 ? 256 : 128;
 }
 
 int hm_g_launch(GKind kind, bool w_kmajor, int32_t dtype, int32_t y_dtype, const GProduct& p_, hipStream_t s) {

@@ -15,8 +15,9 @@
 //   w                 fragment j's row i is column 32 (j / 2) + 8 (i / 4) + 4 (j % 2) + i % 4 of the wave's, so that a
 //                     lane ends with 8 consecutive results of a row from two fragments, and four lanes with 32.  In
 //                     the transposed form j % 2 is (j + i / 4) % 2, or half of the banks would stand idle.
-//   order             tiles are cut into 8 contiguous ranges, one per XCD (workgroup i runs on XCD i % 8); within
-//                     a group m-tiles by SUPER, so what is read by several workgroups at once is in one L2.
+//   order             tiles are cut into 8 ranges, one per XCD (workgroup i runs on XCD i % 8), whose workgroups take them
+//                     in turn; within a group m-tiles by kSuper, so what is read by several workgroups at once is in
+//                     one L2 (128 groups of 256 rows, 2048 x 1536: 279 us; each workgroup a range of its own: 418).
 #pragma once
 
 #include "hm_grouped.h"
@@ -59,7 +60,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     static_assert(DMA || NW == 4, "fetch() takes the swizzles to be the same for every c");
     static_assert(XF % 2 == 0 && (SH == 2 || SH == 4 || SH == 8) && BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "tile");
     __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * STAGE];
-    __shared__ int s_pre[WG ? 1 : HM_GROUPED_MAX_GROUPS + 1];  // m-tiles before each group
+    __shared__ int s_pre[HM_GROUPED_MAX_GROUPS + 1], s_cost[HM_GROUPED_MAX_GROUPS + 1];  // m-tiles, cost before a group
 
     // (the barriers are hand-written: without this the compiler may take the ring, whose address would leave the
     // function nowhere where there is no DMA, to be out of their reach)
@@ -72,53 +73,71 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     const T* xp = static_cast<const T*>(p.x);
     const T* wp = static_cast<const T*>(p.w);
 
-    // ---- tiles
-    int total;
-    if constexpr (WG) {
-        total = p.groups * (int)((p.M + BM - 1) / BM) * ntn;
-    } else {
-        if (p.offsets) {
-            // 4 groups a thread; a group's rows are cut to 0 .. rows, and none where its offsets descend
-            const int e0 = 4 * threadIdx.x;
-            int cnt[4], sum = 0;
+    // ---- tiles: an XCD takes a range of them of an eighth of the cost, its workgroups every step-th tile of that.
+    // A tile costs its rows, 16 at a time (weight gradient: its stages), and COST besides.
+    constexpr int COST = WG ? 6 : 3 * BM / 64;
+    const int mtw = (int)((p.M + BM - 1) / BM);       // weight gradient: m-tiles
+    int total, cost = 0;
+    if (p.offsets) {
+        // 4 groups a thread; a group's rows are cut to 0 .. rows, and none where its offsets descend
+        const int e0 = 4 * threadIdx.x;
+        int cnt[4], cst[4], sum = 0, csum = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                cnt[i] = 0;
-                if (e0 + i < p.groups) {
-                    const int lo = max(0, p.offsets[e0 + i]);
-                    const int hi = (int)min((int64_t)p.offsets[e0 + i + 1], p.rows);
-                    cnt[i] = hi > lo ? (hi - lo - 1) / BM + 1 : 0;
-                }
-                sum += cnt[i];
+        for (int i = 0; i < 4; ++i) {
+            cnt[i] = cst[i] = 0;
+            if (e0 + i < p.groups) {
+                const int lo = max(0, p.offsets[e0 + i]);
+                const int n = max(0, (int)min((int64_t)p.offsets[e0 + i + 1], p.rows) - lo);
+                cnt[i] = (n + BM - 1) / BM;
+                cst[i] = WG ? (n + kBK - 1) / kBK + COST : (n + 15) / 16 + cnt[i] * COST;
             }
-            int incl = sum;
-#pragma unroll
-            for (int m = 1; m < 64; m <<= 1) {
-                const int o = __shfl_up(incl, m, 64);
-                if (lane >= m) incl += o;
-            }
-            int* s_wave = reinterpret_cast<int*>(ring);
-            if (lane == 63) s_wave[wave] = incl;
-            __syncthreads();
-            int base = incl - sum;
-            for (int i = 0; i < wave; ++i) base += s_wave[i];
-            if (threadIdx.x == 0) s_pre[0] = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                base += cnt[i];
-                if (e0 + i < p.groups) s_pre[e0 + i + 1] = base;
-            }
-            __syncthreads();
-            total = s_pre[p.groups] * ntn;
-        } else {
-            total = (int)((p.rows + BM - 1) / BM) * ntn;
+            sum += cnt[i];
+            csum += cst[i];
         }
+        int incl = sum, cincl = csum;
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const int o = __shfl_up(incl, m, 64), co = __shfl_up(cincl, m, 64);
+            if (lane >= m) incl += o, cincl += co;
+        }
+        int* s_wave = reinterpret_cast<int*>(ring);
+        if (lane == 63) s_wave[wave] = incl, s_wave[NW + wave] = cincl;
+        __syncthreads();
+        int base = incl - sum, cbase = cincl - csum;
+        for (int i = 0; i < wave; ++i) base += s_wave[i], cbase += s_wave[NW + i];
+        if (threadIdx.x == 0) s_pre[0] = s_cost[0] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            base += cnt[i];
+            cbase += cst[i];
+            if (e0 + i < p.groups) s_pre[e0 + i + 1] = base, s_cost[e0 + i + 1] = cbase;
+        }
+        __syncthreads();
+        total = uni(WG ? p.groups * mtw * ntn : s_pre[p.groups] * ntn);
+        cost = uni(s_cost[p.groups]);
+    } else {
+        total = (int)((p.rows + BM - 1) / BM) * ntn;
     }
-    total = uni(total);
-    const int per = (total + kXcds - 1) / kXcds;
+    // how many entries 1 .. groups of an ascending array are at most v / scale
+    auto below = [&](const int* pre, int64_t scale, int64_t v) __attribute__((always_inline)) {
+        int e = 0;
+        for (int c = 0; c < p.groups; c += 64)
+            e += __popcll(__ballot(c + lane < p.groups && pre[min(c + lane, p.groups - 1) + 1] * scale <= v));
+        return min(uni(e), p.groups - 1);
+    };
+    auto share = [&](int x) __attribute__((always_inline)) {
+        if (!p.offsets) return (int)(((int64_t)total * x) >> 3);
+        if (x == kXcds) return total;
+        const int64_t v = (int64_t)cost * x;
+        const int e = below(s_cost, kXcds, v);
+        const int first = WG ? e * mtw * ntn : uni(s_pre[e]) * ntn;
+        const int tiles = WG ? mtw * ntn : (uni(s_pre[e + 1]) - uni(s_pre[e])) * ntn;
+        const int c0 = uni(s_cost[e]), c1 = uni(s_cost[e + 1]);
+        return uni(first + min(tiles, (int)((float)(v - (int64_t)c0 * kXcds) * tiles / ((float)(c1 - c0) * kXcds))));
+    };
     const int step = gridDim.x / kXcds;
-    const int jbeg = (blockIdx.x % kXcds) * per + blockIdx.x / kXcds;
-    const int jend = min((int)(blockIdx.x % kXcds + 1) * per, total);
+    const int jbeg = uni(share(blockIdx.x % kXcds)) + blockIdx.x / kXcds;
+    const int jend = uni(share(blockIdx.x % kXcds + 1));
     if (jbeg >= jend) return;
 
     // Tile j (the same in every lane).
@@ -126,7 +145,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
         TileAt t;
         int mt, jl = j;
         if constexpr (WG) {
-            mt = (int)((p.M + BM - 1) / BM);
+            mt = mtw;
             t.e = j / (mt * ntn);
             jl = j - t.e * mt * ntn;
             const int lo = max(0, p.offsets[t.e]);
@@ -135,11 +154,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
             t.kn = uni(max(0, hi - lo));
             t.nb = max(1, (t.kn + kBK - 1) / kBK);
         } else if (p.offsets) {
-            const int m = j / ntn;
-            int e = 0;
-            for (int c = 0; c < p.groups; c += 64)
-                e += __popcll(__ballot(c + lane < p.groups && s_pre[min(c + lane, p.groups - 1) + 1] <= m));
-            t.e = min(uni(e), p.groups - 1);
+            t.e = below(s_pre, 1, j / ntn);
             mt = uni(s_pre[t.e + 1]) - uni(s_pre[t.e]);
             jl = j - uni(s_pre[t.e]) * ntn;
         } else {
@@ -539,7 +554,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     // ---- the stream
     TileAt cur = tile_at(jbeg);
     int cj = jbeg, slot = 0;
-    bool stored = false;
+    int stored = 0;            // steps whose wait comes before the end of a whole tile's stores
     pt = cur;
     make_src();
 #pragma unroll
@@ -568,18 +583,18 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
         if constexpr (DMA) {
             if (stored) wait_vmcnt<std::min(60, (NS - 2) * LPW + STORES)>();
             else wait_vmcnt<(NS - 2) * LPW>();
-            stored = false;
+            stored = max(0, stored - 1);
         }
         lds_barrier();
         const int next = slot == NS - 1 ? 0 : slot + 1;
-        mma(fb, fa, ring + next * STAGE, 0, true, slot);
         const bool done = uni((int)(last >> slot)) & 1;
+        mma(fb, fa, ring + next * STAGE, 0, true, slot);
         advance(slot);
         if constexpr (!DMA) fetch();
         slot = next;
         if (!done) continue;
         finish(cur);
-        stored = whole(cur);
+        stored = whole(cur) ? NS - 1 : 0;
         cj += step;
         if (cj >= jend) break;
         cur = tile_at(cj);
