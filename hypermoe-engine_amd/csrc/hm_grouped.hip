@@ -316,7 +316,8 @@ static int pick(GKind kind, bool w_kmajor, const GProduct& p) {
     // 1001 x 1333, 70 us and 190, but 8 of 100, 1001 x 777, transposed 44 and 36: few tiles leave most of the chip idle.
     if (!dma_ok(kind, w_kmajor, p)) return nt || m128 * ((p.N + 127) / 128) >= 128 ? 32 : 0;
     // 128 x 128 where larger tiles are fewer than the chip's CUs: 2048 x 2048 x 2048 27 us, 128 x 256 34, 256 x 256 48.
-    if (m128 * ((p.N + 255) / 256) < 256) return 64;
+    const int wide = kind == G_SWIGLU ? 128 : 256;   // (gate and up share a tile)
+    if (m128 * ((p.N + wide - 1) / wide) < 256) return 64;
     // 256 x 256 from 384 rows a group on: 8 groups of 4096 rows, 2048 x 1536, 195 us against 219 of 128 x 256; but 128
     // of 256 rows on average, uneven, 196 and 164: half of the second tile of a group is empty.
     return wg || each >= 384 ? 256 : 128;
@@ -441,6 +442,23 @@ int hm_grouped_weight_grad(const void* dy, const void* x, int32_t dtype, const i
     p.groups = (int)groups;
     p.accumulate = accumulate;
     return hm_g_launch(G_WEIGHT_GRAD, false, dtype, dw_dtype, p, hm_stream(stream));
+}
+
+int hm_debug_grouped_form(int32_t kind, int64_t groups, int64_t rows, int64_t inner, int64_t cols, int32_t rank,
+                          int32_t aligned16) {
+    if (kind < 0 || kind > 6 || check_sizes(groups, rows, inner, cols) || rows == 0) return -1;
+    static const GKind kinds[7] = {G_MATMUL, G_MATMUL, G_SWIGLU, G_SWIGLU_GRAD, G_WEIGHT_GRAD, G_ADAPTER, G_ADAPTER};
+    const void* at = reinterpret_cast<const void*>((uintptr_t)(aligned16 ? 1 << 20 : (1 << 20) + 2));
+    GProduct p = {};
+    p.x = p.w = p.mid = p.up = at;
+    p.offsets = kind < 5 ? static_cast<const int32_t*>(at) : nullptr;
+    p.rows = p.x_rows = rows;
+    p.groups = (int)groups;
+    p.K = inner;
+    p.M = cols;   // weight gradient: [cols x inner]
+    p.N = kind == 4 ? inner : cols;
+    p.rank = rank;
+    return pick(kinds[kind], kind == 0 || kind == 2 || kind == 5, p);
 }
 
 }  // extern "C"

@@ -120,6 +120,7 @@ SIGNATURES = {
                                        c_sz, vp]),
     "hm_debug_fp8_matmul_form": (c_i32, [c_i64, c_i64, c_i64, c_i32]),
     "hm_debug_fp8_experts_form": (c_i32, [C.POINTER(HmLayer), c_i64, c_i64, c_i32]),
+    "hm_debug_grouped_form": (c_i32, [c_i32, c_i64, c_i64, c_i64, c_i64, c_i32, c_i32]),
     "hm_debug_expf": (c_i32, [vp, vp, c_i64, vp]),
 }
 

@@ -582,6 +582,17 @@ int hm_debug_fp8_matmul_form(int64_t rows, int64_t inner, int64_t cols,
 int hm_debug_fp8_experts_form(const hm_layer* layer, int64_t tokens,
                               int64_t pairs, int32_t y_dtype);
 
+/* The same for F4 and F5.  kind 0, 1: hm_grouped_matmul, w_transposed; 2:
+ * hm_grouped_swiglu (its own rows); 3: hm_grouped_swiglu_grad (inner: hidden,
+ * cols: intermediate); 4: hm_grouped_weight_grad; 5, 6: hm_adapter_matmul,
+ * w_transposed (groups 1).  m << 16: the kernel that streams w for 16 m rows
+ * at a time; 256, 128, 64: tiles of 256 x 256, 128 x 256 and 128 x
+ * 128; 32: tiles of 128 x 128 for operands off 16 bytes; 0: the generic kernel.
+ * -1: not a call. */
+int hm_debug_grouped_form(int32_t kind, int64_t groups, int64_t rows,
+                          int64_t inner, int64_t cols, int32_t rank,
+                          int32_t aligned16);
+
 #ifdef __cplusplus
 }
 #endif
