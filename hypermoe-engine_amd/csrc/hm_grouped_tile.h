@@ -32,7 +32,6 @@ namespace {
 
 constexpr int kXcds = 8;
 constexpr int kThreads = 256;
-constexpr int kBK = 64;
 constexpr int kSuper = 4;
 
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -50,17 +49,20 @@ struct TileAt {
     int nb;             // stages of k
 };
 
-template <int WMC, int WNC, int XF, int WF, int NS, bool DMA, GKind KIND, bool WK, typename T, typename O>
+template <int WMC, int WNC, int XF, int WF, int KB, int NS, bool DMA, GKind KIND, bool WK, typename T, typename O>
 __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     typedef typename Elem16<T>::v8 v8;
     constexpr bool WG = KIND == G_WEIGHT_GRAD, XK = !WG, GU = KIND == G_SWIGLU;
     constexpr int NW = WMC * WNC, BM = 16 * XF * WMC, BN = 16 * WF * WNC, SH = GU ? WF / 2 : WF, TN = GU ? BN / 2 : BN;
-    constexpr int STAGE = 128 * (BM + BN), WOFF = 128 * BM;
-    constexpr int XL = BM / 8 / NW, LPW = (BM + BN) / 8 / NW;   // a wave's 1 KB loads a stage, of x first
+    constexpr int ROW = 2 * KB, RPB = 1024 / ROW, PCS = KB / 8;   // a k-major row's bytes, rows in 1 KB, pieces
+    constexpr int STAGE = ROW * (BM + BN), WOFF = ROW * BM;
+    constexpr int XL = BM / RPB / NW, LPW = (BM + BN) / RPB / NW;   // a wave's 1 KB loads a stage, of x first
+    static_assert(KB == 64 || (KB == 32 && DMA), "stage");
+    static_assert(RPB * NW <= 64, "ids");
     static_assert(DMA || NW == 4, "fetch() takes the swizzles to be the same for every c");
-    static_assert(XF % 2 == 0 && (SH == 2 || SH == 4 || SH == 8) && BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "tile");
+    static_assert(XF % 2 == 0 && (SH == 2 || SH == 4 || SH == 8) && BM % (RPB * NW) == 0 && BN % (RPB * NW) == 0, "tile");
     __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * STAGE];
-    __shared__ int s_pre[HM_GROUPED_MAX_GROUPS + 1], s_cost[HM_GROUPED_MAX_GROUPS + 1];  // m-tiles, cost before a group
+    __shared__ int s_pre[HM_GROUPED_MAX_GROUPS], s_cost[HM_GROUPED_MAX_GROUPS];  // m-tiles, cost to a group's end
 
     // (the barriers are hand-written: without this the compiler may take the ring, whose address would leave the
     // function nowhere where there is no DMA, to be out of their reach)
@@ -75,7 +77,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
 
     // ---- tiles: an XCD takes a range of them of an eighth of the cost, its workgroups every step-th tile of that.
     // A tile costs its rows, 16 at a time (weight gradient: its stages), and COST besides.
-    constexpr int COST = WG ? 6 : 3 * BM / 64;
+    constexpr int COST = WG ? 6 * 64 / KB : 3 * BM / 64;
     const int mtw = (int)((p.M + BM - 1) / BM);       // weight gradient: m-tiles
     int total, cost = 0;
     if (p.offsets) {
@@ -89,7 +91,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
                 const int lo = max(0, p.offsets[e0 + i]);
                 const int n = max(0, (int)min((int64_t)p.offsets[e0 + i + 1], p.rows) - lo);
                 cnt[i] = (n + BM - 1) / BM;
-                cst[i] = WG ? (n + kBK - 1) / kBK + COST : (n + 15) / 16 + cnt[i] * COST;
+                cst[i] = WG ? (n + KB - 1) / KB + COST : (n + 15) / 16 + cnt[i] * COST;
             }
             sum += cnt[i];
             csum += cst[i];
@@ -105,24 +107,24 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
         __syncthreads();
         int base = incl - sum, cbase = cincl - csum;
         for (int i = 0; i < wave; ++i) base += s_wave[i], cbase += s_wave[NW + i];
-        if (threadIdx.x == 0) s_pre[0] = s_cost[0] = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             base += cnt[i];
             cbase += cst[i];
-            if (e0 + i < p.groups) s_pre[e0 + i + 1] = base, s_cost[e0 + i + 1] = cbase;
+            if (e0 + i < p.groups) s_pre[e0 + i] = base, s_cost[e0 + i] = cbase;
         }
         __syncthreads();
-        total = uni(WG ? p.groups * mtw * ntn : s_pre[p.groups] * ntn);
-        cost = uni(s_cost[p.groups]);
+        total = uni(WG ? p.groups * mtw * ntn : s_pre[p.groups - 1] * ntn);
+        cost = uni(s_cost[p.groups - 1]);
     } else {
         total = (int)((p.rows + BM - 1) / BM) * ntn;
     }
-    // how many entries 1 .. groups of an ascending array are at most v / scale
+    auto before = [&](const int* pre, int e) __attribute__((always_inline)) { return e ? uni(pre[e - 1]) : 0; };
+    // how many of an ascending array are at most v / scale
     auto below = [&](const int* pre, int64_t scale, int64_t v) __attribute__((always_inline)) {
         int e = 0;
         for (int c = 0; c < p.groups; c += 64)
-            e += __popcll(__ballot(c + lane < p.groups && pre[min(c + lane, p.groups - 1) + 1] * scale <= v));
+            e += __popcll(__ballot(c + lane < p.groups && pre[min(c + lane, p.groups - 1)] * scale <= v));
         return min(uni(e), p.groups - 1);
     };
     auto share = [&](int x) __attribute__((always_inline)) {
@@ -130,9 +132,9 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
         if (x == kXcds) return total;
         const int64_t v = (int64_t)cost * x;
         const int e = below(s_cost, kXcds, v);
-        const int first = WG ? e * mtw * ntn : uni(s_pre[e]) * ntn;
-        const int tiles = WG ? mtw * ntn : (uni(s_pre[e + 1]) - uni(s_pre[e])) * ntn;
-        const int c0 = uni(s_cost[e]), c1 = uni(s_cost[e + 1]);
+        const int first = WG ? e * mtw * ntn : before(s_pre, e) * ntn;
+        const int tiles = WG ? mtw * ntn : (uni(s_pre[e]) - before(s_pre, e)) * ntn;
+        const int c0 = before(s_cost, e), c1 = uni(s_cost[e]);
         return uni(first + min(tiles, (int)((float)(v - (int64_t)c0 * kXcds) * tiles / ((float)(c1 - c0) * kXcds))));
     };
     const int step = gridDim.x / kXcds;
@@ -152,11 +154,11 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
             const int hi = (int)min((int64_t)p.offsets[t.e + 1], p.rows);
             t.k0 = uni(lo);
             t.kn = uni(max(0, hi - lo));
-            t.nb = max(1, (t.kn + kBK - 1) / kBK);
+            t.nb = max(1, (t.kn + KB - 1) / KB);
         } else if (p.offsets) {
             t.e = below(s_pre, 1, j / ntn);
-            mt = uni(s_pre[t.e + 1]) - uni(s_pre[t.e]);
-            jl = j - uni(s_pre[t.e]) * ntn;
+            mt = uni(s_pre[t.e]) - before(s_pre, t.e);
+            jl = j - before(s_pre, t.e) * ntn;
         } else {
             t.e = 0;
             mt = (int)((p.rows + BM - 1) / BM);
@@ -175,7 +177,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
             t.nrows = min(BM, hi - t.row0);
             t.k0 = 0;
             t.kn = K;
-            t.nb = (K + kBK - 1) / kBK;
+            t.nb = (K + KB - 1) / KB;
         }
         t.row0 = uni(t.row0);
         t.nrows = uni(t.nrows);
@@ -191,10 +193,12 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     int left = 0;              // k from the stage's first on
     int xcols = 0, wcols = 0;  // without DMA, operands that are not k-major: columns from this lane's on
     auto x_swz = [](int r) __attribute__((always_inline)) {
-        return XK ? (r >> 1) & 7 : ((r & 3) << 1) | (r & 8);
+        if constexpr (XK) return KB == 64 ? (r >> 1) & 7 : (r >> 2) & 3;
+        return ((r & 3) << 1) | (r & 8);
     };
     auto w_swz = [](int r) __attribute__((always_inline)) {
-        return WK ? ((r >> 1) & 1) | (((r >> 3) & 3) << 1) : (r & 1) | ((r & 2) << 1) | (r & 8);
+        if constexpr (WK) return KB == 64 ? ((r >> 1) & 1) | (((r >> 3) & 3) << 1) : (r >> 3) & 3;
+        return (r & 1) | ((r & 2) << 1) | (r & 8);
     };
     // byte offset of the row of x that tile row r reads (from xbase)
     auto x_off = [&](const TileAt& t, int r) __attribute__((always_inline)) -> uint32_t {
@@ -217,8 +221,8 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     };
     // where the stage is the last of k: what lies past it counts as zeros in both operands
     auto cut = [&]() __attribute__((always_inline)) {
-        left = uni(pt.kn - pks * kBK);
-        if (left >= kBK || (!DMA && XK && WK)) return;
+        left = uni(pt.kn - pks * KB);
+        if (left >= KB || (!DMA && XK && WK)) return;
         int l = lane;
         asm volatile("" : "+v"(l));
 #pragma unroll
@@ -228,8 +232,8 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
             int k;
             if ((isx && XK) || (!isx && WK)) {
                 if (!DMA) continue;   // (these count what is left of a piece)
-                const int r = 8 * b + (l >> 3);
-                k = 8 * ((l & 7) ^ (isx ? x_swz(r) : w_swz(r)));
+                const int r = RPB * b + l / PCS;
+                k = 8 * (l % PCS ^ (isx ? x_swz(r) : w_swz(r)));
             } else {
                 const int pcs = isx ? BM / 8 : BN / 8;
                 k = b * (64 / pcs) + l / pcs;
@@ -240,7 +244,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     // ---- adapters: behind a tile's stages of k, for each adapter that its rows name (ascending) the stages of its
     // rank: mid, with the rows of other adapters as zeros, and the adapter's matrix.  A lane knows the adapters of the
     // tile's rows lane + 64 i.
-    constexpr int IDS = KIND == G_ADAPTER ? BM / 64 : 1;
+    constexpr int IDS = KIND == G_ADAPTER ? (BM + 63) / 64 : 1;
     int ids[IDS];
     int low = -1;              // the adapter whose stages are loaded, -1: k's; INT_MAX: past the last tile
     int lows = 0;              // its stage
@@ -256,10 +260,10 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     };
     auto next_low = [&]() __attribute__((always_inline)) {
         if (low == INT_MAX) return false;
-        if (low >= 0 && (lows + 1) * kBK < p.rank) {
+        if (low >= 0 && (lows + 1) * KB < p.rank) {
             ++lows;
-            xbase += 2 * kBK;
-            wbase = uni(wbase + (WK ? 2 * kBK : 2 * (int64_t)kBK * N));
+            xbase += 2 * KB;
+            wbase = uni(wbase + (WK ? 2 * KB : 2 * (int64_t)KB * N));
         } else {
             int v = INT_MAX;
 #pragma unroll
@@ -272,7 +276,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
             wbase = uni(static_cast<const uint8_t*>(p.up) +
                         2 * ((int64_t)low * N * p.rank + (WK ? (int64_t)pt.n0 * p.rank : (int64_t)pt.n0)));
         }
-        left = uni(p.rank - lows * kBK);
+        left = uni(p.rank - lows * KB);
         int l = lane;
         asm volatile("" : "+v"(l));
 #pragma unroll
@@ -280,8 +284,8 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
             const bool isx = c < XL;
             const int b = wave + NW * (isx ? c : c - XL);
             if (isx || WK) {
-                const int r = 8 * b + (l >> 3), pc = (l & 7) ^ (isx ? x_swz(r) : w_swz(r));
-                const bool mine = isx ? __shfl(ids[NW * c / 8 % IDS], r & 63, 64) == low : pt.n0 + r < N;
+                const int r = RPB * b + l / PCS, pc = l % PCS ^ (isx ? x_swz(r) : w_swz(r));
+                const bool mine = isx ? __shfl(ids[RPB * NW * c / 64 % IDS], r & 63, 64) == low : pt.n0 + r < N;
                 voff[c] = mine && (!DMA || 8 * pc < left) ? (uint32_t)r * (uint32_t)p.rank * 2 + 16 * pc : HM_BUF_RANGE;
             } else {
                 const int r = b * (512 / BN) + l / (BN / 8), col = 8 * ((l % (BN / 8)) ^ w_swz(r));
@@ -308,9 +312,9 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
             const bool isx = c < XL;
             const int b = wave + NW * (isx ? c : c - XL);
             if ((isx && XK) || (!isx && WK)) {
-                const int r = 8 * b + (l >> 3);
+                const int r = RPB * b + l / PCS;
                 const uint32_t row = isx ? x_off(t, r) : w_off(t, r);
-                voff[c] = row + 16 * ((l & 7) ^ (isx ? x_swz(r) : w_swz(r)));
+                voff[c] = row + 16 * (l % PCS ^ (isx ? x_swz(r) : w_swz(r)));
             } else {
                 const int pcs = isx ? BM / 8 : BN / 8;   // pieces a row
                 const int ld = isx ? (int)p.M : N;
@@ -325,8 +329,8 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
         if constexpr (KIND == G_ADAPTER) read_ids();
     };
     // bytes from one stage's values to the next one's
-    const int64_t xstep = XK ? 2 * kBK : 2 * (int64_t)kBK * p.M;
-    const int64_t wstep = WK ? 2 * kBK : 2 * (int64_t)kBK * N;
+    const int64_t xstep = XK ? 2 * KB : 2 * (int64_t)KB * p.M;
+    const int64_t wstep = WK ? 2 * KB : 2 * (int64_t)KB * N;
     // load c of the producer's stage into a slot
     hm_buf xbuf, wbuf;
     v8 regs[DMA ? 1 : LPW];
@@ -350,7 +354,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
         // values of a row, and from the stage's first piece on; whether every piece is whole
         const int xrow = XK ? (low >= 0 ? p.rank : K) : (int)p.M, wrow = WK ? (low >= 0 ? p.rank : K) : N;
         const int xleft = XK ? left : (int)p.M - pt.row0, wleft = WK ? left : N - pt.n0;
-        const bool whole = xleft >= (XK ? kBK : BM) && wleft >= (WK ? kBK : BN);
+        const bool whole = xleft >= (XK ? KB : BM) && wleft >= (WK ? KB : BN);
         auto load = [&](auto kind) __attribute__((always_inline)) {
 #pragma unroll
             for (int c = 0; c < LPW; ++c) {
@@ -426,11 +430,11 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     // values of row i16 / 4 and gets the values of column i16
     int xrd, wrd[WK ? 1 : WF];
     const int trow = 8 * g + (i16 >> 2), tc = i16 & 3;
-    if constexpr (XK) xrd = (wm * 16 * XF + i16) * 128 + 16 * (g ^ x_swz(i16));
+    if constexpr (XK) xrd = (wm * 16 * XF + i16) * ROW + 16 * (g ^ x_swz(i16));
     else xrd = trow * 2 * BM + 16 * ((wm * 2 * XF + (tc >> 1)) ^ x_swz(trow)) + 8 * (tc & 1);
     if constexpr (WK) {
         const int r = 8 * (i16 >> 2) + (i16 & 3);
-        wrd[0] = WOFF + (wn * 16 * SH + r) * 128 + 16 * (g ^ w_swz(r));
+        wrd[0] = WOFF + (wn * 16 * SH + r) * ROW + 16 * (g ^ w_swz(r));
     } else {
         const int at = WOFF + trow * 2 * BN + 16 * ((wn * 2 * WF + tc) ^ w_swz(trow)) + 8 * (tc & 1);
 #pragma unroll
@@ -438,7 +442,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     }
     auto read_x = [&](const uint8_t* st, int h, int i) __attribute__((always_inline)) {
         if constexpr (XK) {
-            return *reinterpret_cast<const v8*>(st + (xrd ^ (64 * h)) + i * 16 * 128);
+            return *reinterpret_cast<const v8*>(st + (xrd ^ (64 * h)) + i * 16 * ROW);
         } else {
             const uint8_t* at = st + (xrd ^ (32 * i)) + 32 * h * 2 * BM;
             return read_transposed<v8>(at, 4 * 2 * BM);
@@ -447,7 +451,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     auto read_w = [&](const uint8_t* st, int h, int j) __attribute__((always_inline)) {
         if constexpr (WK) {
             return *reinterpret_cast<const v8*>(st + (wrd[0] ^ (64 * h)) +
-                                                ((j / SH) * TN + 32 * ((j % SH) >> 1) + 4 * (j & 1)) * 128);
+                                                ((j / SH) * TN + 32 * ((j % SH) >> 1) + 4 * (j & 1)) * ROW);
         } else {
             const uint8_t* at = st + wrd[j] + 32 * h * 2 * BN;
             return read_transposed<v8>(at, 4 * 2 * BN);
@@ -481,20 +485,27 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
 
     // ---- results
     // (lanes are taken anew, or the compiler keeps every address of it through the main loop and spills)
-    auto finish = [&](const TileAt& t) __attribute__((always_inline)) {
+    // WHOLE: all rows and columns of this wave are results, so nothing is asked and loads go out together.
+    auto results = [&](const TileAt& t, auto whole_) __attribute__((always_inline)) {
+        constexpr bool WHOLE = decltype(whole_)::value;
         int l = lane;
         asm volatile("" : "+v"(l));
         const int gg = l >> 4;
         const bool odd = !WK && (gg & 1);   // transposed reads: the two fragments of 8 columns in the other order
         const int c0 = t.n0 + wn * 16 * SH + 8 * gg;
+        const int r0 = wm * 16 * XF + (l & 15);
+        const int64_t at0 = (WG ? (int64_t)t.e * p.M + t.row0 : (int64_t)t.row0) + r0;
+        auto put = [&](auto* to, int n, const float (&f)[8]) __attribute__((always_inline)) {
+            if constexpr (WHOLE) stream8(to, f);
+            else store8(to, n, f);
+        };
 #pragma unroll
         for (int i = 0; i < XF; ++i) {
-            const int r = wm * 16 * XF + 16 * i + (l & 15);
-            if (r >= t.nrows) continue;
-            const int64_t row = t.row0 + r;
+            if (!WHOLE && r0 + 16 * i >= t.nrows) continue;
+            const int64_t row = at0 + 16 * i;
 #pragma unroll
             for (int q = 0; q < SH; q += 2) {
-                const int c = c0 + 16 * q, n = N - c;
+                const int c = c0 + 16 * q, n = WHOLE ? 8 : N - c;
                 if (n <= 0) continue;
                 float a[8], b[8], d[8];
 #pragma unroll
@@ -508,11 +519,11 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
                         b[v] = acc[i][SH + q + v / 4][v % 4];
                         d[v] = fast_silu(a[v]) * b[v];
                     }
-                    store8(static_cast<T*>(p.y) + row * N + c, n, d);
+                    put(static_cast<T*>(p.y) + row * N + c, n, d);
                     if (p.pre_out) {
                         T* pre = static_cast<T*>(p.pre_out) + row * 2 * N + c;
-                        store8(pre, n, a);
-                        store8(pre + N, n, b);
+                        put(pre, n, a);
+                        put(pre + N, n, b);
                     }
                 } else if constexpr (KIND == G_SWIGLU_GRAD) {
                     const T* pre = static_cast<const T*>(p.pre_in) + row * 2 * N + c;
@@ -522,24 +533,22 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
 #pragma unroll
                     for (int v = 0; v < 8; ++v) swiglu_grad(a[v], b[v], d[v], &a[v], &d[v], &z[v]);
                     T* to = static_cast<T*>(p.y) + row * 2 * N + c;
-                    store8(to, n, a);
-                    store8(to + N, n, d);
-                    if (p.z) store8(static_cast<T*>(p.z) + row * N + c, n, z);
-                } else if constexpr (WG) {
-                    O* y = static_cast<O*>(p.y) + ((int64_t)t.e * p.M + row) * N + c;
-                    if (p.accumulate) {
+                    put(to, n, a);
+                    put(to + N, n, d);
+                    if (p.z) put(static_cast<T*>(p.z) + row * N + c, n, z);
+                } else {
+                    O* y = static_cast<O*>(p.y) + row * N + c;
+                    if (WG && p.accumulate) {
                         load8(y, n, b);
 #pragma unroll
                         for (int v = 0; v < 8; ++v) a[v] += b[v];
                     }
-                    store8(y, n, a);
-                } else {
-                    store8(static_cast<O*>(p.y) + row * N + c, n, a);
+                    put(y, n, a);
                 }
             }
         }
     };
-    // memory instructions that finish() issues at least for a tile whose rows and columns of this wave are whole
+    // memory instructions of the results at least, where this wave's rows and columns are whole
     constexpr int STORES = XF * (GU ? SH / 2 : KIND == G_SWIGLU_GRAD ? 4 * SH / 2 : (int)sizeof(O) / 2 * SH / 2);
     auto whole = [&](const TileAt& t) __attribute__((always_inline)) {
         return t.nrows >= (wm + 1) * 16 * XF && t.n0 + TN <= N;
@@ -575,26 +584,47 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     for (int j = 0; j < WF; ++j) fa.w[j] = read_w(ring, 0, j);
 #pragma unroll
     for (int i = 1; i < XF; ++i) fa.x[i] = read_x(ring, 0, i);
-    while (true) {
-        describe();
-        mma(fa, fb, ring + slot * STAGE, 1, false, 0);
-        // this wave's loads of the next stage have landed, then every wave's; and every wave has read this stage
-        // (after a whole tile's stores, which are younger, they may be in flight too)
+    // What a stage's barrier waits for: this wave's loads of the next stage have landed, then every wave's; and every
+    // wave has read this stage (after a whole tile's stores, which are younger, they may be in flight too).
+    auto meet = [&]() __attribute__((always_inline)) {
         if constexpr (DMA) {
             if (stored) wait_vmcnt<std::min(60, (NS - 2) * LPW + STORES)>();
             else wait_vmcnt<(NS - 2) * LPW>();
             stored = max(0, stored - 1);
         }
         lds_barrier();
+    };
+    // The step that reads the next stage's first fragments into `n` and refills this stage's slot; whether this stage
+    // was its tile's last.
+    auto turn = [&](const Frags& f, Frags& n) __attribute__((always_inline)) {
         const int next = slot == NS - 1 ? 0 : slot + 1;
+        mma(f, n, ring + next * STAGE, 0, true, slot);
         const bool done = uni((int)(last >> slot)) & 1;
-        mma(fb, fa, ring + next * STAGE, 0, true, slot);
         advance(slot);
         if constexpr (!DMA) fetch();
         slot = next;
-        if (!done) continue;
-        finish(cur);
-        stored = whole(cur) ? NS - 1 : 0;
+        return done;
+    };
+    while (true) {
+        describe();
+        if constexpr (KB == 64) {
+            mma(fa, fb, ring + slot * STAGE, 1, false, 0);
+            meet();
+            if (!turn(fb, fa)) continue;
+        } else {
+            meet();
+            if (turn(fa, fb)) {
+                fa = fb;
+            } else {
+                describe();
+                meet();
+                if (!turn(fb, fa)) continue;
+            }
+        }
+        const bool all = whole(cur);
+        if (all) results(cur, std::true_type{});
+        else results(cur, std::false_type{});
+        stored = all ? NS - 1 : 0;
         cj += step;
         if (cj >= jend) break;
         cur = tile_at(cj);
@@ -617,7 +647,7 @@ int cu_count() {
 }
 
 // per_cu workgroups share a CU (their LDS)
-template <int WMC, int WNC, int XF, int WF, int NS, bool DMA, GKind KIND, bool WK, typename T, typename O>
+template <int WMC, int WNC, int XF, int WF, int KB, int NS, bool DMA, GKind KIND, bool WK, typename T, typename O>
 int launch(const GProduct& p, hipStream_t s) {
     constexpr int BM = 16 * XF * WMC, BN = 16 * WF * WNC, TN = KIND == G_SWIGLU ? BN / 2 : BN;
     const int64_t n = (p.N + TN - 1) / TN;
@@ -625,17 +655,17 @@ int launch(const GProduct& p, hipStream_t s) {
                       : p.offsets           ? p.rows / BM + std::min((int64_t)p.groups, p.rows)
                                             : (p.rows + BM - 1) / BM;
     if (m * n > INT_MAX / 2) return HM_ERR_OVERFLOW;
-    const int64_t slots = (int64_t)cu_count() / kXcds * (NS * 128 * (BM + BN) > 76 * 1024 ? 1 : 2);
+    const int64_t slots = (int64_t)cu_count() / kXcds * (NS * 2 * KB * (BM + BN) > 76 * 1024 ? 1 : 2);
     const int64_t grid = kXcds * std::min((m * n + kXcds - 1) / kXcds, slots);
-    hipLaunchKernelGGL((g_tile_kernel<WMC, WNC, XF, WF, NS, DMA, KIND, WK, T, O>), dim3((unsigned)grid),
+    hipLaunchKernelGGL((g_tile_kernel<WMC, WNC, XF, WF, KB, NS, DMA, KIND, WK, T, O>), dim3((unsigned)grid),
                        dim3(64 * WMC * WNC), 0, s, p);
     HM_LAUNCHED();
     return HM_OK;
 }
 
-template <int WMC, int WNC, int XF, int WF, int NS, bool DMA, typename T>
+template <int WMC, int WNC, int XF, int WF, int KB, int NS, bool DMA, typename T>
 int launch_kind(GKind kind, bool wk, bool f32, const GProduct& p, hipStream_t s) {
-#define HM_G(KIND, WK, O) launch<WMC, WNC, XF, WF, NS, DMA, KIND, WK, T, O>(p, s)
+#define HM_G(KIND, WK, O) launch<WMC, WNC, XF, WF, KB, NS, DMA, KIND, WK, T, O>(p, s)
     switch (kind) {
     case G_SWIGLU: return HM_G(G_SWIGLU, true, T);
     case G_SWIGLU_GRAD: return HM_G(G_SWIGLU_GRAD, false, T);
@@ -650,10 +680,10 @@ int launch_kind(GKind kind, bool wk, bool f32, const GProduct& p, hipStream_t s)
 
 template <typename T>
 int launch_tiles(int form, GKind kind, bool wk, bool f32, const GProduct& p, hipStream_t s) {
-    if (form == 256) return launch_kind<2, 4, 8, 4, 2, true, T>(kind, wk, f32, p, s);
-    if (form == 128) return launch_kind<2, 4, 4, 4, 3, true, T>(kind, wk, f32, p, s);
-    if (form == 64) return launch_kind<2, 2, 4, 4, 2, true, T>(kind, wk, f32, p, s);
-    return launch_kind<2, 2, 4, 4, 2, false, T>(kind, wk, f32, p, s);
+    if (form == 256) return launch_kind<2, 4, 8, 4, 64, 2, true, T>(kind, wk, f32, p, s);
+    if (form == 128) return launch_kind<2, 4, 4, 4, 64, 3, true, T>(kind, wk, f32, p, s);
+    if (form == 64) return launch_kind<2, 2, 4, 4, 64, 2, true, T>(kind, wk, f32, p, s);
+    return launch_kind<2, 2, 4, 4, 64, 2, false, T>(kind, wk, f32, p, s);
 }
 
 }  // namespace
