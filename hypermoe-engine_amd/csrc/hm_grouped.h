@@ -117,17 +117,29 @@ __device__ __forceinline__ u64x2 load16(const void* p) {
 
 // 8 values to a place aligned to their element, past the L2's other contents (a result is larger than the L2 by far, and
 // what the L2 holds is read again: weight gradients of 128 groups, 805 MB of results, 435 us without the hint, 303 with).
+__device__ __forceinline__ void stream16(void* p, u64x2 v) {
+    typedef uint64_t loose __attribute__((ext_vector_type(2), aligned(2)));
+    __builtin_nontemporal_store(v, (__attribute__((address_space(1))) loose*)p);
+}
+template <typename T>
+__device__ __forceinline__ u64x2 pack8(const float (&f)[8]) {
+    Loose8<T> w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w.v[i] = (T)f[i];
+    return __builtin_bit_cast(u64x2, w);
+}
 template <typename T>
 __device__ __forceinline__ void stream8(T* p, const float (&f)[8]) {
-    typedef uint64_t loose __attribute__((ext_vector_type(2), aligned(2)));
-    if constexpr (sizeof(T) == 2) {
-        Loose8<T> w;
+    if constexpr (sizeof(T) == 2) stream16(p, pack8<T>(f));
+    else store8(p, 8, f);
+}
+// The value of the lane 8 further in its 16 (DPP row_ror:8).
+__device__ __forceinline__ u64x2 other8(u64x2 v) {
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    i32x4 w = __builtin_bit_cast(i32x4, v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w.v[i] = (T)f[i];
-        __builtin_nontemporal_store(__builtin_bit_cast(u64x2, w), (__attribute__((address_space(1))) loose*)p);
-    } else {
-        store8(p, 8, f);
-    }
+    for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_update_dpp(0, w[i], 0x128, 0xF, 0xF, false);
+    return __builtin_bit_cast(u64x2, w);
 }
 
 // n values (8 at most) of a row as a fragment's 8, zeros behind them.

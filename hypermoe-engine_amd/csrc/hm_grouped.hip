@@ -319,8 +319,11 @@ static int pick(GKind kind, bool w_kmajor, const GProduct& p) {
     const int wide = kind == G_SWIGLU ? 128 : 256;   // (gate and up share a tile)
     if (m128 * ((p.N + wide - 1) / wide) < 256) return 64;
     // 256 x 256 from 384 rows a group on: 8 groups of 4096 rows, 2048 x 1536, 195 us against 219 of 128 x 256; but 128
-    // of 256 rows on average, uneven, 196 and 164: half of the second tile of a group is empty.
-    return wg || each >= 384 ? 256 : 128;
+    // of 256 rows on average, uneven, 182 and 157: half of the second tile of a group is empty.  Gate and up from 256 on
+    // (those groups 289 and 297).  The SwiGLU's gradient not at all: its results take more time than the matrix
+    // instructions, and 128 x 256 tiles spread them better (8 groups of 4096 rows, 2048 x 768, 171 us and 157).
+    if (kind == G_SWIGLU_GRAD) return 128;
+    return wg || each >= (kind == G_SWIGLU ? 256 : 384) ? 256 : 128;
 }
 
 int hm_g_launch(GKind kind, bool w_kmajor, int32_t dtype, int32_t y_dtype, const GProduct& p_, hipStream_t s) {

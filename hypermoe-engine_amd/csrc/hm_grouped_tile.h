@@ -1,11 +1,11 @@
 // hm_grouped_tile.h -- tiles of the 16-bit products (hm_grouped.h) through an LDS ring; one source for each type
 // (hm_grouped_tile_f16.hip, hm_grouped_tile_bf16.hip).
 //
-// Persistent workgroups of 4 waves, 2 (rows of x) x 2 (columns); a wave owns 16 XF x 16 WF results, a tile is
-// BM = 32 XF rows x BN = 32 WF columns.  A stage is 64 of k of both operands, 128 (BM + BN) bytes, moved to the
-// LDS by DMA; the stages of consecutive tiles form one stream, so a tile's first stages load while its
-// predecessor ends.  A stage is two steps of 32 k.  A step multiplies fragments that the step before read from
-// the LDS, so no matrix instruction waits for the LDS; between the two steps lies the one barrier of a stage:
+// Persistent workgroups of WMC (rows of x) x WNC (columns) waves; a wave owns 16 XF x 16 WF results, a tile is BM = 16 XF
+// WMC rows x BN = 16 WF WNC columns.  A stage is KB = 64 of k of both operands, 128 (BM + BN) bytes, moved to the LDS by
+// DMA (operands off 16 bytes: through registers); the stages of consecutive tiles form one stream, so a tile's first
+// stages load while its predecessor ends.  A stage is two steps of 32 k.  A step multiplies fragments that the step before
+// read from the LDS, so no matrix instruction waits for the LDS; between the two steps lies the one barrier of a stage:
 // the next stage has landed, and this one, which every wave now has in registers, is refilled.
 //   k-major operand   LDS row r is 64 k of one row; its 16-byte piece c sits at position c ^ s(r), and s
 //                     separates the 16 rows that a read takes of one piece.
@@ -33,6 +33,7 @@ namespace {
 constexpr int kXcds = 8;
 constexpr int kThreads = 256;
 constexpr int kSuper = 4;
+constexpr int KB = 64;
 
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 template <typename P>
@@ -49,7 +50,7 @@ struct TileAt {
     int nb;             // stages of k
 };
 
-template <int WMC, int WNC, int XF, int WF, int KB, int NS, bool DMA, GKind KIND, bool WK, typename T, typename O>
+template <int WMC, int WNC, int XF, int WF, int NS, bool DMA, GKind KIND, bool WK, typename T, typename O>
 __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     typedef typename Elem16<T>::v8 v8;
     constexpr bool WG = KIND == G_WEIGHT_GRAD, XK = !WG, GU = KIND == G_SWIGLU;
@@ -57,7 +58,6 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     constexpr int ROW = 2 * KB, RPB = 1024 / ROW, PCS = KB / 8;   // a k-major row's bytes, rows in 1 KB, pieces
     constexpr int STAGE = ROW * (BM + BN), WOFF = ROW * BM;
     constexpr int XL = BM / RPB / NW, LPW = (BM + BN) / RPB / NW;   // a wave's 1 KB loads a stage, of x first
-    static_assert(KB == 64 || (KB == 32 && DMA), "stage");
     static_assert(RPB * NW <= 64, "ids");
     static_assert(DMA || NW == 4, "fetch() takes the swizzles to be the same for every c");
     static_assert(XF % 2 == 0 && (SH == 2 || SH == 4 || SH == 8) && BM % (RPB * NW) == 0 && BN % (RPB * NW) == 0, "tile");
@@ -193,11 +193,11 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     int left = 0;              // k from the stage's first on
     int xcols = 0, wcols = 0;  // without DMA, operands that are not k-major: columns from this lane's on
     auto x_swz = [](int r) __attribute__((always_inline)) {
-        if constexpr (XK) return KB == 64 ? (r >> 1) & 7 : (r >> 2) & 3;
+        if constexpr (XK) return (r >> 1) & 7;
         return ((r & 3) << 1) | (r & 8);
     };
     auto w_swz = [](int r) __attribute__((always_inline)) {
-        if constexpr (WK) return KB == 64 ? ((r >> 1) & 1) | (((r >> 3) & 3) << 1) : (r >> 3) & 3;
+        if constexpr (WK) return ((r >> 1) & 1) | (((r >> 3) & 3) << 1);
         return (r & 1) | ((r & 2) << 1) | (r & 8);
     };
     // byte offset of the row of x that tile row r reads (from xbase)
@@ -495,14 +495,30 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
         const int c0 = t.n0 + wn * 16 * SH + 8 * gg;
         const int r0 = wm * 16 * XF + (l & 15);
         const int64_t at0 = (WG ? (int64_t)t.e * p.M + t.row0 : (int64_t)t.row0) + r0;
-        auto put = [&](auto* to, int n, const float (&f)[8]) __attribute__((always_inline)) {
-            if constexpr (WHOLE) stream8(to, f);
-            else store8(to, n, f);
+        // PAIR: a lane's two pieces of a row are 32 values apart, and four lanes' pieces 64 bytes.  Lanes i and i + 8 trade
+        // one, so that a store takes 8 whole rows of 128 bytes instead of 16 halves.
+        constexpr bool PAIR = WHOLE && SH == 4 && sizeof(O) == 2;
+        const bool high = l & 8;
+        auto put = [&](auto* to, int64_t ld, int n, int q, const float (&f)[8], u64x2& kept) __attribute__((always_inline)) {
+            typedef std::remove_pointer_t<decltype(to)> E;
+            if constexpr (!WHOLE) {
+                store8(to, n, f);
+            } else if constexpr (!PAIR) {
+                stream8(to, f);
+            } else if (q == 0) {
+                kept = pack8<E>(f);
+            } else {
+                // (`to` is this row's second piece, `ld` what lies between rows)
+                const u64x2 second = pack8<E>(f), got = other8(high ? kept : second);
+                stream16(to + (high ? -8 * ld : -32), high ? got : kept);
+                stream16(to + (high ? 0 : 8 * ld - 32), high ? second : got);
+            }
         };
 #pragma unroll
         for (int i = 0; i < XF; ++i) {
             if (!WHOLE && r0 + 16 * i >= t.nrows) continue;
             const int64_t row = at0 + 16 * i;
+            u64x2 k0, k1, k2;
 #pragma unroll
             for (int q = 0; q < SH; q += 2) {
                 const int c = c0 + 16 * q, n = WHOLE ? 8 : N - c;
@@ -519,11 +535,11 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
                         b[v] = acc[i][SH + q + v / 4][v % 4];
                         d[v] = fast_silu(a[v]) * b[v];
                     }
-                    put(static_cast<T*>(p.y) + row * N + c, n, d);
+                    put(static_cast<T*>(p.y) + row * N + c, N, n, q, d, k0);
                     if (p.pre_out) {
                         T* pre = static_cast<T*>(p.pre_out) + row * 2 * N + c;
-                        put(pre, n, a);
-                        put(pre + N, n, b);
+                        put(pre, 2 * N, n, q, a, k1);
+                        put(pre + N, 2 * N, n, q, b, k2);
                     }
                 } else if constexpr (KIND == G_SWIGLU_GRAD) {
                     const T* pre = static_cast<const T*>(p.pre_in) + row * 2 * N + c;
@@ -533,9 +549,9 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
 #pragma unroll
                     for (int v = 0; v < 8; ++v) swiglu_grad(a[v], b[v], d[v], &a[v], &d[v], &z[v]);
                     T* to = static_cast<T*>(p.y) + row * 2 * N + c;
-                    put(to, n, a);
-                    put(to + N, n, d);
-                    if (p.z) put(static_cast<T*>(p.z) + row * N + c, n, z);
+                    put(to, 2 * N, n, q, a, k0);
+                    put(to + N, 2 * N, n, q, d, k1);
+                    if (p.z) put(static_cast<T*>(p.z) + row * N + c, N, n, q, z, k2);
                 } else {
                     O* y = static_cast<O*>(p.y) + row * N + c;
                     if (WG && p.accumulate) {
@@ -543,7 +559,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
 #pragma unroll
                         for (int v = 0; v < 8; ++v) a[v] += b[v];
                     }
-                    put(y, n, a);
+                    put(y, N, n, q, a, k0);
                 }
             }
         }
@@ -607,20 +623,9 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
     };
     while (true) {
         describe();
-        if constexpr (KB == 64) {
-            mma(fa, fb, ring + slot * STAGE, 1, false, 0);
-            meet();
-            if (!turn(fb, fa)) continue;
-        } else {
-            meet();
-            if (turn(fa, fb)) {
-                fa = fb;
-            } else {
-                describe();
-                meet();
-                if (!turn(fb, fa)) continue;
-            }
-        }
+        mma(fa, fb, ring + slot * STAGE, 1, false, 0);
+        meet();
+        if (!turn(fb, fa)) continue;
         const bool all = whole(cur);
         if (all) results(cur, std::true_type{});
         else results(cur, std::false_type{});
@@ -647,7 +652,7 @@ int cu_count() {
 }
 
 // per_cu workgroups share a CU (their LDS)
-template <int WMC, int WNC, int XF, int WF, int KB, int NS, bool DMA, GKind KIND, bool WK, typename T, typename O>
+template <int WMC, int WNC, int XF, int WF, int NS, bool DMA, GKind KIND, bool WK, typename T, typename O>
 int launch(const GProduct& p, hipStream_t s) {
     constexpr int BM = 16 * XF * WMC, BN = 16 * WF * WNC, TN = KIND == G_SWIGLU ? BN / 2 : BN;
     const int64_t n = (p.N + TN - 1) / TN;
@@ -657,33 +662,41 @@ int launch(const GProduct& p, hipStream_t s) {
     if (m * n > INT_MAX / 2) return HM_ERR_OVERFLOW;
     const int64_t slots = (int64_t)cu_count() / kXcds * (NS * 2 * KB * (BM + BN) > 76 * 1024 ? 1 : 2);
     const int64_t grid = kXcds * std::min((m * n + kXcds - 1) / kXcds, slots);
-    hipLaunchKernelGGL((g_tile_kernel<WMC, WNC, XF, WF, KB, NS, DMA, KIND, WK, T, O>), dim3((unsigned)grid),
+    hipLaunchKernelGGL((g_tile_kernel<WMC, WNC, XF, WF, NS, DMA, KIND, WK, T, O>), dim3((unsigned)grid),
                        dim3(64 * WMC * WNC), 0, s, p);
     HM_LAUNCHED();
     return HM_OK;
 }
 
-template <int WMC, int WNC, int XF, int WF, int KB, int NS, bool DMA, typename T>
+template <int WMC, int WNC, int XF, int WF, int NS, bool DMA, typename T>
 int launch_kind(GKind kind, bool wk, bool f32, const GProduct& p, hipStream_t s) {
-#define HM_G(KIND, WK, O) launch<WMC, WNC, XF, WF, KB, NS, DMA, KIND, WK, T, O>(p, s)
+#define HM_G(KIND, WK, O) launch<WMC, WNC, XF, WF, NS, DMA, KIND, WK, T, O>(p, s)
     switch (kind) {
-    case G_SWIGLU: return HM_G(G_SWIGLU, true, T);
-    case G_SWIGLU_GRAD: return HM_G(G_SWIGLU_GRAD, false, T);
+    case G_SWIGLU:
+        if constexpr (XF * WMC * 16 < 256 && WNC == 2) return HM_G(G_SWIGLU, true, T);
+        break;   // (launch_tiles has their own)
+    case G_SWIGLU_GRAD:
+        if constexpr (XF * WMC * 16 < 256) return HM_G(G_SWIGLU_GRAD, false, T);
+        break;   // (hm_grouped.hip asks for none)
     case G_WEIGHT_GRAD: return f32 ? HM_G(G_WEIGHT_GRAD, false, float) : HM_G(G_WEIGHT_GRAD, false, T);
     case G_ADAPTER: return wk ? HM_G(G_ADAPTER, true, T) : HM_G(G_ADAPTER, false, T);
-    default: break;
+    case G_MATMUL:
+        if (wk) return f32 ? HM_G(G_MATMUL, true, float) : HM_G(G_MATMUL, true, T);
+        return f32 ? HM_G(G_MATMUL, false, float) : HM_G(G_MATMUL, false, T);
     }
-    if (wk) return f32 ? HM_G(G_MATMUL, true, float) : HM_G(G_MATMUL, true, T);
-    return f32 ? HM_G(G_MATMUL, false, float) : HM_G(G_MATMUL, false, T);
+    return HM_ERR_UNSUPPORTED;
 #undef HM_G
 }
 
 template <typename T>
 int launch_tiles(int form, GKind kind, bool wk, bool f32, const GProduct& p, hipStream_t s) {
-    if (form == 256) return launch_kind<2, 4, 8, 4, 64, 2, true, T>(kind, wk, f32, p, s);
-    if (form == 128) return launch_kind<2, 4, 4, 4, 64, 3, true, T>(kind, wk, f32, p, s);
-    if (form == 64) return launch_kind<2, 2, 4, 4, 64, 2, true, T>(kind, wk, f32, p, s);
-    return launch_kind<2, 2, 4, 4, 64, 2, false, T>(kind, wk, f32, p, s);
+    // (gate and up: waves of twice the columns, whose results then fill lines)
+    if (form == 256 && kind == G_SWIGLU) return launch<4, 2, 4, 8, 2, true, G_SWIGLU, true, T, T>(p, s);
+    if (form == 128 && kind == G_SWIGLU) return launch<4, 2, 2, 8, 3, true, G_SWIGLU, true, T, T>(p, s);
+    if (form == 256) return launch_kind<2, 4, 8, 4, 2, true, T>(kind, wk, f32, p, s);
+    if (form == 128) return launch_kind<2, 4, 4, 4, 3, true, T>(kind, wk, f32, p, s);
+    if (form == 64) return launch_kind<2, 2, 4, 4, 2, true, T>(kind, wk, f32, p, s);
+    return launch_kind<2, 2, 4, 4, 2, false, T>(kind, wk, f32, p, s);
 }
 
 }  // namespace

@@ -20,7 +20,7 @@ CASES = (
     [(128, k, _MANY, inner, cols, 0, 1) for k, inner, cols in
      ((MATMUL, 200, 520), (TRANSPOSED, 136, 776), (SWIGLU, 72, 264), (SWIGLU_GRAD, 328, 520))] +
     [(256, k, _BIG * 2, inner, cols, 0, 1) for k, inner, cols in
-     ((MATMUL, 264, 2312), (TRANSPOSED, 200, 2064), (SWIGLU, 136, 1160), (SWIGLU_GRAD, 72, 2056))] +
+     ((MATMUL, 264, 2312), (TRANSPOSED, 200, 2064), (SWIGLU, 136, 1160))] + [(128, SWIGLU_GRAD, _BIG * 2, 72, 2056, 0, 1)] +
     [(256, WEIGHT_GRAD, [5, 0, 64, 65, 300, 1] * 8, 776, 648, 0, 1), (64, WEIGHT_GRAD, [5, 0, 64, 65, 300], 200, 136, 0, 1)] +
     [(64, k, [70, 0, 257, 3, 128, 129, 40], inner, cols, 0, 1) for k, inner, cols in
      ((MATMUL, 200, 136), (TRANSPOSED, 328, 264), (SWIGLU, 72, 200), (SWIGLU_GRAD, 520, 264))] +
