@@ -100,6 +100,7 @@ __global__ __launch_bounds__(kThreads) void grouped_generic_kernel(GProduct p) {
     w += KIND == G_WEIGHT_GRAD ? 0 : (int64_t)e * p.w_group;
 
     v4f acc[2][2] = {};
+    int named = 0;   // adapters that the tile's rows name
     auto step = [&]() __attribute__((always_inline)) {
         __syncthreads();
         v8 a[2], b[2];
@@ -171,6 +172,7 @@ __global__ __launch_bounds__(kThreads) void grouped_generic_kernel(GProduct p) {
                 for (int m = 32; m >= 1; m >>= 1) next = min(next, __shfl_xor(next, m, 64));
                 if (next == INT_MAX) break;
                 cur = next;
+                ++named;
                 const T* upm = static_cast<const T*>(p.up) + (int64_t)cur * p.N * p.rank;
                 const int r = t >> 2;
                 const bool take = __shfl(mine, r & 63, 64) == cur && r < nrows;
@@ -223,7 +225,11 @@ __global__ __launch_bounds__(kThreads) void grouped_generic_kernel(GProduct p) {
                     O* y = static_cast<O*>(p.y) + ((int64_t)e * p.M + row) * p.N + c;
                     *y = (O)(acc[i][j][v] + (p.accumulate ? (float)*y : 0.0f));
                 } else {
-                    static_cast<O*>(p.y)[row * p.N + c] = (O)acc[i][j][v];
+                    float r = acc[i][j][v];
+                    if constexpr (KIND == G_ADAPTER) {
+                        if (named && r * 0.0f != 0.0f) r = adapter_result<T, WK>(p, row, c);
+                    }
+                    static_cast<O*>(p.y)[row * p.N + c] = (O)r;
                 }
             }
     }
@@ -288,11 +294,12 @@ int hm_g_launch_generic(GKind kind, bool w_kmajor, int32_t dtype, int32_t y_dtyp
 
 // Whether a product fits the tile kernels: offsets from a tile's first row (x's first row where rows are gathered)
 // stay below HM_BUF_RANGE.
-static bool tile_ok(GKind kind, const GProduct& p) {
+static bool tile_ok(GKind kind, bool w_kmajor, const GProduct& p) {
     const int64_t top = HM_BUF_RANGE;
+    const int64_t wide = (int64_t)1 << 24;   // columns, of which a stage has 64 rows
     if (p.rows > INT_MAX - 256) return false;
-    if (kind == G_WEIGHT_GRAD) return true;
-    if (p.K > (int64_t)1 << 22) return false;
+    if (kind == G_WEIGHT_GRAD) return p.M <= wide && p.N <= wide;
+    if (p.K > (int64_t)1 << 22 || (!w_kmajor && p.N > wide)) return false;
     return kind != G_SWIGLU || ((p.N + 256) * p.K * 2 < top && (!p.perm || p.x_rows * p.K * 2 < top));
 }
 
@@ -310,7 +317,7 @@ static int pick(GKind kind, bool w_kmajor, const GProduct& p) {
     const int64_t groups = p.offsets ? p.groups : 1, each = (p.rows + groups - 1) / groups;
     if (nt && (each <= 16 || p.rows <= 64)) return (p.rows <= 16 || each <= 4 ? 1 : p.rows <= 32 || each <= 8 ? 2 : 4) << 16;
     if (kind == G_ADAPTER && nt && p.rows <= 128) return 8 << 16;
-    if (!tile_ok(kind, p)) return 0;
+    if (!tile_ok(kind, w_kmajor, p)) return 0;
     const bool wg = kind == G_WEIGHT_GRAD;
     const int64_t m128 = wg ? p.groups * ((p.M + 127) / 128) : p.rows / 128 + groups;
     // Off 16 bytes (128 x 128 tiles through registers against the generic kernel's 64 x 64): 16 groups of 512 rows,

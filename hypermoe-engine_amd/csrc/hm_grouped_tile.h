@@ -181,6 +181,7 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
             const int hi = p.offsets ? uni((int)min((int64_t)p.offsets[t.e + 1], p.rows)) : (int)p.rows;
             t.row0 = lo + m * BM;
             t.nrows = min(BM, hi - t.row0);
+            if (m < 0 || r < 0) t.row0 = lo, t.nrows = 0, t.n0 = N;   // (offsets of no batch: counts past 32 bits)
             t.k0 = 0;
             t.kn = K;
             t.nb = (K + KB - 1) / KB;
@@ -501,6 +502,17 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
         const int c0 = t.n0 + wn * 16 * SH + 8 * gg;
         const int r0 = wm * 16 * XF + (l & 15);
         const int64_t at0 = (WG ? (int64_t)t.e * p.M + t.row0 : (int64_t)t.row0) + r0;
+        // whether the tile's rows name another adapter than this row's
+        auto named_other = [&](int64_t row) __attribute__((always_inline)) {
+            const int own = p.ids[row];
+            bool other = false;
+#pragma unroll 1
+            for (int r = 0; r < t.nrows; ++r) {
+                const int id = p.ids[t.row0 + r];
+                other = other || (id != own && id >= 0 && id < p.adapters);
+            }
+            return other;
+        };
         // PAIR: a lane's two pieces of a row are 32 values apart, and four lanes' pieces 64 bytes.  Lanes i and i + 8 trade
         // one, so that a store takes 8 whole rows of 128 bytes instead of 16 halves.
         constexpr bool PAIR = WHOLE && SH == 4 && sizeof(O) == 2;
@@ -560,6 +572,19 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
                     if (p.z) put(static_cast<T*>(p.z) + row * N + c, N, n, q, z, k2);
                 } else {
                     O* y = static_cast<O*>(p.y) + row * N + c;
+                    if constexpr (KIND == G_ADAPTER) {
+                        float bad = 0.0f;
+#pragma unroll
+                        for (int v = 0; v < 8; ++v) bad = __builtin_fmaf(a[v], 0.0f, bad);
+                        if (bad != 0.0f && named_other(row)) {
+#pragma unroll 1
+                            for (int v = 0; v < min(n, 8); ++v) {
+                                const float e = adapter_result<T, WK>(p, row, c + v);
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) a[k] = k == v ? e : a[k];
+                            }
+                        }
+                    }
                     if (WG && p.accumulate) {
                         load8(y, n, b);
 #pragma unroll

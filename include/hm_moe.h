@@ -551,7 +551,8 @@ int hm_grouped_weight_grad(const void* dy, const void* x, int32_t dtype,
  * mid and x, B's of dy and mid.  Zeros for an adapter without rows; accumulate,
  * dw_dtype and workspace as F4's.  mid and y must not overlap anything.  Rank
  * up to 256, up to 65535 adapters and 2^23 - 1 rows.
- * Rows of one adapter side by side are fastest. */
+ * Rows of one adapter side by side are fastest.  An infinity or a NaN in an
+ * adapter's matrices reaches the rows of that adapter only. */
 #define HM_ADAPTER_MAX_RANK 256
 int hm_adapter_matmul(const void* x, int32_t dtype, const void* w,
                       int32_t w_transposed, const void* down, const void* up,

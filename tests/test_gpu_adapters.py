@@ -198,3 +198,49 @@ def test_infinities_stay_in_their_rows(dev, dtype):
         assert not np.isfinite(y[4]).all()
         assert np.isfinite(np.delete(y, 4, axis=0)).all() and np.isfinite(got["dx"].double().cpu().numpy()).all()
         assert not got["da"][2:].any() and not got["db"][2:].any()
+
+
+@pytest.mark.parametrize("transposed", [False, True], ids=["nt", "nn"])
+@pytest.mark.parametrize("value", ["inf", "nan"])
+@pytest.mark.parametrize("rows,inner,cols,rank", [(9, 64, 40, 8), (70, 72, 136, 16), (200, 72, 520, 16), (150, 77, 141, 5),
+                                                  (2100, 137, 1301, 9), (700, 64, 25000, 8), (4200, 72, 4104, 16)])
+def test_an_adapters_infinity_stays_with_its_rows(dev, dtype, rows, inner, cols, rank, value, transposed):
+    """An adapter whose matrices hold an infinity or a NaN is its own rows' affair, in every kernel, also where its rows
+    and others share a tile; its own rows show it."""
+    from hmoe import adapters
+    torch = dev.torch
+    g = torch.Generator(device="cuda")
+    g.manual_seed(rows)
+
+    def make(*shape, std=1.0):
+        return torch.empty(shape, dtype=R.torch_type(torch, dtype), device="cuda").normal_(0, std, generator=g)
+    n = 4
+    x = make(rows, inner)
+    w = make(*((inner, cols) if transposed else (cols, inner)), std=inner ** -0.5)
+    down = make(n, *((inner, rank) if transposed else (rank, inner)), std=inner ** -0.5)
+    up = make(n, *((rank, cols) if transposed else (cols, rank)), std=0.3)
+    scale = torch.ones(n, device="cuda")
+    ids = (torch.arange(rows, device="cuda", dtype=torch.int32) // 3 % 5 - 1).contiguous()
+    clean, mid = adapters.matmul(x, w, down, up, scale, ids, transposed=transposed)
+    column = cols - 2
+    up[(1, 0, column) if transposed else (1, column, 0)] = float(value)
+    down[2] = float(value)
+    y, mid2 = adapters.matmul(x, w, down, up, scale, ids, transposed=transposed)
+    other = (ids != 1) & (ids != 2)
+    assert torch.equal(mid2[ids != 2], mid[ids != 2]) and not torch.isfinite(mid2[ids == 2]).any()
+    assert not torch.isfinite(y[ids == 2]).any() and not torch.isfinite(y[ids == 1][:, column]).any()
+    # sums in another order where a result was taken again: both are within the bound of the same sum
+    wt, ut = (w, up) if transposed else (w.t(), up.transpose(1, 2))
+    size = torch.mm(x.double().abs(), wt.double().abs().contiguous())
+    for a in (0, 1, 3):
+        at = ids == a
+        u = ut[a].double().abs()
+        u[:, column] = torch.where(torch.isfinite(u[:, column]), u[:, column], 0.0)
+        size[at] += torch.mm(mid[at].double().abs(), u.contiguous())
+    keep = torch.ones(cols, dtype=torch.bool, device="cuda")
+    keep[column] = False
+    for at, some in ((other, slice(None)), (ids == 1, keep)):
+        a, b = y[at][:, some].double(), clean[at][:, some].double()
+        tol = 2 * R.sum_error(inner + rank, size[at][:, some])
+        tol = tol + 2 * R.HALF[dtype] * (b.abs() + tol) + R.TINY[dtype]
+        assert bool(((a - b).abs() <= tol).all())

@@ -188,6 +188,8 @@ def test_wide_operands(dev):
     # (the worst case, (k + 16) U size, says nothing for so long a sum.  Partial sums grow as the root of their length,
     # so roundings of U / 2 of them add up, as independent ones do, to U k / 4 or so: under U size; 16 times that)
     assert bool(((y.double() - want).abs() <= 16 * R.U * size).all())
+    assert capi.load().hm_debug_grouped_form(TRANSPOSED, 1, 70, 64, (1 << 24) + 8, 0, 1) == 0
+    assert capi.load().hm_debug_grouped_form(WEIGHT_GRAD, 1, 70, 64, (1 << 24) + 8, 0, 1) == 0
     tokens, h = 1 << 20, 2048
     x = torch.zeros(tokens, h, dtype=torch.bfloat16, device="cuda")
     perm = torch.randint(0, tokens, (300,), generator=g, device="cuda", dtype=torch.int32)
