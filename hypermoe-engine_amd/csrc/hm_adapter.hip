@@ -2,6 +2,8 @@
 //   mid[t] = s_a x[t] A_a^T,  y[t] = x[t] W^T + mid[t] B_a^T,  a = ids[t]
 // the input's gradient by the same entry point with the matrices transposed, and the adapters' gradients
 //   d_a = sum over the rows t of adapter a of  left[t]^T right[t].
+// mid is held in the operands' 16 bits: it is an operand of the second product's matrix instructions and of B's gradient,
+// and half a step of it (BF16 2^-8) is that much of the adapter's part of y alone, beside y's own rounding.
 #include "hm_grouped.h"
 
 #include <limits.h>
