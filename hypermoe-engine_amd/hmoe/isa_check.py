@@ -88,6 +88,14 @@ def _functions(text: str, asm_flags: list | None = None
                     asm_flags.append(flags)
             name, ins, labels, flags = m.group(1), [], {}, []
             continue
+        if line.startswith(".Lfunc_end"):
+            # (not s_endpgm: blocks may follow it)
+            if name is not None:
+                out.append((name, ins, labels))
+                if asm_flags is not None:
+                    asm_flags.append(flags)
+            name, ins, labels, flags = None, [], {}, []
+            continue
         if line.endswith(":"):
             if name is not None:
                 labels[line[:-1]] = len(ins)
@@ -96,11 +104,6 @@ def _functions(text: str, asm_flags: list | None = None
             continue
         ins.append(line.replace(",", " ").split())
         flags.append(in_asm)
-        if ins[-1][0] == "s_endpgm":
-            out.append((name, ins, labels))
-            if asm_flags is not None:
-                asm_flags.append(flags)
-            name, ins, labels, flags = None, [], {}, []
     if name is not None and ins:
         out.append((name, ins, labels))
         if asm_flags is not None:
