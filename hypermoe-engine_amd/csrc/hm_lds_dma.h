@@ -45,12 +45,14 @@ __device__ __forceinline__ void lds_barrier_keep() {
 // reading a stage, lds_barrier before refilling a slot.  The statement sets
 // M0 itself, and the kernels hold nothing else in M0 (no LDS DMA through the
 // builtin, no indirect register indexing, no GWS or messages).  The memory
-// clobber keeps other memory accesses on their side of the load.
+// clobber keeps other memory accesses on their side of the load.  s_nop: an
+// LDS load may follow a scalar write of M0 after one wait state, and nobody
+// else puts it there (hmoe.isa_check looks for it).
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void dma16(const void* gsrc, void* lds_base) {
     const unsigned m0 = (unsigned)(uintptr_t)(lds_ptr_t)lds_base;
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off"
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
                  :: "v"(gsrc), "s"(m0) : "memory", "m0");
 }
 // The same with 4 bytes per lane: lane l's dword lands at lds_base + 4*l.
@@ -58,18 +60,18 @@ __device__ __forceinline__ void dma16(const void* gsrc, void* lds_base) {
 // same in-order load queue as the operand stages.
 __device__ __forceinline__ void dma4(const void* gsrc, void* lds_base) {
     const unsigned m0 = (unsigned)(uintptr_t)(lds_ptr_t)lds_base;
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off"
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
                  :: "v"(gsrc), "s"(m0) : "memory", "m0");
 }
 // dma16 and dma4 from a uniform base plus a 32-bit byte offset per lane.
 __device__ __forceinline__ void dma16_off(const void* base, uint32_t off, void* lds_base) {
     const unsigned m0 = (unsigned)(uintptr_t)(lds_ptr_t)lds_base;
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                  :: "v"(off), "s"(base), "s"(m0) : "memory", "m0");
 }
 __device__ __forceinline__ void dma4_off(const void* base, uint32_t off, void* lds_base) {
     const unsigned m0 = (unsigned)(uintptr_t)(lds_ptr_t)lds_base;
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1"
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1"
                  :: "v"(off), "s"(base), "s"(m0) : "memory", "m0");
 }
 // dma16 through a buffer descriptor: the same, and a lane whose offset is at or past HM_BUF_RANGE reads
@@ -83,7 +85,7 @@ __device__ __forceinline__ hm_buf make_buf(const void* base) {
 }
 __device__ __forceinline__ void dma16_buf(hm_buf buf, uint32_t off, void* lds_base) {
     const unsigned m0 = (unsigned)(uintptr_t)(lds_ptr_t)lds_base;
-    asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
                  :: "v"(off), "s"(buf), "s"(m0) : "memory", "m0");
 }
 #pragma clang diagnostic pop

@@ -39,6 +39,15 @@ Three further rules guard the hand-written blocks (between the compiler's
 - Accumulator of a chain.  The FP64 chains (csrc/hm_router.hip, hm_chain64)
   write their accumulator at every step and read their terms until the last
   one, so no term may share a register with the accumulator.
+
+And the wait states that the hardware leaves to software.  The compiler puts
+them between its own instructions and does not look into the blocks
+(check_waits):
+
+- a scalar write of M0, one wait state, an LDS-DMA load (what the compiler
+  keeps around its own such loads);
+- a vector instruction's write of a scalar register (v_readfirstlane and the
+  like), five wait states, a vector memory instruction that reads it.
 """
 from __future__ import annotations
 
@@ -218,8 +227,71 @@ def check_text(text: str) -> list[str]:
     return problems
 
 
+# a vector instruction's scalar destination: the operand it is
+_VALU_SDST = ((re.compile(r"^v_(readfirstlane|readlane|cmp)"), 1),
+              (re.compile(r"^v_(add|sub|subrev|addc|subb|subbrev)_co_|^v_(mad_[ui]64|div_scale)"), 2))
+
+
+def _sregs(op: str) -> set[int]:
+    m = re.match(r"s\[(\d+):(\d+)\]$", op)
+    if m:
+        return set(range(int(m.group(1)), int(m.group(2)) + 1))
+    m = re.match(r"s(\d+)$", op)
+    return {int(m.group(1))} if m else set()
+
+
+def _writes(u: list[str]) -> tuple[set[int], bool]:
+    """Scalar registers that a vector instruction writes; whether a scalar one writes M0."""
+    if u[0].startswith("s_"):
+        return set(), len(u) > 1 and u[1] == "m0"
+    for form, at in _VALU_SDST:
+        if form.match(u[0]) and len(u) > at:
+            return _sregs(u[at]), False
+    return set(), False
+
+
+def _check_waits(ins: list[list[str]], labels: dict[str, int], flags: list[bool]) -> list[tuple[int, str]]:
+    before: list[list[int]] = [[] for _ in ins]
+    for i, (_, _, _, succ, _) in enumerate(_decode(ins, labels)):
+        for n in succ:
+            if n < len(ins):
+                before[n].append(i)
+    bad = []
+    for i, (u, in_asm) in enumerate(zip(ins, flags)):
+        if not in_asm or not _VMEM.match(u[0]):
+            continue
+        lds = "lds" in u[1:] or "_lds_" in u[0]
+        read = set().union(*(_sregs(o) for o in u[1:]))
+        stack, seen = [(b, 0) for b in before[i]], set()   # (instruction, wait states between it and the load)
+        while stack:
+            j, states = stack.pop()
+            if states >= 5 or (j, states) in seen:
+                continue
+            seen.add((j, states))
+            scalars, m0 = _writes(ins[j])
+            if lds and m0 and states < 1:
+                bad.append((i, "no wait state after the write of M0"))
+            if scalars & read:
+                bad.append((i, f"reads a scalar register {states} wait states after {' '.join(ins[j])}"))
+            states += int(ins[j][1], 0) + 1 if ins[j][0] == "s_nop" else 1
+            stack += [(b, states) for b in before[j]]
+    return bad
+
+
+def check_waits(text: str) -> list[str]:
+    """Vector memory instructions of hand-written blocks that come too early after the write of a scalar
+    register that they read, one line each (empty: clean)."""
+    problems = []
+    flags: list[list[bool]] = []
+    for (name, ins, labels), fl in zip(_functions(text, flags), flags):
+        for i, what in _check_waits(ins, labels, fl):
+            problems.append(f"{name}: instruction #{i} ({' '.join(ins[i])}): {what}")
+    return problems
+
+
 def check_file(path: str | Path) -> list[str]:
-    return check_text(Path(path).read_text())
+    text = Path(path).read_text()
+    return check_text(text) + check_waits(text)
 
 
 if __name__ == "__main__":
