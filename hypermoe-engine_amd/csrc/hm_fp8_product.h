@@ -119,15 +119,17 @@ struct Tile {
     int e;
     int64_t row0, nrows;
 };
-// Every lane of the wave must be active.  False past the last tile; rows stays inside [0, rows).
+// Every lane of the wave must be active.  False past the last tile; offsets are cut to [0, rows] before anything
+// is counted, so that a last one of 2^31 - 1 does not take a count past 31 bits.
 __device__ __forceinline__ bool locate(const int32_t* __restrict__ offsets, int experts, int64_t rows,
                                        int bm, int64_t tile, Tile* t) {
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, top = (int)min(rows, (int64_t)0x7fffffff);
     int64_t base = 0;
     for (int c0 = 0; c0 < experts; c0 += 64) {
-        const int e = c0 + lane;
-        const int n = e < experts ? offsets[e + 1] - offsets[e] : 0;
-        const int64_t tiles = (n + bm - 1) / bm;
+        const int e = min(c0 + lane, experts - 1);
+        const int from = offsets[e], to = offsets[e + 1];   // (both in one round trip: no branch between them)
+        const int lo = max(0, min(from, top)), hi = max(lo, min(to, top));
+        const int64_t tiles = c0 + lane < experts ? ((uint32_t)(hi - lo) + (uint32_t)bm - 1) / (uint32_t)bm : 0;
         int64_t incl = tiles;
 #pragma unroll
         for (int sft = 1; sft < 64; sft <<= 1) {
@@ -139,9 +141,9 @@ __device__ __forceinline__ bool locate(const int32_t* __restrict__ offsets, int 
             const int first = __ffsll((long long)__ballot(base + incl > tile)) - 1;
             const int64_t in = tile - base - __shfl(incl - tiles, first, 64);
             t->e = c0 + first;
-            t->row0 = offsets[t->e] + in * bm;
+            t->row0 = max(0, offsets[t->e]) + in * bm;
             t->nrows = min((int64_t)bm, min((int64_t)offsets[t->e + 1], rows) - t->row0);
-            return t->row0 >= 0 && t->nrows > 0;
+            return t->nrows > 0;
         }
         base += total;
     }
