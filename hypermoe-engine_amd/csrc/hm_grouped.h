@@ -177,26 +177,6 @@ __device__ __forceinline__ int wave_min(int v) {
                min(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
 
-// Result (row, c) of a projection with adapters by its definition, in FP32.  Rows share a tile's stages with rows of other
-// adapters, whose mid is 0 for them, but 0 times an infinity or a NaN of another adapter's matrix is NaN.  So a result that
-// is not finite, in a tile that names another adapter than the row's own, is taken again here: slowly, and seldom.
-template <typename T, bool WK>
-__device__ __forceinline__ float adapter_result(const GProduct& p, int64_t row, int64_t c) {
-    const T *x = static_cast<const T*>(p.x) + row * p.K, *w = static_cast<const T*>(p.w) + (WK ? c * p.K : c);
-    const int64_t step = WK ? 1 : p.N;
-    float v = 0.0f;
-#pragma unroll 1
-    for (int64_t k = 0; k < p.K; ++k) v = __builtin_fmaf((float)x[k], (float)w[k * step], v);
-    const int a = p.ids[row];
-    if (a >= 0 && a < p.adapters) {
-        const T* mid = static_cast<const T*>(p.mid) + row * p.rank;
-        const T* up = static_cast<const T*>(p.up) + (int64_t)a * p.N * p.rank + (WK ? c * p.rank : c);
-#pragma unroll 1
-        for (int64_t r = 0; r < p.rank; ++r) v = __builtin_fmaf((float)mid[r], (float)up[r * step], v);
-    }
-    return v;
-}
-
 // Whether two arrays of so many bytes share memory.
 static inline bool hm_overlap(const void* a, int64_t na, const void* b, int64_t nb) {
     const uint64_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);

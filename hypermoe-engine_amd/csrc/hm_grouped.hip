@@ -100,8 +100,10 @@ __global__ __launch_bounds__(kThreads) void grouped_generic_kernel(GProduct p) {
     w += KIND == G_WEIGHT_GRAD ? 0 : (int64_t)e * p.w_group;
 
     v4f acc[2][2] = {};
-    int named = 0;   // adapters that the tile's rows name
-    auto step = [&]() __attribute__((always_inline)) {
+    int at[2];   // the adapters of the lane's rows
+    // `own`: of an adapter's step, whose rows alone take it: the others' operand is zeros, but 0 times an infinity or a NaN
+    // of the adapter's matrix is NaN
+    auto step = [&](int own) __attribute__((always_inline)) {
         __syncthreads();
         v8 a[2], b[2];
 #pragma unroll
@@ -112,7 +114,10 @@ __global__ __launch_bounds__(kThreads) void grouped_generic_kernel(GProduct p) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) acc[i][j] = Elem16<T>::mfma(a[j], b[i], acc[i][j]);
+            for (int j = 0; j < 2; ++j) {
+                const v4f r = Elem16<T>::mfma(a[j], b[i], acc[i][j]);
+                acc[i][j] = own < 0 || at[i] == own ? r : acc[i][j];
+            }
         __syncthreads();
     };
     // the row of x of tile row r
@@ -141,7 +146,7 @@ __global__ __launch_bounds__(kThreads) void grouped_generic_kernel(GProduct p) {
             sw.load_k(mine ? w + k * p.N : nullptr, n0 + 8 * (t & 7), p.N);
             sx.store(s_x);
             sw.store(s_w);
-            step();
+            step(-1);
         }
     } else {
         bool up;
@@ -159,11 +164,13 @@ __global__ __launch_bounds__(kThreads) void grouped_generic_kernel(GProduct p) {
             }
             sx.store(s_x);
             sw.store(s_w);
-            step();
+            step(-1);
         }
         if constexpr (KIND == G_ADAPTER) {
             const T* mid = static_cast<const T*>(p.mid);
             const int mine = lane < nrows ? p.ids[row0 + lane] : -1;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) at[i] = __shfl(mine, 32 * wm + 16 * i + i16, 64);
             int cur = -1;
             while (true) {
                 // the next adapter of these rows (the same in every wave)
@@ -172,7 +179,6 @@ __global__ __launch_bounds__(kThreads) void grouped_generic_kernel(GProduct p) {
                 for (int m = 32; m >= 1; m >>= 1) next = min(next, __shfl_xor(next, m, 64));
                 if (next == INT_MAX) break;
                 cur = next;
-                ++named;
                 const T* upm = static_cast<const T*>(p.up) + (int64_t)cur * p.N * p.rank;
                 const int r = t >> 2;
                 const bool take = __shfl(mine, r & 63, 64) == cur && r < nrows;
@@ -188,7 +194,7 @@ __global__ __launch_bounds__(kThreads) void grouped_generic_kernel(GProduct p) {
                     }
                     sx.store(s_x);
                     sw.store(s_w);
-                    step();
+                    step(cur);
                 }
             }
         }
@@ -225,11 +231,7 @@ __global__ __launch_bounds__(kThreads) void grouped_generic_kernel(GProduct p) {
                     O* y = static_cast<O*>(p.y) + ((int64_t)e * p.M + row) * p.N + c;
                     *y = (O)(acc[i][j][v] + (p.accumulate ? (float)*y : 0.0f));
                 } else {
-                    float r = acc[i][j][v];
-                    if constexpr (KIND == G_ADAPTER) {
-                        if (named && r * 0.0f != 0.0f) r = adapter_result<T, WK>(p, row, c);
-                    }
-                    static_cast<O*>(p.y)[row * p.N + c] = (O)r;
+                    static_cast<O*>(p.y)[row * p.N + c] = (O)acc[i][j][v];
                 }
             }
     }

@@ -552,7 +552,8 @@ int hm_grouped_weight_grad(const void* dy, const void* x, int32_t dtype,
  * dw_dtype and workspace as F4's.  mid and y must not overlap anything.  Rank
  * up to 256, up to 65535 adapters and 2^23 - 1 rows.
  * Rows of one adapter side by side are fastest.  An infinity or a NaN in an
- * adapter's matrices reaches the rows of that adapter only. */
+ * adapter's matrices reaches the rows of that adapter only: others have the
+ * bits that they have without it, at up to some 25 times the call's time. */
 #define HM_ADAPTER_MAX_RANK 256
 int hm_adapter_matmul(const void* x, int32_t dtype, const void* w,
                       int32_t w_transposed, const void* down, const void* up,
