@@ -685,7 +685,8 @@ __global__ __launch_bounds__(64 * WMC * WNC, 2) void g_tile_kernel(GProduct p) {
             }
         }
     };
-    // memory instructions of the results at least, where this wave's rows and columns are whole
+    // memory instructions of the results at least, where this wave's rows and columns are whole and nothing is asked for
+    // that may be left out (pre, z, what is added to): 16 bytes a lane are the most that one of them moves
     constexpr int STORES = XF * (GU ? SH / 2 : KIND == G_SWIGLU_GRAD ? 4 * SH / 2 : (int)sizeof(O) / 2 * SH / 2);
     auto whole = [&](const TileAt& t) __attribute__((always_inline)) {
         return t.nrows >= (wm + 1) * 16 * XF && t.n0 + TN <= N;
