@@ -77,8 +77,8 @@ __device__ __forceinline__ v4f block_product(const Frag<true>& a, const Frag<tru
     return c;
 }
 
-// g / (1 + e^-g) on the exponential and reciprocal units, a unit in the last place each (below g = -87, where
-// it is under 3e-37 in size, 0).
+// g / (1 + e^-g) on the exponential and reciprocal units, a unit in the last place each, and for negative g |g| / 2 units
+// of the exponent's rounding (below g = -87, where it is under 3e-37 in size, 0).
 __device__ __forceinline__ float fast_silu(float g) {
     return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896f));
 }

@@ -65,8 +65,9 @@ struct GProduct {
 
 // The SwiGLU's gradient for one value: dz, gate and up to the gradients of both, and z.
 __device__ __forceinline__ void swiglu_grad(float dz, float g, float u, float* dg, float* du, float* z) {
-    // s = 1 / (1 + e^-g) on the exponential and reciprocal units, within two units in the last place; e^-g
-    // is infinite below g = -88.7, s then 0, and g s too
+    // s = 1 / (1 + e^-g) on the exponential and reciprocal units, a unit in the last place each; the exponent g log2 e is
+    // rounded to FP32 before, which is |g| 2^-24 of e^-g, so for negative g |g| / 2 units of s besides (10 at -20, 40 at
+    // -80).  Below g = -87, where it is under 2e-38, s is 0, and g s too
     const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504088896f));
     const float a = g * s;
     *du = dz * a;
