@@ -64,7 +64,7 @@ __global__ __launch_bounds__(kThreads) void adapter_mid_rows_kernel(const T* __r
     }
 }
 
-// More rows: a workgroup takes 16 MT rows and 16 RF ranks, its 8 waves k in parts of 64, straight from memory into
+// More rows: a workgroup takes 16 rows and 16 RF ranks, its 8 waves k in parts of 64, straight from memory into
 // fragments (x is read once; the adapters' matrices, read by every workgroup, stay in the L2 and bound it); once for
 // each adapter that the rows name, its own rows kept.  The waves' sums meet in the LDS in wave order.
 constexpr int kMidWaves = 8;
@@ -77,23 +77,17 @@ __global__ __launch_bounds__(64 * kMidWaves, 2) void adapter_mid_tile_kernel(con
                                                                           int adapters, int rank, int64_t rows,
                                                                           int64_t K, T* __restrict__ mid) {
     typedef typename Elem16<T>::v8 v8;
-    constexpr int MT = 1, kPart = 64 * kMidWaves;
-    __shared__ v4f s_part[kMidWaves][MT * RF][64];
+    constexpr int kPart = 64 * kMidWaves;
+    __shared__ v4f s_part[kMidWaves][RF][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i16 = lane & 15, g = lane >> 4;
-    const int64_t row0 = (int64_t)blockIdx.x * 16 * MT;
+    const int64_t row0 = (int64_t)blockIdx.x * 16, row = row0 + i16;
     const int r0 = (int)blockIdx.y * 16 * RF;
-    int mine[MT];
-    const T* xr[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int64_t row = row0 + 16 * i + i16;
-        mine[i] = row < rows ? ids[row] : -1;
-        if (mine[i] >= adapters) mine[i] = -1;
-        xr[i] = x + min(row, rows - 1) * K;
-    }
+    int mine = row < rows ? ids[row] : -1;
+    if (mine >= adapters) mine = -1;
+    const T* xr = x + min(row, rows - 1) * K;
     // rows without adapter
-    for (int q = threadIdx.x; q < 16 * MT * 16 * RF; q += 64 * kMidWaves) {
+    for (int q = threadIdx.x; q < 16 * 16 * RF; q += 64 * kMidWaves) {
         const int r = r0 + q % (16 * RF), m = q / (16 * RF);
         if (row0 + m >= rows || r >= rank) continue;
         const int id = ids[row0 + m];
@@ -101,25 +95,21 @@ __global__ __launch_bounds__(64 * kMidWaves, 2) void adapter_mid_tile_kernel(con
     }
     int cur = -1;
     while (true) {
-        int next = INT_MAX;
-#pragma unroll
-        for (int i = 0; i < MT; ++i) next = min(next, mine[i] > cur ? mine[i] : INT_MAX);
-        cur = wave_min(next);
+        cur = wave_min(mine > cur ? mine : INT_MAX);
         if (cur == INT_MAX) break;
         const T* d = down + (int64_t)cur * rank * K;
-        v4f acc[MT][RF] = {};
+        v4f acc[RF] = {};
         int64_t k0 = 64 * wave;
         // U parts at a time, all their loads in flight; `whole`: within K
         auto parts = [&](auto u_, bool whole) __attribute__((always_inline)) {
             constexpr int U = decltype(u_)::value;
-            v8 xf[U][2][MT], df[U][2][RF];
+            v8 xf[U][2], df[U][2][RF];
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int64_t k = k0 + kPart * u + 32 * h + 8 * g, n = whole ? 8 : K - k;
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) xf[u][h][i] = load_frag8<T>(xr[i] + k, n);
+                    xf[u][h] = load_frag8<T>(xr + k, n);
 #pragma unroll
                     for (int f = 0; f < RF; ++f) {
                         const int r = min(r0 + 16 * f + i16, rank - 1);   // (ranks past the last are dropped)
@@ -138,32 +128,26 @@ __global__ __launch_bounds__(64 * kMidWaves, 2) void adapter_mid_tile_kernel(con
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < MT; ++i)
-#pragma unroll
-                        for (int f = 0; f < RF; ++f)
-                            acc[i][f] = Elem16<T>::mfma(df[u][h][f], xf[u][h][i], acc[i][f]);
+                    for (int f = 0; f < RF; ++f) acc[f] = Elem16<T>::mfma(df[u][h][f], xf[u][h], acc[f]);
             k0 += kPart * U;
         };
         constexpr int U = KM ? 4 : 2;
         while (k0 + kPart * (U - 1) + 64 <= K) parts(std::integral_constant<int, U>{}, true);
         while (k0 < K) parts(std::integral_constant<int, 1>{}, false);
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int f = 0; f < RF; ++f) s_part[wave][i * RF + f][lane] = acc[i][f];
+        for (int f = 0; f < RF; ++f) s_part[wave][f][lane] = acc[f];
         __syncthreads();
-        // entry (i, f, lane): row 16 i + i16, ranks 4 g .. of fragment f; a wave each
-        if (wave < MT * RF) {
-            const int i = wave / RF, f = wave % RF;
+        // entry (f, lane): row i16, ranks 4 g .. of fragment f; a wave each
+        if (wave < RF) {
             v4f v = s_part[0][wave][lane];
 #pragma unroll
             for (int w = 1; w < kMidWaves; ++w) v += s_part[w][wave][lane];
-            if (mine[MT == 1 ? 0 : i] == cur) {
+            if (mine == cur) {
                 const float s = scale[cur];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int r = r0 + 16 * f + 4 * g + j;
-                    if (r < rank) mid[(row0 + 16 * i + i16) * rank + r] = (T)(s * v[j]);
+                    const int r = r0 + 16 * wave + 4 * g + j;
+                    if (r < rank) mid[row * rank + r] = (T)(s * v[j]);
                 }
             }
         }

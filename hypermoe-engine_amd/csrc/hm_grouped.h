@@ -189,8 +189,8 @@ int hm_g_launch_generic(GKind kind, bool w_kmajor, int32_t dtype, int32_t y_dtyp
 // these three for operands aligned to 16 bytes throughout; 32: of 128 x 128 for others.
 int hm_g_launch_tiles_f16(GKind kind, int form, bool w_kmajor, bool f32, const GProduct& p, hipStream_t s);
 int hm_g_launch_tiles_bf16(GKind kind, int form, bool w_kmajor, bool f32, const GProduct& p, hipStream_t s);
-// The kernel for few rows (hm_grouped_stream.hip): x w^T, SwiGLU or adapters, 16 mt rows a workgroup (1, 2, 4; 8 but
-// for SwiGLU).
+// The kernel for few rows (hm_grouped_stream.hip): x w^T, SwiGLU or adapters, 16 mt rows a workgroup (1, 2, 4; 8 for
+// adapters).
 int hm_g_launch_stream(GKind kind, int mt, int32_t dtype, bool f32, const GProduct& p, hipStream_t s);
 // The kernel that a product's sizes and alignment ask for (hm_grouped.hip).
 int hm_g_launch(GKind kind, bool w_kmajor, int32_t dtype, int32_t y_dtype, const GProduct& p, hipStream_t s);

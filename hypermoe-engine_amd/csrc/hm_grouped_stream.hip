@@ -171,7 +171,7 @@ int launch(int mt, const GProduct& p, hipStream_t s) {
     if (mt == 1) kp == 8 ? run(g_stream_kernel<T, O, KIND, 1, 8>) : run(g_stream_kernel<T, O, KIND, 1, 2>);
     else if (mt == 2) kp == 8 ? run(g_stream_kernel<T, O, KIND, 2, 8>) : run(g_stream_kernel<T, O, KIND, 2, 2>);
     else if (mt == 4) kp == 8 ? run(g_stream_kernel<T, O, KIND, 4, 8>) : run(g_stream_kernel<T, O, KIND, 4, 2>);
-    else if constexpr (KIND != G_SWIGLU) run(g_stream_kernel<T, O, KIND, 8, 8>);
+    else if constexpr (KIND == G_ADAPTER) run(g_stream_kernel<T, O, KIND, 8, 8>);
     HM_LAUNCHED();
     return HM_OK;
 }

@@ -37,7 +37,6 @@
 namespace {
 
 constexpr int kXcds = 8;
-constexpr int kThreads = 256;
 constexpr int kSuper = 4;
 constexpr int KB = 64;
 
@@ -804,15 +803,18 @@ int launch(const GProduct& p, hipStream_t s) {
 
 template <int WMC, int WNC, int XF, int WF, int NS, bool DMA, typename T>
 int launch_kind(GKind kind, bool wk, bool f32, const GProduct& p, hipStream_t s) {
+    constexpr int BM = 16 * XF * WMC, BN = 16 * WF * WNC;
 #define HM_G(KIND, WK, O) launch<WMC, WNC, XF, WF, NS, DMA, KIND, WK, T, O>(p, s)
     switch (kind) {
     case G_SWIGLU:
-        if constexpr (XF * WMC * 16 < 256 && WNC == 2) return HM_G(G_SWIGLU, true, T);
+        if constexpr (BM < 256 && WNC == 2) return HM_G(G_SWIGLU, true, T);
         break;   // (launch_tiles has their own)
     case G_SWIGLU_GRAD:
-        if constexpr (XF * WMC * 16 < 256) return HM_G(G_SWIGLU_GRAD, false, T);
+        if constexpr (BM < 256) return HM_G(G_SWIGLU_GRAD, false, T);
         break;   // (hm_grouped.hip asks for none)
-    case G_WEIGHT_GRAD: return f32 ? HM_G(G_WEIGHT_GRAD, false, float) : HM_G(G_WEIGHT_GRAD, false, T);
+    case G_WEIGHT_GRAD:
+        if constexpr (BM == BN) return f32 ? HM_G(G_WEIGHT_GRAD, false, float) : HM_G(G_WEIGHT_GRAD, false, T);
+        break;   // (nor for 128 x 256)
     case G_ADAPTER: return wk ? HM_G(G_ADAPTER, true, T) : HM_G(G_ADAPTER, false, T);
     case G_MATMUL:
         if (wk) return f32 ? HM_G(G_MATMUL, true, float) : HM_G(G_MATMUL, true, T);
