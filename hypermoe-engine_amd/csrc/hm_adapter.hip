@@ -352,10 +352,13 @@ __global__ __launch_bounds__(kThreads) void adapter_grad_join_kernel(const float
     }
 }
 
-// Parts that the rows are cut into: so many that about 512 workgroups share the work, 256 rows a part at least.
+// Parts that the rows are cut into: so many that about 512 workgroups share the work, 256 rows a part at least, and their
+// sums within 1 GB (each part holds every adapter's; with so many adapters those fill the chip, in turn, by themselves).
+constexpr int64_t kPartsBytes = (int64_t)1 << 30;
 int grad_parts(int64_t adapters, int64_t rows, int64_t L, int64_t R) {
     const int64_t tiles = ((L + kGT - 1) / kGT) * ((R + kGT - 1) / kGT);
-    return (int)std::max((int64_t)1, std::min(std::min((int64_t)512 / tiles, (rows + 255) / 256), (int64_t)64));
+    const int64_t most = std::min((int64_t)64, kPartsBytes / (4 * adapters * (L * R + 1)));
+    return (int)std::max((int64_t)1, std::min(std::min((int64_t)512 / tiles, (rows + 255) / 256), most));
 }
 
 template <typename T, typename O>

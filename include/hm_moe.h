@@ -549,8 +549,10 @@ int hm_grouped_weight_grad(const void* dy, const void* x, int32_t dtype,
  * hm_adapter_weight_grad: dw[a] = sum over the rows t with ids[t] = a of
  * left[t]^T right[t], [left_cols x right_cols]: A's gradient of the gradient of
  * mid and x, B's of dy and mid.  Zeros for an adapter without rows; accumulate,
- * dw_dtype and workspace as F4's.  mid and y must not overlap anything.  Rank
- * up to 256, up to 65535 adapters and 2^23 - 1 rows.
+ * dw_dtype and workspace as F4's (at most 1 GB); every adapter goes through
+ * the ids of all rows, so its time grows with adapters times rows.  mid and y
+ * must not overlap anything.  Rank up to 256, up to 65535 adapters and 2^23 - 1
+ * rows.
  * Rows of one adapter side by side are fastest.  An infinity or a NaN in an
  * adapter's matrices reaches the rows of that adapter only: others have the
  * bits that they have without it, at up to some 25 times the call's time. */
