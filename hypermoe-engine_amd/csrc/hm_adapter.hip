@@ -411,7 +411,9 @@ int hm_adapter_matmul(const void* x, int32_t dtype, const void* w, int32_t w_tra
                   nd = 2 * adapters * rank * inner, nu = 2 * adapters * rank * cols;
     HM_REQUIRE(!hm_overlap(y, ny, x, nx) && !hm_overlap(y, ny, w, nw) && !hm_overlap(y, ny, down, nd) &&
                !hm_overlap(y, ny, up, nu) && !hm_overlap(y, ny, mid, nm) && !hm_overlap(mid, nm, x, nx) &&
-               !hm_overlap(mid, nm, w, nw) && !hm_overlap(mid, nm, down, nd) && !hm_overlap(mid, nm, up, nu));
+               !hm_overlap(mid, nm, w, nw) && !hm_overlap(mid, nm, down, nd) && !hm_overlap(mid, nm, up, nu) &&
+               !hm_overlap(y, ny, scale, 4 * adapters) && !hm_overlap(mid, nm, scale, 4 * adapters) &&
+               !hm_overlap(y, ny, ids, 4 * rows) && !hm_overlap(mid, nm, ids, 4 * rows));
     const hipStream_t s = hm_stream(stream);
     const int rc = dtype == HM_DTYPE_FP16
                        ? launch_mid<hm_f16>(x, !w_transposed, down, scale, ids, (int)adapters, (int)rank, rows,
@@ -457,11 +459,13 @@ int hm_adapter_weight_grad(const void* left, const void* right, int32_t dtype, c
     HM_REQUIRE((rows == 0 || (left && right && ids)) && dw && aligned(left, 2) && aligned(right, 2) &&
                aligned(ids, 4) && aligned(dw, dw_dtype == HM_DTYPE_FP32 ? 4 : 2));
     const int64_t nw = adapters * left_cols * right_cols * (dw_dtype == HM_DTYPE_FP32 ? 4 : 2);
-    HM_REQUIRE(!hm_overlap(dw, nw, left, 2 * rows * left_cols) && !hm_overlap(dw, nw, right, 2 * rows * right_cols));
+    HM_REQUIRE(!hm_overlap(dw, nw, left, 2 * rows * left_cols) && !hm_overlap(dw, nw, right, 2 * rows * right_cols) &&
+               !hm_overlap(dw, nw, ids, 4 * rows));
     const size_t need = hm_adapter_weight_grad_workspace_bytes(adapters, rows, left_cols, right_cols);
     HM_REQUIRE(workspace_bytes >= need && (!need || (workspace && aligned(workspace, 4))));
     HM_REQUIRE(!need || (!hm_overlap(workspace, need, dw, nw) && !hm_overlap(workspace, need, left, 2 * rows * left_cols) &&
-                         !hm_overlap(workspace, need, right, 2 * rows * right_cols)));
+                         !hm_overlap(workspace, need, right, 2 * rows * right_cols) &&
+                         !hm_overlap(workspace, need, ids, 4 * rows)));
     const hipStream_t s = hm_stream(stream);
     auto run = [&](auto launcher) {
         return launcher(left, right, ids, adapters, rows, left_cols, right_cols, dw, accumulate, workspace, s);

@@ -358,7 +358,8 @@ int hm_grouped_matmul(const void* x, int32_t dtype, const void* w, int32_t w_tra
     HM_REQUIRE(x && w && offsets && y && aligned(x, 2) && aligned(w, 2) && aligned(offsets, 4) &&
                aligned(y, y_dtype == HM_DTYPE_FP32 ? 4 : 2));
     const int64_t ny = rows * cols * (y_dtype == HM_DTYPE_FP32 ? 4 : 2);
-    HM_REQUIRE(!hm_overlap(y, ny, x, 2 * rows * inner) && !hm_overlap(y, ny, w, 2 * groups * inner * cols));
+    HM_REQUIRE(!hm_overlap(y, ny, x, 2 * rows * inner) && !hm_overlap(y, ny, w, 2 * groups * inner * cols) &&
+               !hm_overlap(y, ny, offsets, 4 * (groups + 1)));
     GProduct p = {};
     p.x = x;
     p.w = w;
@@ -382,10 +383,12 @@ int hm_grouped_swiglu(const void* x, int32_t dtype, int64_t x_rows, const int32_
     if (rows == 0) return HM_OK;
     HM_REQUIRE(x && w && offsets && z && aligned(x, 2) && aligned(w, 2) && aligned(offsets, 4) &&
                aligned(perm_tokens, 4) && aligned(z, 2) && aligned(pre, 2));
-    const int64_t nz = 2 * rows * intermediate, nx = 2 * x_rows * hidden, nw = 4 * groups * hidden * intermediate;
+    const int64_t nz = 2 * rows * intermediate, nx = 2 * x_rows * hidden, nw = 4 * groups * hidden * intermediate,
+                  no = 4 * (groups + 1);
     HM_REQUIRE(!hm_overlap(z, nz, x, nx) && !hm_overlap(z, nz, w, nw) && !hm_overlap(z, nz, perm_tokens, 4 * rows) &&
                !hm_overlap(pre, 2 * nz, x, nx) && !hm_overlap(pre, 2 * nz, w, nw) &&
-               !hm_overlap(pre, 2 * nz, perm_tokens, 4 * rows) && !hm_overlap(z, nz, pre, 2 * nz));
+               !hm_overlap(pre, 2 * nz, perm_tokens, 4 * rows) && !hm_overlap(z, nz, pre, 2 * nz) &&
+               !hm_overlap(z, nz, offsets, no) && !hm_overlap(pre, 2 * nz, offsets, no));
     GProduct p = {};
     p.x = x;
     p.w = w;
@@ -410,10 +413,12 @@ int hm_grouped_swiglu_grad(const void* dy, int32_t dtype, const void* w, const v
     if (rows == 0) return HM_OK;
     HM_REQUIRE(dy && w && pre && offsets && dpre && aligned(dy, 2) && aligned(w, 2) && aligned(pre, 2) &&
                aligned(offsets, 4) && aligned(dpre, 2) && aligned(z, 2));
-    const int64_t nz = 2 * rows * intermediate, ny = 2 * rows * hidden, nw = 2 * groups * hidden * intermediate;
+    const int64_t nz = 2 * rows * intermediate, ny = 2 * rows * hidden, nw = 2 * groups * hidden * intermediate,
+                  no = 4 * (groups + 1);
     HM_REQUIRE(!hm_overlap(dpre, 2 * nz, dy, ny) && !hm_overlap(dpre, 2 * nz, w, nw) &&
                !hm_overlap(dpre, 2 * nz, pre, 2 * nz) && !hm_overlap(z, nz, dy, ny) && !hm_overlap(z, nz, w, nw) &&
-               !hm_overlap(z, nz, pre, 2 * nz) && !hm_overlap(z, nz, dpre, 2 * nz));
+               !hm_overlap(z, nz, pre, 2 * nz) && !hm_overlap(z, nz, dpre, 2 * nz) &&
+               !hm_overlap(dpre, 2 * nz, offsets, no) && !hm_overlap(z, nz, offsets, no));
     GProduct p = {};
     p.x = dy;
     p.w = w;
@@ -442,7 +447,8 @@ int hm_grouped_weight_grad(const void* dy, const void* x, int32_t dtype, const i
     HM_REQUIRE((rows == 0 || (dy && x)) && offsets && dw && aligned(dy, 2) && aligned(x, 2) &&
                aligned(offsets, 4) && aligned(dw, dw_dtype == HM_DTYPE_FP32 ? 4 : 2));
     const int64_t nw = groups * cols * inner * (dw_dtype == HM_DTYPE_FP32 ? 4 : 2);
-    HM_REQUIRE(!hm_overlap(dw, nw, dy, 2 * rows * cols) && !hm_overlap(dw, nw, x, 2 * rows * inner));
+    HM_REQUIRE(!hm_overlap(dw, nw, dy, 2 * rows * cols) && !hm_overlap(dw, nw, x, 2 * rows * inner) &&
+               !hm_overlap(dw, nw, offsets, 4 * (groups + 1)));
     if (workspace_bytes < hm_grouped_weight_grad_workspace_bytes(groups, rows, cols, inner)) return HM_ERR_INVALID;
     GProduct p = {};
     p.x = dy;
