@@ -318,6 +318,11 @@ static int pick(GKind kind, bool w_kmajor, const GProduct& p) {
     const bool nt = w_kmajor && kind != G_WEIGHT_GRAD;
     const int64_t groups = p.offsets ? p.groups : 1, each = (p.rows + groups - 1) / groups;
     if (nt && (each <= 16 || p.rows <= 64)) return (p.rows <= 16 || each <= 4 ? 1 : p.rows <= 32 || each <= 8 ? 2 : 4) << 16;
+    // Adapters of up to 128 rows: the stream kernel takes an adapter for each row as easily as one for all (the host does
+    // not know which), tiles take a stage more for every adapter: 128 rows, 2048 x 2048, rank 16, one adapter 31 us
+    // against 29 on tiles, one a row 33 against 184; rank 64 65 and 31, 72 and 192.  Beyond, rows of one adapter are
+    // taken to lie side by side: 256 rows, rank 16, one adapter 30 (streamed 31), one a row 186 (35); 512 rows 31 (58)
+    // and 249 (123).
     if (kind == G_ADAPTER && nt && p.rows <= 128) return 8 << 16;
     if (!tile_ok(kind, w_kmajor, p)) return 0;
     const bool wg = kind == G_WEIGHT_GRAD;
@@ -330,7 +335,8 @@ static int pick(GKind kind, bool w_kmajor, const GProduct& p) {
     if (m128 * ((p.N + wide - 1) / wide) < 256) return 64;
     // 256 x 256 from 384 rows a group on: 8 groups of 4096 rows, 2048 x 1536, 195 us against 219 of 128 x 256; but 128
     // of 256 rows on average, uneven, 182 and 157: half of the second tile of a group is empty.  Gate and up from 256 on
-    // (those groups 289 and 297).  The SwiGLU's gradient not at all: its results take more time than the matrix
+    // (those groups 289 and 297; even groups 32 x 272 rows 87 and 90, 32 x 512 93 and 96, but 64 x 256 131 and 120, and
+    // below it 64 x 240 140 and 125).  The SwiGLU's gradient not at all: its results take more time than the matrix
     // instructions, and 128 x 256 tiles spread them better (8 groups of 4096 rows, 2048 x 768, 171 us and 157).
     if (kind == G_SWIGLU_GRAD) return 128;
     return wg || each >= (kind == G_SWIGLU ? 256 : 384) ? 256 : 128;

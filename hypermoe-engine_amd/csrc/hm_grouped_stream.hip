@@ -5,7 +5,7 @@
 // times 16 columns of up to 16 MT rows of one group; KP waves share the k of 16 columns by 64 in turn, straight from
 // memory into fragments (128 bytes of each of 16 rows of w), no LDS and no barrier before their sums meet, in wave
 // order.  x's rows come from the caches.
-// Bound by the weights' bytes: 16 tokens, top-8 of 128 experts, 2048 x 768 matrices, 48 us (260 MB, 5.4 TB/s; all eight
+// Bound by the weights' bytes: 16 tokens, top-8 of 128 experts, 2048 x 768 matrices, 50 us (260 MB, 5.2 TB/s; all eight
 // waves on 16 columns 83).  At one token by latency: gate and up 13.4 us (50 MB).
 #include "hm_grouped.h"
 

@@ -19,10 +19,11 @@
 //                     in turn; within a group m-tiles by kSuper, so what is read by several workgroups at once is in
 //                     one L2 (128 groups of 256 rows, 2048 x 1536: 279 us; each workgroup a range of its own: 418).
 //
-// Bound by memory where groups are of some 256 rows (their weights are read for few products), by the matrix
-// instructions and the clock that they leave otherwise: 8192 x 8192 x 8192 to BF16 780 us, 1.41 PFLOP/s (the library's
-// product 1.45); 8 groups of 4096 rows, gate and up of 2048 x 768 with SwiGLU 165 us, 1.25 PFLOP/s; 128 groups of 256 rows
-// 218 us, 4 TB/s, and their weight gradients (805 MB of results) 281 us.  Off 16 bytes, 16 groups of 512 rows, 1001 x
+// Between memory and the matrix instructions where groups are of some 256 rows (their weights are read for few products),
+// bound by the matrix instructions and the clock that they leave otherwise: 8192 x 8192 x 8192 to BF16 780 us, 1.41
+// PFLOP/s (the library's product 1.45); 8 groups of 4096 rows, gate and up of 2048 x 768 with SwiGLU 165 us, 1.25 PFLOP/s;
+// 128 groups of 256 rows 218 us, 4 TB/s (165 at the rate of reads, 137 by operations; without the results 204), and their
+// weight gradients (805 MB of results) 281 to 293 us (without the results 192).  Off 16 bytes, 16 groups of 512 rows, 1001 x
 // 1333: 70 us, 310 TFLOP/s, where a stage waits for the one that the registers hold.
 #pragma once
 

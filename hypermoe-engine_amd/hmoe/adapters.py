@@ -8,7 +8,7 @@
 
 w [N, K], a [adapters, rank, K], b [adapters, N, rank] float16 or bfloat16, scale [adapters] float32, ids [rows]
 int32 (outside 0 .. adapters - 1: a row without adapter).  Calls go to the current stream of the operands'
-device; the gradients are plain functions.
+device; the gradients are plain functions, and no result has an autograd history.
 """
 from __future__ import annotations
 

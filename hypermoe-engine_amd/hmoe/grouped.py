@@ -11,7 +11,7 @@
 
 Operands are float16 or bfloat16, sums FP32.  Calls go to the current stream of the operands' device; results
 are new tensors unless given.  The backward passes are plain functions, so a training step captured into a
-graph holds no autograd state of an eager one.
+graph holds no autograd state of an eager one; no result has an autograd history.
 """
 from __future__ import annotations
 
